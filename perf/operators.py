@@ -1,0 +1,549 @@
+"""The operators between a layer's q / k / v projections and its output projection, one
+pass each: pages and slots for a step's tokens, rotary positions, the cache write and the
+attention of single new tokens over the paged cache.
+
+A case names an operator and its sizes.  `prepare` makes what a program holds before the
+call (the cache, tables, activations and output buffers on the GPU, all values from the
+seed; request lengths belong to the case), `run` makes one pass, in elementary torch
+operations or, with `own` set, through openmini_qmm; `work` counts the bytes and
+operations the result cannot do without; `exact` gives the results in 64 bits from the
+operators' definitions.
+
+  plan    block tables and slot maps from request lengths (whole numbers throughout)
+  rope    rotary positions with one to three axes on a dense [tokens, heads, dim] tensor,
+          forward or inverse (the inverse is the gradient)
+  append  the same on a step's q and k, with k and v written to their cache slots
+  attn    attention of one query token a row over a paged cache
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+_PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "openmini-v1_amd")
+_FLOAT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "f8": torch.float8_e4m3fn}
+_SIZE = {"f32": 4, "f16": 2, "bf16": 2, "f8": 1}
+_F8_MOST = 448.0  # the largest e4m3 value
+
+
+def _qmm():
+    if _PKG not in sys.path:
+        sys.path.insert(0, _PKG)
+    import openmini_qmm
+    openmini_qmm.init(torch.cuda.current_device())
+    return openmini_qmm
+
+
+def listed():
+    return [
+        # One conversation takes its next token: the smallest call of a decode step.
+        {"name": "plan_one", "op": "plan", "requests": 1, "cached": 1000, "new": 1, "prompts": 0, "page": 16, "spare": 8},
+        # A step of a full server: 240 decoding requests and 16 prompts of up to 4096 tokens.
+        {"name": "plan_mixed_256", "op": "plan", "requests": 256, "cached": 8000, "new": 4096, "prompts": 16, "page": 16,
+         "spare": 4096},
+        # Queries of one text token, one axis.
+        {"name": "rope_text_1", "op": "rope", "tokens": 1, "heads": 32, "dim": 128, "rot": 128, "axes": 1, "order": "blocks",
+         "pairing": "halves", "in": "bf16", "out": "bf16", "inverse": False, "offset": 5000},
+        # A video of 16 frames of 24 x 42 patches, three axes, fp32 projections to bf16.
+        {"name": "rope_video_16k", "op": "rope", "tokens": 16128, "heads": 16, "dim": 128, "rot": 128, "axes": 3,
+         "order": "cycled", "pairing": "halves", "in": "f32", "out": "bf16", "inverse": False, "offset": 100},
+        # A 70B layer's step for one request.
+        {"name": "append_70b_1", "op": "append", "tokens": 1, "heads": 64, "kv_heads": 8, "dim": 128, "rot": 128, "axes": 1,
+         "order": "blocks", "pairing": "halves", "in": "f32", "q": "bf16", "cache": "bf16", "page": 16, "layout": "token"},
+        # The same for 200 requests decoded together, e4m3 cache.
+        {"name": "append_70b_200_f8", "op": "append", "tokens": 200, "heads": 64, "kv_heads": 8, "dim": 128, "rot": 128,
+         "axes": 1, "order": "blocks", "pairing": "halves", "in": "f32", "q": "bf16", "cache": "f8", "page": 32,
+         "layout": "token"},
+        # A prompt of 8191 tokens (images among them: three axes) through a 7B layer.
+        {"name": "append_7b_8191", "op": "append", "tokens": 8191, "heads": 32, "kv_heads": 32, "dim": 128, "rot": 128,
+         "axes": 3, "order": "blocks", "pairing": "halves", "in": "f32", "q": "f16", "cache": "f16", "page": 16,
+         "layout": "head"},
+        # One short conversation, 70B heads: the smallest attention call.
+        {"name": "attn_70b_r1_300", "op": "attn", "rows": 1, "least": 300, "most": 300, "heads": 64, "kv_heads": 8, "dim": 128,
+         "page": 16, "cache": "bf16", "q": "bf16", "out": "f32", "window": 0, "layout": "token", "empty": 0},
+        # One conversation over a long document, length not a multiple of anything.
+        {"name": "attn_70b_r1_131071", "op": "attn", "rows": 1, "least": 131071, "most": 131071, "heads": 64, "kv_heads": 8,
+         "dim": 128, "page": 16, "cache": "bf16", "q": "bf16", "out": "bf16", "window": 0, "layout": "token", "empty": 0},
+        # Sixteen requests on a 7B layer (a key head for each query head), f16, output for the fp32 projection.
+        {"name": "attn_7b_r16_f16", "op": "attn", "rows": 16, "least": 700, "most": 2100, "heads": 32, "kv_heads": 32,
+         "dim": 128, "page": 32, "cache": "f16", "q": "f16", "out": "f32", "window": 0, "layout": "head", "empty": 0},
+        # Sixty-four ragged requests, heads of 64, a sliding window, two rows of padding.
+        {"name": "attn_d64_r64_window", "op": "attn", "rows": 64, "least": 50, "most": 16000, "heads": 32, "kv_heads": 4,
+         "dim": 64, "page": 16, "cache": "bf16", "q": "bf16", "out": "bf16", "window": 4096, "layout": "token", "empty": 2},
+        # A full server on a 70B layer with an e4m3 cache: the largest.
+        {"name": "attn_70b_r128_f8", "op": "attn", "rows": 128, "least": 2000, "most": 12000, "heads": 64, "kv_heads": 8,
+         "dim": 128, "page": 64, "cache": "f8", "q": "bf16", "out": "bf16", "window": 0, "layout": "token", "empty": 0},
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number in [lo, hi], spread over the logarithm."""
+    return max(lo, min(hi, int(round(lo * (hi / lo) ** rng.random()))))
+
+
+def _rotary(rng, dim):
+    axes = rng.choice([1, 1, 3])
+    return {"rot": rng.choice([dim, dim, dim // 2]), "axes": axes, "order": rng.choice(["blocks", "cycled"]),
+            "pairing": rng.choice(["halves", "halves", "adjacent"])}
+
+
+def draw(rng):
+    op = rng.choice(["plan", "rope", "append", "append", "attn", "attn", "attn", "attn"])
+    if op == "plan":
+        requests = _spread(rng, 1, 1500)
+        prompts = min(requests, rng.choice([0, 1, 4, 16]))
+        return {"op": op, "requests": requests, "cached": _spread(rng, 1, 20000), "new": _spread(rng, 2, 4096), "prompts": prompts,
+                "page": rng.choice([8, 16, 17, 64, 256]), "spare": _spread(rng, 4, 20000)}
+    if op == "rope":
+        dim = rng.choice([64, 96, 128, 256])
+        heads = _spread(rng, 1, 64)
+        return {"op": op, "tokens": _spread(rng, 1, min(16000, 33000000 // (heads * dim))), "heads": heads, "dim": dim,
+                **_rotary(rng, dim), "in": rng.choice(["f32", "bf16", "f16"]), "out": rng.choice(["bf16", "f16"]),
+                "inverse": rng.random() < 0.3, "offset": _spread(rng, 1, 30000)}
+    if op == "append":
+        dim = rng.choice([64, 96, 128, 128, 256])
+        kv_heads = rng.choice([1, 2, 4, 8, 16, 32])
+        heads = kv_heads * rng.choice([h for h in (1, 2, 4, 5, 8, 16) if kv_heads * h <= 64])
+        q = rng.choice(["bf16", "f16"])
+        return {"op": op, "tokens": _spread(rng, 1, min(8192, 66000000 // ((heads + 2 * kv_heads) * dim))), "heads": heads,
+                "kv_heads": kv_heads, "dim": dim, **_rotary(rng, dim), "in": rng.choice(["f32", "f32", q]), "q": q,
+                "cache": rng.choice([q, q, "f8"]), "page": rng.choice([8, 16, 64, 256]), "layout": rng.choice(["token", "head"])}
+    dim = rng.choice([64, 96, 128, 128, 128, 192, 256])
+    kv_heads = rng.choice([1, 2, 4, 8, 8, 16, 32])
+    heads = kv_heads * rng.choice([h for h in (1, 2, 3, 4, 5, 7, 8, 16, 32) if kv_heads * h <= 64])
+    rows = _spread(rng, 1, 256)
+    q = rng.choice(["bf16", "f16"])
+    cache = rng.choice([q, q, "f8"])
+    # at most 350M elements of keys, and as many of values, were all rows as long as the longest
+    most = _spread(rng, 20, max(21, min(100000, 350000000 // (rows * kv_heads * dim))))
+    return {"op": op, "rows": rows, "least": max(1, int(most * rng.choice([1.0, 0.5, 0.05]))), "most": most, "heads": heads,
+            "kv_heads": kv_heads, "dim": dim, "page": rng.choice([8, 16, 16, 24, 64, 256]), "cache": cache, "q": q,
+            "out": rng.choice(["f32", q]), "window": rng.choice([0, 0, 0, 1000]), "layout": rng.choice(["token", "head"]),
+            "empty": min(rows - 1, rng.choice([0, 0, 0, 3]))}
+
+
+# ---- inputs ----------------------------------------------------------------------------
+
+class _Dev:
+    """A torch tensor as the package's calls take device memory (ptr, nbytes)."""
+
+    def __init__(self, t):
+        self.t = t
+        self.ptr = ctypes.c_void_p(t.data_ptr())
+        self.nbytes = t.numel() * t.element_size()
+
+
+def _gen(seed, salt):
+    g = torch.Generator(device="cuda")
+    g.manual_seed((int(seed) * 1000003 + salt) & 0x7FFFFFFFFFFF)
+    return g
+
+
+def _normal(g, shape, kind, scale=1.0):
+    """N(0, scale) in the type, made in pieces so that a large cache needs no fp32 copy of itself."""
+    out = torch.empty(shape, device="cuda", dtype=_FLOAT[kind])
+    flat = out.view(-1)
+    for at in range(0, flat.numel(), 1 << 27):
+        n = min(1 << 27, flat.numel() - at)
+        flat[at:at + n] = (torch.randn(n, generator=g, device="cuda") * scale).to(_FLOAT[kind])
+    return out
+
+
+def _ints(values):
+    return torch.tensor(values, device="cuda", dtype=torch.int32)
+
+
+def _of_case(case):
+    """The random numbers that belong to the case itself, whatever the seed."""
+    return random.Random(repr(sorted((k, v) for k, v in case.items() if k != "name")))
+
+
+def _request_lengths(case):
+    rng = _of_case(case)
+    cached, new = [], []
+    prompt = set(rng.sample(range(case["requests"]), case["prompts"]))
+    for r in range(case["requests"]):
+        if r in prompt:  # a prompt, or a later piece of one
+            cached.append(rng.choice([0, 0, _spread(rng, 1, case["cached"])]))
+            new.append(_spread(rng, max(1, case["new"] // 8), case["new"]))
+        else:
+            cached.append(_spread(rng, 1, case["cached"]))
+            new.append(1 if case["requests"] == 1 or rng.random() < 0.97 else 0)
+    return cached, new
+
+
+def _row_lengths(case):
+    rng = _of_case(case)
+    lens = [_spread(rng, case["least"], case["most"]) for _ in range(case["rows"])]
+    lens[0] = case["most"]
+    for r in rng.sample(range(1, case["rows"]), case["empty"]):
+        lens[r] = 0
+    return lens
+
+
+def _read_lengths(case):
+    """Keys that each row attends to: all of them, or its window's."""
+    return [min(n, case["window"]) if case["window"] else n for n in _row_lengths(case)]
+
+
+def _frequencies(case):
+    """Radians a position of each pair, and the pair's axis: equal blocks of pairs to each
+    axis (the first takes the rest), or the axes in turn."""
+    pairs = case["rot"] // 2
+    freq = [10000.0 ** (-i / pairs) for i in range(pairs)]
+    if case["order"] == "cycled":
+        axis = [i % case["axes"] for i in range(pairs)]
+    else:
+        each = pairs // case["axes"]
+        axis = [max(0, i - (pairs - each * case["axes"])) // each for i in range(pairs)]
+    return freq, axis
+
+
+def _positions(case, seed):
+    """[axes, tokens]: running text, or frames of patches (time, height, width)."""
+    g = _gen(seed, 3)
+    n, most = case["tokens"], case.get("offset", 4000)
+    first = torch.randint(0, most + 1, (1,), generator=g, device="cuda", dtype=torch.int64)
+    i = torch.arange(n, device="cuda", dtype=torch.int64)
+    if case["axes"] == 1:
+        pos = (first + i)[None]
+    else:
+        pos = torch.stack([first + i // (24 * 42), first + i // 42 % 24, first + i % 42])
+    return pos.to(torch.int32).contiguous()
+
+
+def _cache_shape(case, pages):
+    p, h, d = case["page"], case["kv_heads"], case["dim"]
+    return (pages, p, h, d) if case["layout"] == "token" else (pages, h, p, d)
+
+
+def prepare(case, seed):
+    st = {"case": case}
+    {"plan": _prepare_plan, "rope": _prepare_rope, "append": _prepare_append, "attn": _prepare_attn}[case["op"]](case, seed, st)
+    return st
+
+
+def _prepare_plan(case, seed, st):
+    cached, new = _request_lengths(case)
+    page, requests = case["page"], case["requests"]
+    held = [-(-c // page) for c in cached]
+    widest = max(-(-(c + n) // page) for c, n in zip(cached, new)) + 1
+    tokens = sum(new) + 5  # a step's arrays are as long as its largest step
+    total = sum(held) + case["spare"]
+    order = torch.randperm(total, generator=_gen(seed, 1), device="cuda").to(torch.int32)
+    tables = torch.full((requests, widest), -1, device="cuda", dtype=torch.int32)
+    have = _ints(held).long()
+    before = torch.cumsum(have, 0) - have
+    column = torch.arange(widest, device="cuda")[None]
+    at = (before[:, None] + column).clamp_(max=max(total - 1, 0))
+    st["tables"] = torch.where(column < have[:, None], order[at], tables).contiguous()
+    st["free"] = order[sum(held):].contiguous()
+    st.update(cached=_ints(cached), new=_ints(new), tokens=tokens)
+    if own:
+        q = _qmm()
+        st["out"] = {k: torch.empty(n, device="cuda", dtype=torch.int32)
+                     for k, n in (("starts", requests + 1), ("lens", requests), ("slots", tokens), ("positions", tokens),
+                                  ("rows", tokens), ("row_lens", tokens), ("counts", 4))}
+        st["plan"] = q.StepPlan(page, requests, tokens, widest, buffers={k: _Dev(t) for k, t in st["out"].items()})
+        st["dev"] = {k: _Dev(st[k]) for k in ("cached", "new", "tables", "free")}
+
+
+def _prepare_rope(case, seed, st):
+    st["x"] = _normal(_gen(seed, 2), (case["tokens"], case["heads"], case["dim"]), case["in"])
+    _rotary_state(case, seed, st)
+    if own:
+        q = _qmm()
+        st["y"] = torch.empty(case["tokens"], case["heads"], case["dim"], device="cuda", dtype=_FLOAT[case["out"]])
+        st["dev"] = {k: _Dev(st[k]) for k in ("x", "y", "pos")}
+        st["types"] = (q.DType.of(case["in"]), q.DType.of(case["out"]))
+
+
+def _rotary_state(case, seed, st):
+    freq, axis = _frequencies(case)
+    st["pos"] = _positions(case, seed)
+    st["freq"] = torch.tensor(freq, device="cuda", dtype=torch.float32)
+    st["axis"] = torch.tensor(axis, device="cuda", dtype=torch.int64)
+    if own:
+        st["rope"] = _qmm().Rope(freq, axes=axis, pairing=case["pairing"])
+
+
+def _scales(case):
+    return (1.0, 1.0) if case["cache"] != "f8" else (0.03125, 0.02)
+
+
+def _prepare_append(case, seed, st):
+    n, page = case["tokens"], case["page"]
+    pages = n // page + 8
+    for i, (name, heads) in enumerate((("q", case["heads"]), ("k", case["kv_heads"]), ("v", case["kv_heads"]))):
+        st[name] = _normal(_gen(seed, 10 + i), (n, heads, case["dim"]), case["in"])
+    for i, name in enumerate(("kc", "vc")):
+        st[name] = _normal(_gen(seed, 20 + i), _cache_shape(case, pages), case["cache"])
+    order = torch.randperm(pages, generator=_gen(seed, 1), device="cuda")
+    if n <= 256:  # single tokens of many requests: a slot anywhere
+        slots = torch.randperm(pages * page, generator=_gen(seed, 4), device="cuda")[:n]
+    else:  # a prompt: consecutive slots of scattered pages
+        i = torch.arange(n, device="cuda")
+        slots = order[i // page] * page + i % page
+    st["slots"] = slots.to(torch.int32)
+    _rotary_state(case, seed, st)
+    if own:
+        q = _qmm()
+        st["qo"] = torch.empty(n, case["heads"], case["dim"], device="cuda", dtype=_FLOAT[case["q"]])
+        st["dev"] = {k: _Dev(st[k]) for k in ("q", "k", "v", "kc", "vc", "qo", "pos", "slots")}
+        st["cache"] = q.KVCache(st["dev"]["kc"], st["dev"]["vc"], q.DType.of(case["cache"]), pages, page, case["kv_heads"],
+                                case["dim"], layout=case["layout"], k_scale=_scales(case)[0], v_scale=_scales(case)[1])
+        st["types"] = (q.DType.of(case["in"]), q.DType.of(case["q"]))
+
+
+def _prepare_attn(case, seed, st):
+    lens, page, rows = _row_lengths(case), case["page"], case["rows"]
+    widest = max(-(-n // page) for n in lens)
+    held = _ints([-(-n // page) for n in lens]).long()
+    pages = sum(-(-n // page) for n in lens) + 3
+    order = torch.randperm(pages, generator=_gen(seed, 1), device="cuda").to(torch.int32)
+    before = torch.cumsum(held, 0) - held
+    column = torch.arange(widest, device="cuda")[None]
+    st["tables"] = torch.where(column < held[:, None], order[(before[:, None] + column).clamp_(max=pages - 1)], 0).contiguous()
+    st["lens"] = _ints(lens)
+    spread = 1.0 if case["cache"] != "f8" else 30.0  # e4m3 codes over their range, brought back by the scales
+    st["kc"] = _normal(_gen(seed, 20), _cache_shape(case, pages), case["cache"], spread)
+    st["vc"] = _normal(_gen(seed, 21), _cache_shape(case, pages), case["cache"], spread)
+    st["q"] = _normal(_gen(seed, 2), (rows, case["heads"], case["dim"]), case["q"], 1.5)
+    if own:
+        q = _qmm()
+        st["o"] = torch.empty(rows, case["heads"], case["dim"], device="cuda", dtype=_FLOAT[case["out"]])
+        st["lse"] = torch.empty(rows, case["heads"], device="cuda", dtype=torch.float32)
+        st["dev"] = {k: _Dev(st[k]) for k in ("kc", "vc", "q", "o", "lse", "tables", "lens")}
+        cache = q.KVCache(st["dev"]["kc"], st["dev"]["vc"], q.DType.of(case["cache"]), pages, page, case["kv_heads"],
+                          case["dim"], layout=case["layout"], k_scale=_scales(case)[0], v_scale=_scales(case)[1])
+        st["cache"] = cache
+        st["attn"] = q.PagedAttention(case["heads"], case["kv_heads"], case["dim"], rows, q_dtype=q.DType.of(case["q"]),
+                                      out_dtype=q.DType.of(case["out"]), window=case["window"])
+
+
+# ---- one pass --------------------------------------------------------------------------
+
+def run(st):
+    op = st["case"]["op"]
+    if own:
+        return {"plan": _own_plan, "rope": _own_rope, "append": _own_append, "attn": _own_attn}[op](st)
+    return {"plan": _plain_plan, "rope": _plain_rope, "append": _plain_append, "attn": _plain_attn}[op](st)
+
+
+def _own_plan(st):
+    d = st["dev"]
+    st["plan"].run(d["cached"], d["new"], st["case"]["requests"], d["tables"], d["free"], st["free"].numel())
+    return {"tables": st["tables"], **st["out"]}
+
+
+def _own_rope(st):
+    case, d = st["case"], st["dev"]
+    st["rope"].apply(d["x"], st["types"][0], d["y"], st["types"][1], d["pos"], case["tokens"], case["heads"], case["dim"],
+                     inverse=case["inverse"])
+    return st["y"]
+
+
+def _own_append(st):
+    case, d = st["case"], st["dev"]
+    st["rope"].append(st["cache"], d["q"], d["k"], d["v"], st["types"][0], d["qo"], st["types"][1], d["pos"], d["slots"],
+                      case["tokens"], case["heads"])
+    return {"q": st["qo"], "k": st["kc"], "v": st["vc"]}
+
+
+def _own_attn(st):
+    case, d = st["case"], st["dev"]
+    st["attn"].run(st["cache"], d["q"], d["o"], d["tables"], st["tables"].shape[1], d["lens"], case["rows"], d_lse=d["lse"])
+    return {"o": st["o"], "lse": st["lse"]}
+
+
+def _plain_plan(st):
+    page, tokens, tables, free = st["case"]["page"], st["tokens"], st["tables"], st["free"]
+    cached, new = st["cached"].long(), st["new"].long()
+    requests, widest = tables.shape
+    held, last = (cached + page - 1) // page, (cached + new + page - 1) // page
+    too_long = last > widest
+    need = torch.where(too_long, 0, last - held)
+    upto = torch.cumsum(need, 0)
+    refused = too_long | ((need > 0) & (upto > free.numel()))
+    column = torch.arange(widest, device="cuda")[None]
+    fresh = (column >= held[:, None]) & (column < last[:, None]) & ~refused[:, None]
+    at = ((upto - need)[:, None] + column - held[:, None]).clamp_(0, max(free.numel() - 1, 0))
+    tables.copy_(torch.where(fresh, free[at], tables))
+    ends = torch.cumsum(new, 0)
+    starts = torch.cat([ends.new_zeros(1), ends])
+    t = torch.arange(tokens, device="cuda")
+    row = torch.searchsorted(ends, t, right=True)
+    real = row < requests
+    r = row.clamp(max=requests - 1)
+    pos = cached[r] + t - starts[r]
+    placed = real & ~refused[r]
+    slot = tables[r, (pos // page).clamp(0, widest - 1)].long() * page + pos % page
+    taken = torch.where(refused, 0, need).sum()
+    return {"tables": tables, "starts": starts.int(), "lens": torch.where(refused, cached, cached + new).int(),
+            "slots": torch.where(placed, slot, -1).int(), "positions": torch.where(real, pos, -1).int(),
+            "rows": torch.where(real, row, -1).int(), "row_lens": torch.where(placed, pos + 1, 0).int(),
+            "counts": torch.stack([ends[-1], taken, refused.sum(), taken]).int()}
+
+
+def _turned(x, st, inverse=False):
+    """x [tokens, heads, dim] in 32 bits with its first `rot` dimensions rotated."""
+    case = st["case"]
+    angle = st["pos"].float()[st["axis"]].t() * st["freq"]  # [tokens, pairs]
+    c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    if inverse:
+        s = -s
+    x = x.float()
+    turn, rest = x[..., :case["rot"]], x[..., case["rot"]:]
+    if case["pairing"] == "halves":
+        a, b = turn[..., :case["rot"] // 2], turn[..., case["rot"] // 2:]
+        return torch.cat([a * c - b * s, a * s + b * c, rest], -1)
+    a, b = turn[..., 0::2], turn[..., 1::2]
+    return torch.cat([torch.stack([a * c - b * s, a * s + b * c], -1).flatten(-2), rest], -1)
+
+
+def _plain_rope(st):
+    return _turned(st["x"], st, st["case"]["inverse"]).to(_FLOAT[st["case"]["out"]])
+
+
+def _by_token(cache, case):
+    """The cache as [pages, page, heads, dim]."""
+    return cache if case["layout"] == "token" else cache.transpose(1, 2)
+
+
+def _bits(t):
+    return t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+
+
+def _plain_append(st):
+    case = st["case"]
+    at, off = st["slots"].long() // case["page"], st["slots"].long() % case["page"]
+    for new, cache, scale in ((_turned(st["k"], st), st["kc"], _scales(case)[0]), (st["v"].float(), st["vc"], _scales(case)[1])):
+        new = new / scale
+        if case["cache"] == "f8":
+            new = new.clamp(-_F8_MOST, _F8_MOST)
+        _by_token(_bits(cache), case)[at, off] = _bits(new.to(cache.dtype))
+    return {"q": _turned(st["q"], st).to(_FLOAT[case["q"]]), "k": st["kc"], "v": st["vc"]}
+
+
+def _plain_attn(st):
+    case, tables, lens = st["case"], st["tables"].long(), st["lens"].long()
+    rows, heads, kv_heads, dim = case["rows"], case["heads"], case["kv_heads"], case["dim"]
+    k, v = (_bits(_by_token(c, case))[tables].view(c.dtype).float().reshape(rows, -1, kv_heads, dim).transpose(1, 2).contiguous()
+            for c in (st["kc"], st["vc"]))  # [rows, kv_heads, keys, dim]
+    q = st["q"].float().view(rows, kv_heads, heads // kv_heads, dim) * (_scales(case)[0] / math.sqrt(dim))
+    s = torch.matmul(k, q.transpose(2, 3).contiguous())  # [rows, kv_heads, keys, group]
+    j = torch.arange(k.shape[2], device="cuda")[None]
+    seen = j < lens[:, None]
+    if case["window"]:
+        seen = seen & (j >= lens[:, None] - case["window"])
+    s = s.masked_fill(~seen[:, None, :, None], -math.inf)
+    most = s.amax(2, keepdim=True)
+    p = torch.exp(s - torch.where(most == -math.inf, 0.0, most))
+    total = p.sum(2, keepdim=True)
+    p = p / torch.where(total == 0, 1.0, total)
+    o = torch.matmul(p.transpose(2, 3).contiguous(), v) * _scales(case)[1]
+    lse = (most + torch.log(total)).squeeze(2)
+    return {"o": o.view(rows, heads, dim).to(_FLOAT[case["out"]]), "lse": lse.reshape(rows, heads)}
+
+
+# ---- what a pass needs -----------------------------------------------------------------
+
+def work(case):
+    op = case["op"]
+    if op == "plan":
+        cached, new = _request_lengths(case)
+        pages = sum(-(-(c + n) // case["page"]) - -(-c // case["page"]) for c, n in zip(cached, new))
+        return {"bytes": 16 * case["requests"] + 8 * pages + 16 * (sum(new) + 5) + 20, "flops": 0}
+    if op == "rope":
+        elems = case["tokens"] * case["heads"] * case["dim"]
+        return {"bytes": elems * (_SIZE[case["in"]] + _SIZE[case["out"]]) + 4 * case["axes"] * case["tokens"],
+                "flops": 3 * case["tokens"] * case["heads"] * case["rot"]}
+    if op == "append":
+        n, d, h, kv = case["tokens"], case["dim"], case["heads"], case["kv_heads"]
+        return {"bytes": n * d * ((h + 2 * kv) * _SIZE[case["in"]] + h * _SIZE[case["q"]] + 2 * kv * _SIZE[case["cache"]]) +
+                4 * n * (case["axes"] + 1), "flops": 3 * n * (h + kv) * case["rot"]}
+    keys, rows, h, d = sum(_read_lengths(case)), case["rows"], case["heads"], case["dim"]
+    pages = sum(-(-n // case["page"]) for n in _read_lengths(case))
+    return {"bytes": 2 * keys * case["kv_heads"] * d * _SIZE[case["cache"]] + rows * h * (d * (_SIZE[case["q"]] + _SIZE[case["out"]]) + 4) +
+            4 * (pages + rows), "flops": 4 * keys * h * d}
+
+
+# ---- the definitions, in 64 bits -------------------------------------------------------
+
+def exact(case, seed):
+    """What `run` returns, from the definitions in 64 bits: whole numbers have no such value."""
+    if case["op"] == "plan":
+        return None
+    global own
+    was, own = own, False  # the inputs alone
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = was
+    if case["op"] == "rope":
+        return _exact_turn(st["x"], st, -1.0 if case["inverse"] else 1.0)
+    if case["op"] == "append":
+        return _exact_append(st)
+    return _exact_attn(st)
+
+
+def _exact_turn(x, st, sign):
+    """Each pair as a complex number, times exp(i angle)."""
+    case = st["case"]
+    freq, axis = _frequencies(case)
+    angle = sign * st["pos"].double()[torch.tensor(axis, device="cuda")].t() * torch.tensor(freq, device="cuda", dtype=torch.float64)
+    by = torch.polar(torch.ones_like(angle), angle)[:, None]
+    y = x.double().clone()
+    half = case["rot"] // 2
+    first, second = (slice(0, half), slice(half, 2 * half)) if case["pairing"] == "halves" else (slice(0, 2 * half, 2), slice(1, 2 * half, 2))
+    z = torch.complex(y[..., first], y[..., second]) * by
+    y[..., first], y[..., second] = z.real, z.imag
+    return y
+
+
+def _exact_append(st):
+    case = st["case"]
+    page = st["slots"].long() // case["page"]
+    off = st["slots"].long() % case["page"]
+    caches = []
+    for new, cache, scale in ((_exact_turn(st["k"], st, 1.0), st["kc"], _scales(case)[0]), (st["v"].double(), st["vc"], _scales(case)[1])):
+        full = cache.float().double()
+        new = new / scale
+        if case["cache"] == "f8":
+            new = new.clamp(-_F8_MOST, _F8_MOST)
+        if case["layout"] == "token":
+            full[page, off] = new
+        else:
+            full[page, :, off] = new
+        caches.append(full)
+    return {"q": _exact_turn(st["q"], st, 1.0), "k": caches[0], "v": caches[1]}
+
+
+def _exact_attn(st):
+    """Row by row and key head by key head over the keys that the row's mask leaves."""
+    case = st["case"]
+    group, page = case["heads"] // case["kv_heads"], case["page"]
+    k_scale, v_scale = _scales(case)
+    lens = _row_lengths(case)
+    out = torch.zeros(case["rows"], case["heads"], case["dim"], device="cuda", dtype=torch.float64)
+    lse = torch.full((case["rows"], case["heads"]), -math.inf, device="cuda", dtype=torch.float64)
+    for r, n in enumerate(lens):
+        if n == 0:
+            continue
+        at = torch.arange(max(0, n - case["window"]) if case["window"] else 0, n, device="cuda")
+        page_id, off = st["tables"][r].long()[at // page], at % page
+        keys, values = (_bits(c)[page_id, off] if case["layout"] == "token" else _bits(c)[page_id, :, off] for c in (st["kc"], st["vc"]))
+        keys, values = keys.view(st["kc"].dtype).double() * k_scale, values.view(st["vc"].dtype).double() * v_scale
+        for h in range(case["kv_heads"]):
+            mine = slice(h * group, (h + 1) * group)
+            s = st["q"][r, mine].double() @ keys[:, h].t().contiguous() / math.sqrt(case["dim"])
+            lse[r, mine] = torch.logsumexp(s, 1)
+            out[r, mine] = torch.exp(s - lse[r, mine, None]) @ values[:, h].contiguous()
+    return {"o": out, "lse": lse}
