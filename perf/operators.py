@@ -324,7 +324,7 @@ def _prepare_attn(case, seed, st):
         cache = q.KVCache(st["dev"]["kc"], st["dev"]["vc"], q.DType.of(case["cache"]), pages, page, case["kv_heads"],
                           case["dim"], layout=case["layout"], k_scale=_scales(case)[0], v_scale=_scales(case)[1])
         st["cache"] = cache
-        st["attn"] = q.PagedAttention(case["heads"], case["kv_heads"], case["dim"], rows, q_dtype=q.DType.of(case["q"]),
+        st["attn"] = q.PagedAttention(case["heads"], case["kv_heads"], case["dim"], q_dtype=q.DType.of(case["q"]),
                                       out_dtype=q.DType.of(case["out"]), window=case["window"])
 
 
