@@ -1,0 +1,127 @@
+// Declarations shared by the attention step's C ABI (attn_api.hip) and its kernels
+// (attn_plan.hip, attn_rope.hip, attn_decode.hpp).
+#pragma once
+
+#include "qmm_internal.hpp"
+
+#include "../../include/openmini_attn.h"
+
+namespace attn {
+
+// n / d for 0 <= n < 2^31 by one multiplication: with l = ceil(log2 d) >= 1 and
+// m = ceil(2^(31 + l) / d) < 2^32, m d exceeds 2^(31 + l) by less than d <= 2^l, so
+// floor(n m / 2^(31 + l)) = floor(n / d) while n < 2^31.  d = 1 is m = 0.
+struct FastDiv {
+    uint32_t d = 1, m = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div) {
+        uint32_t l = 0;
+        while (((uint64_t)1 << l) < div) ++l;
+        if (l == 0) return;
+        shift = l - 1;
+        m = (uint32_t)((((uint64_t)1 << (31 + l)) + div - 1) / div);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) >> shift : n; }
+};
+
+// A cache as the kernels see it: strides in bytes.
+struct Cache {
+    uint8_t* k;
+    uint8_t* v;
+    int64_t page_stride, token_stride, head_stride;
+    uint32_t n_pages, slots;  // slots = n_pages * page_size
+    FastDiv page;
+    float k_scale, v_scale;
+};
+
+// ---- attn_plan.hip -------------------------------------------------------------------
+constexpr int kMaxPlanRequests = 4096;  // two words a request in a workgroup's LDS
+
+struct PlanArgs {
+    const int32_t *cached, *fresh, *free, *head;
+    int32_t *tables, *starts, *lens, *rows, *positions, *slots, *row_lens, *counts;
+    int64_t table_stride;
+    uint32_t requests, n_free, max_pages, max_held, max_tokens;  // max_held = max_pages * page_size
+    FastDiv page;
+};
+hipError_t launch_plan(const PlanArgs& a, hipStream_t s);
+
+// ---- attn_rope.hip -------------------------------------------------------------------
+constexpr int kMaxPairs = 128;
+constexpr int kMaxAxes = 8;
+
+struct RopePair {
+    uint64_t step;  // revolutions a position, as a fraction of 2^64
+    int32_t axis;
+    int32_t unused;
+};
+
+struct Rope {
+    RopePair* pairs;  // device
+    int32_t n_pairs, axes, adjacent;
+    float scale;
+};
+
+struct RopeArgs {
+    // tokens x (heads + 2 kv_heads) heads: the first `heads` turned into y, then (append)
+    // kv_heads of k turned into the cache and kv_heads of v written to it
+    const uint8_t *x, *k, *v;
+    int64_t x_stride, k_stride, v_stride, y_stride;  // bytes a token
+    uint8_t* y;
+    const int32_t* positions;
+    int64_t position_stride;
+    const int32_t* slots;  // NULL: no cache
+    Cache cache;
+    const RopePair* pairs;
+    float scale;
+    float k_over, v_over;  // 1 / k_scale, 1 / v_scale
+    int32_t tokens, heads, kv_heads, n_pairs;
+    int32_t x_dtype, y_dtype, cache_dtype;
+    int32_t adjacent, inverse;
+    FastDiv per_token, per_head, by_pairs;  // items of a token and of a head; n_pairs
+};
+hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s);
+
+// ---- attn_decode_*.hip ---------------------------------------------------------------
+constexpr int kTile = 32;        // keys a wave takes at a time
+constexpr int kHeadTile = 16;    // query heads a workgroup serves (the MFMA's columns)
+constexpr int kMaxParts = 256;   // parts of one row
+constexpr int kMaxHeads = 1024;  // query heads
+constexpr int kRound = 1024;     // workgroups that decode_shape() aims at, at most
+constexpr size_t kCounters = 2 * (kRound + kMaxHeads);  // at least 2 ceil(kRound / units) units
+
+struct DecodeArgs {
+    Cache cache;
+    const uint8_t* q;
+    uint8_t* out;
+    float* lse;
+    const int32_t *lens, *rows, *tables;
+    int64_t q_stride, out_stride;  // bytes
+    int64_t table_stride;
+    int64_t window;
+    uint32_t n_rows, requests, max_len;  // max_len = max_pages * page_size
+    int32_t q_heads, kv_heads, group, head_tiles;
+    int32_t out_f32;
+    float scale;  // of a raw product, in powers of two: scale * k_scale * log2(e)
+    // The cut of long rows: parts of at least min_tiles tiles, about target_parts in all
+    // (for each of the units = kv_heads * head_tiles).
+    uint32_t target_parts, min_tiles, max_parts;
+    FastDiv by_kv_heads, by_head_tiles;
+    uint32_t* counters;  // [place of a split row's first part][units], 0 between calls
+    float* part_acc;     // [parts][units][heads of a tile][head_dim]
+    float* part_ml;      // [parts][units][heads of a tile][2]
+    uint32_t part_acc_bytes, part_ml_bytes;
+};
+
+// The cut for a call.
+struct DecodeShape {
+    uint32_t target_parts, min_tiles, max_parts;
+};
+DecodeShape decode_shape(int64_t rows, int kv_heads, int head_tiles, int head_dim, int64_t max_len);
+// Parts that the split rows of one call have at most (for each unit).
+int64_t decode_split_parts(int kv_heads, int head_tiles, int head_dim);
+
+hipError_t launch_decode_bf16(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s);
+hipError_t launch_decode_f16(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s);
+
+}  // namespace attn

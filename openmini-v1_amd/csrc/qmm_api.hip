@@ -266,6 +266,10 @@ namespace qmm {
 
 void set_last_error(const char* msg) { g_last_error = msg ? msg : ""; }
 
+int report_error(int code, const char* msg) { return fail(code, "%s", msg); }
+
+int current_device(int* out_dev) { return ensure_device(out_dev); }
+
 int upload_from_host(int type, const void* host_blocks, size_t bytes, int64_t n_rows, int64_t k_cols, void* stream,
                      openmini_qweight** out_weight) {
     *out_weight = nullptr;

@@ -319,6 +319,12 @@ hipError_t launch_stream_read(const void* src, size_t bytes, uint32_t* sink, hip
 // Sets the calling thread's openmini_qmm_last_error() message.
 void set_last_error(const char* msg);
 
+// The same, passed to the log callback too; returns `code`.
+int report_error(int code, const char* msg);
+
+// The current device's ordinal, after checking that it is a gfx950 part (a reported status).
+int current_device(int* out_dev);
+
 // Host GGUF blocks of W[n_rows, k_cols] -> a new repacked weight handle (validated like
 // openmini_qmm_upload); the copy and repack run on `stream`, which is synchronised.
 int upload_from_host(int type, const void* host_blocks, size_t bytes, int64_t n_rows, int64_t k_cols, void* stream,

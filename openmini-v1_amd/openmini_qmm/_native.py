@@ -1,4 +1,5 @@
-"""ctypes binding of libopenmini_qmm.so (C-ABI in include/openmini_qmm.h).
+"""ctypes binding of libopenmini_qmm.so (C-ABI in include/openmini_qmm.h and
+include/openmini_attn.h).
 
 The library is the only compute path: if it is missing this module raises, there
 is no CPU fallback.  Build it with `python openmini-v1_amd/build.py`.
@@ -133,6 +134,63 @@ SIGNATURES = {
     "openmini_qmm_convert_to_soa": (_i, [_i, _p, _sz, _sz, _p]),
 }
 
+
+
+class KvCache(ctypes.Structure):  # openmini_kv_cache_t
+    _fields_ = [
+        ("d_k", _p), ("d_v", _p),
+        ("dtype", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("n_pages", _i64), ("page_stride", _i64), ("token_stride", _i64), ("head_stride", _i64),
+        ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float),
+    ]
+
+
+class KvPlanArgs(ctypes.Structure):  # openmini_kv_plan_args_t
+    _fields_ = [
+        ("d_cached", _p), ("d_new", _p), ("requests", _i64), ("d_free", _p), ("n_free", _i64), ("d_head", _p),
+        ("d_tables", _p), ("table_stride", _i64), ("max_pages", _i64), ("page_size", _i64), ("max_tokens", _i64),
+        ("d_starts", _p), ("d_lens", _p), ("d_rows", _p), ("d_positions", _p), ("d_slots", _p), ("d_row_lens", _p),
+        ("d_counts", _p),
+    ]
+
+
+class RopeArgs(ctypes.Structure):  # openmini_rope_args_t
+    _fields_ = [
+        ("d_x", _p), ("d_y", _p), ("x_stride", _i64), ("y_stride", _i64), ("x_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32), ("tokens", _i64), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("inverse", ctypes.c_int32), ("d_positions", _p), ("position_stride", _i64),
+    ]
+
+
+class RopeAppendArgs(ctypes.Structure):  # openmini_rope_append_args_t
+    _fields_ = [
+        ("d_q", _p), ("d_k", _p), ("d_v", _p), ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64),
+        ("d_q_out", _p), ("q_out_stride", _i64), ("in_dtype", ctypes.c_int32), ("q_out_dtype", ctypes.c_int32),
+        ("tokens", _i64), ("q_heads", ctypes.c_int32), ("d_positions", _p), ("position_stride", _i64), ("d_slots", _p),
+    ]
+
+
+class AttnArgs(ctypes.Structure):  # openmini_attn_args_t
+    _fields_ = [
+        ("d_q", _p), ("q_stride", _i64), ("d_out", _p), ("out_stride", _i64), ("d_lse", _p), ("q_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("scale", ctypes.c_float), ("window", _i64),
+        ("rows", _i64), ("d_lens", _p), ("d_rows", _p), ("d_tables", _p), ("table_stride", _i64), ("max_pages", _i64),
+        ("requests", _i64), ("d_work", _p), ("work_bytes", _sz),
+    ]
+
+
+# name -> (restype, argtypes); mirrors include/openmini_attn.h one to one.
+ATTN_SIGNATURES = {
+    "openmini_kv_plan": (_i, [ctypes.POINTER(KvPlanArgs), _p]),
+    "openmini_rope_create": (_i, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int32), _i, _i, _i, ctypes.c_float,
+                                  ctypes.POINTER(_p)]),
+    "openmini_rope_free": (None, [_p]),
+    "openmini_rope_apply": (_i, [_p, ctypes.POINTER(RopeArgs), _p]),
+    "openmini_rope_append": (_i, [_p, ctypes.POINTER(KvCache), ctypes.POINTER(RopeAppendArgs), _p]),
+    "openmini_attn_workspace_bytes": (_sz, [_i, _i, _i]),
+    "openmini_attn_decode": (_i, [ctypes.POINTER(KvCache), ctypes.POINTER(AttnArgs), _p]),
+}
+
 _lib = None
 
 
@@ -145,7 +203,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python openmini-v1_amd/build.py` "
                 "(the HIP library is the only compute path)")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (*SIGNATURES.items(), *ATTN_SIGNATURES.items()):
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

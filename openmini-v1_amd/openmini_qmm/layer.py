@@ -7,8 +7,8 @@ several linear layers on one input:
     engine's fused_gemm_silu (gemm_engine/vulkan_backend.rs:111-131) has the same
     meaning, silu(gate) * up; here gate and up share one launch that writes `hidden` directly;
   * prepare_qkv (model.rs:1379-1410): q, k, v = linear_gemm(x, W_{q,k,v})
-    (model.rs:1392-1394), here one launch for the three.  RoPE and the attention
-    itself are not part of the quantized linear layer.
+    (model.rs:1392-1394), here one launch for the three.  CachedAttention runs them
+    together with the step that lies between them and o_proj (attention.py).
 
 The host-array methods are synchronous and mirror the reference's signatures; from
 the weight's gemm_min_rows() rows on (prefill: 64-128 rows by the weight's shape)
@@ -23,6 +23,7 @@ import ctypes
 import numpy as np
 
 from ._native import check, lib
+from .attention import DType, KVCache, PagedAttention, Rope, StepPlan
 from .ops import DeviceBuffer, InvalidInput, QuantizedWeight, gemm_f32_workspace
 
 MAX_GROUP = 4  # weights per gemv_multi launch
@@ -174,5 +175,47 @@ class AttentionWeights:
         return d_o.download(np.float32, (m, self.o_proj.n_rows))
 
 
-__all__ = ["AttentionWeights", "FFNWeights", "MAX_GROUP", "ffn_gate_up", "ffn_gate_up_bf16",
+class CachedAttention:
+    """One layer's attention over its paged cache: the q / k / v projections, rotary
+    positions and the cache write, attention, and the output projection,
+    for any mix of decoding requests and short prompts (a prompt's tokens are rows of their
+    own, each seeing the keys up to its position).
+
+    `attention` may be shared by layers that run one after the other; buffers for up to
+    max_tokens rows are allocated here."""
+
+    def __init__(self, weights: AttentionWeights, rope: Rope, cache: KVCache, q_heads: int, max_tokens: int,
+                 q_dtype: DType = DType.BF16, attention: PagedAttention | None = None):
+        head_dim = cache.head_dim
+        if weights.o_proj is None:
+            raise InvalidInput("no o_proj")
+        if (weights.q_proj.n_rows, weights.k_proj.n_rows, weights.v_proj.n_rows, weights.o_proj.k_cols) != \
+                (q_heads * head_dim, cache.kv_heads * head_dim, cache.kv_heads * head_dim, q_heads * head_dim):
+            raise InvalidInput(f"projections do not have {q_heads} query and {cache.kv_heads} key heads of {head_dim}")
+        self.weights, self.rope, self.cache = weights, rope, cache
+        self.q_heads, self.max_tokens, self.q_dtype = int(q_heads), int(max_tokens), DType(q_dtype)
+        self.attention = attention or PagedAttention(q_heads, cache.kv_heads, head_dim, q_dtype, DType.F32)
+        if self.attention.q_dtype != self.q_dtype or self.attention.out_dtype != DType.F32:
+            raise InvalidInput("the shared attention has other types")
+        q, kv = q_heads * head_dim, cache.kv_heads * head_dim
+        self.d_q, self.d_k, self.d_v = (DeviceBuffer(max_tokens * n * 4) for n in (q, kv, kv))
+        self.d_q16, self.d_attn = DeviceBuffer(max_tokens * q * 2), DeviceBuffer(max_tokens * q * 4)
+
+    def forward_device(self, d_x: DeviceBuffer, plan: StepPlan, d_tables, requests: int, tokens: int, d_out: DeviceBuffer,
+                       d_positions=None, stream=None) -> None:
+        """d_out [tokens, hidden] for the step that `plan` laid out (plan.run on the same
+        stream before the first layer): d_x [tokens, hidden] fp32, d_tables the tables that
+        the plan filled.  d_positions [axes][tokens]: None takes the plan's (one axis)."""
+        if tokens > min(self.max_tokens, plan.max_tokens):
+            raise InvalidInput(f"{tokens} tokens, planned for {min(self.max_tokens, plan.max_tokens)}")
+        w = self.weights
+        w.project_qkv_device(d_x, self.d_q, self.d_k, self.d_v, tokens, stream)
+        self.rope.append(self.cache, self.d_q, self.d_k, self.d_v, DType.F32, self.d_q16, self.q_dtype,
+                         plan.positions if d_positions is None else d_positions, plan.slots, tokens, self.q_heads, stream)
+        self.attention.run(self.cache, self.d_q16, self.d_attn, d_tables, plan.max_pages, plan.row_lens, tokens,
+                           d_rows=plan.rows, requests=requests, stream=stream)
+        w.o_proj.gemv(self.d_attn, d_out, tokens, stream)
+
+
+__all__ = ["AttentionWeights", "CachedAttention", "FFNWeights", "MAX_GROUP", "ffn_gate_up", "ffn_gate_up_bf16",
            "ffn_gate_up_f32", "gemv_multi"]

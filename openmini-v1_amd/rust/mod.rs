@@ -1,6 +1,7 @@
 //! src/model/inference/hip_quant/: the MI355X quantized linear layer behind the
 //! `hip-quant` cargo feature (declared from src/model/inference/mod.rs as
 //! `#[cfg(feature = "hip-quant")] pub mod hip_quant;`).
+pub mod attn_ffi;
 pub mod engine;
 pub mod ffi;
 pub mod gpu_quant_ops;
