@@ -155,33 +155,28 @@ bool decode_dim(int d) {
 
 size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
-// The workspace: a counter for each split row and unit, in a region of one size for every
-// geometry (so that calls of several share a workspace), then the parts' maxima and sums,
-// then their accumulators.
+// The workspace: the split rows, then the parts' maxima and sums, then their accumulators.
 struct Workspace {
-    size_t ml_at, acc_at, bytes, ml_bytes, acc_bytes;
+    size_t ml_at, acc_at, bytes;
 };
-Workspace workspace(int kv_heads, int head_tiles, int tile_heads, int head_dim) {
-    const size_t entries = (size_t)attn::decode_split_parts(kv_heads, head_tiles, head_dim) * kv_heads * head_tiles;
+Workspace workspace(int q_heads, int kv_heads, int head_tiles, int head_dim) {
+    const size_t shares = attn::decode_shares(kv_heads, head_tiles), entries = 2 * shares * q_heads;
     Workspace w;
-    w.ml_bytes = entries * tile_heads * 8;
-    w.acc_bytes = entries * tile_heads * head_dim * 4;
-    w.ml_at = attn::kCounters * 4;
-    w.acc_at = w.ml_at + round_up(w.ml_bytes, 256);
-    w.bytes = w.acc_at + w.acc_bytes;
+    w.ml_at = round_up(shares * sizeof(attn::Split), 256);
+    w.acc_at = w.ml_at + round_up(entries * 8, 256);
+    w.bytes = w.acc_at + entries * head_dim * 4;
     return w;
 }
 
 constexpr int64_t kMaxRows = (int64_t)1 << 20;
-constexpr int64_t kMostKeys = kMaxI32 - 63;  // whole tiles of keys stay below 2^31
+constexpr int64_t kMostKeys = kMaxI32 - 255;  // whole tiles of keys stay below 2^31
 
-bool decode_sizes(int q_heads, int kv_heads, int head_dim, int* head_tiles, int* tile_heads) {
+bool decode_sizes(int q_heads, int kv_heads, int head_dim, int* head_tiles) {
     if (kv_heads < 1 || q_heads < kv_heads || q_heads > 1024 || q_heads % kv_heads ||
         !decode_dim(head_dim))
         return false;
     const int group = q_heads / kv_heads;
     *head_tiles = (group + attn::kHeadTile - 1) / attn::kHeadTile;
-    *tile_heads = group < attn::kHeadTile ? group : attn::kHeadTile;
     return true;
 }
 
@@ -354,9 +349,9 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
 }
 
 size_t openmini_attn_workspace_bytes(int q_heads, int kv_heads, int head_dim) {
-    int head_tiles = 0, tile_heads = 0;
-    if (!decode_sizes(q_heads, kv_heads, head_dim, &head_tiles, &tile_heads)) return 0;
-    return workspace(kv_heads, head_tiles, tile_heads, head_dim).bytes;
+    int head_tiles = 0;
+    if (!decode_sizes(q_heads, kv_heads, head_dim, &head_tiles)) return 0;
+    return workspace(q_heads, kv_heads, head_tiles, head_dim).bytes;
 }
 
 int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_args_t* p, void* stream) {
@@ -373,8 +368,8 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     if (cache->page_size % 8)
         return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "page_size = %d is not a multiple of 8", cache->page_size);
     TRY(check_range("rows", p->rows, 0, kMaxRows));
-    int head_tiles = 0, tile_heads = 0;
-    if (!decode_sizes(p->q_heads, cache->kv_heads, cache->head_dim, &head_tiles, &tile_heads))
+    int head_tiles = 0;
+    if (!decode_sizes(p->q_heads, cache->kv_heads, cache->head_dim, &head_tiles))
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "q_heads = %d for kv_heads = %d: a multiple, at most 1024", p->q_heads,
                     cache->kv_heads);
     TRY(check_pointer("d_q", p->d_q, 16));
@@ -394,13 +389,13 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     TRY(check_range("requests", p->requests, 1, kMaxI32));
     if (p->rows == 0) return ok();
     const int64_t held = p->max_pages * cache->page_size, max_len = held < kMostKeys ? held : kMostKeys;
-    const auto shape = attn::decode_shape(p->rows, cache->kv_heads, head_tiles, cache->head_dim, max_len);
-    const int64_t tiles = max_len / attn::kTile + 2;
-    if (p->rows * tiles > (int64_t)UINT32_MAX / 2 ||
-        ((int64_t)shape.max_parts * cache->kv_heads + 8) * head_tiles > kMaxI32 / 2)
+    const uint32_t shares = attn::decode_shares(cache->kv_heads, head_tiles);
+    // tiles of the call at most
+    const int64_t tiles = p->rows * (max_len / (32 * attn::decode_subtiles(cache->head_dim, f8)) + 2);
+    if (tiles > (int64_t)UINT32_MAX / 2)
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%lld rows of up to %lld keys are too many for one call",
                     (long long)p->rows, (long long)max_len);
-    const auto w = workspace(cache->kv_heads, head_tiles, tile_heads, cache->head_dim);
+    const auto w = workspace(p->q_heads, cache->kv_heads, head_tiles, cache->head_dim);
     TRY(check_pointer("d_work", p->d_work, 256));
     if (p->work_bytes < w.bytes)
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "workspace of %zu bytes, %zu are needed", p->work_bytes, w.bytes);
@@ -424,21 +419,20 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     a.head_tiles = head_tiles;
     a.out_f32 = p->out_dtype == OPENMINI_ATTN_F32;
     a.scale = (float)((double)p->scale * cache->k_scale * 1.44269504088896340736);
-    a.target_parts = shape.target_parts;
-    a.min_tiles = shape.min_tiles;
-    a.max_parts = shape.max_parts;
-    a.by_kv_heads = attn::FastDiv((uint32_t)cache->kv_heads);
+    a.shares = shares;
+    a.launch_shares = tiles < (int64_t)shares ? (uint32_t)tiles : shares;
+    a.by_units = attn::FastDiv((uint32_t)(cache->kv_heads * head_tiles));
     a.by_head_tiles = attn::FastDiv((uint32_t)head_tiles);
     uint8_t* work = static_cast<uint8_t*>(p->d_work);
-    a.counters = reinterpret_cast<uint32_t*>(work);
-    a.part_ml = reinterpret_cast<float*>(work + w.ml_at);
+    a.split = reinterpret_cast<attn::Split*>(work);
+    a.part_ml = reinterpret_cast<float2*>(work + w.ml_at);
     a.part_acc = reinterpret_cast<float*>(work + w.acc_at);
-    a.part_ml_bytes = (uint32_t)w.ml_bytes;
-    a.part_acc_bytes = (uint32_t)w.acc_bytes;
+    a.by_row = p->rows <= (int64_t)shares;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    return launched(p->q_dtype == OPENMINI_ATTN_BF16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)
-                                                     : attn::launch_decode_f16(a, cache->head_dim, f8, s),
-                    "attention launch");
+    hipError_t e = p->q_dtype == OPENMINI_ATTN_BF16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)
+                                                    : attn::launch_decode_f16(a, cache->head_dim, f8, s);
+    if (e == hipSuccess && a.launch_shares > 1) e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
+    return launched(e, "attention launch");
 }
 
 }  // extern "C"

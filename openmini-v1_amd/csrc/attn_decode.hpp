@@ -1,7 +1,7 @@
 // Attention of single query tokens over a paged cache (openmini_attn_decode).
 //
-// A row's query heads that share a key head are the columns of 16 x 16 MFMA tiles.  A wave
-// takes 32 keys at a time:
+// A row's query heads that share a key head are the columns of 16 x 16 MFMA tiles.  For each
+// 32 keys a wave computes
 //   S^T = K q^T   (two 16-key tiles, head_dim in steps of 32)
 //   p = 2^(s - m), m and l the running maximum and sum of each column (s in powers of two)
 //   O^T += V^T P^T (head_dim in tiles of 16, all 32 keys at once)
@@ -17,14 +17,16 @@
 // neighbouring lanes, whole) and transposes them in registers, two keys to a dword, one
 // byte permutation each; tile e of a chunk is then dimensions e, e + width, ...
 //
-// The probabilities enter the second product as the sum of two 16-bit parts (their rounding
-// to one would be 2^-9 of the output in bf16; the second product is a tenth of the time that
-// its keys take to arrive).  Sums, maxima and the joined parts are fp32.
+// The probabilities enter the second product as the sum of two (fp16) or three (bf16) 16-bit
+// parts, together all of fp32 or nearly: their rounding to one bf16 would be 2^-9 of an fp32
+// output, to two 2^-18 (1.2e-6 measured, against 4e-7 for fp32 arithmetic throughout).
+// Sums, maxima and the joined parts are fp32.
 //
-// Bound by memory: 4 operations a byte and key head's query head.  The loads of the next
-// keys are issued as soon as the registers of the present ones are free, so a wave has one
-// tile in flight all the time and the waves of a CU together some 100 KB, several times
-// what latency times bandwidth asks for.
+// Bound by memory: 4 operations a byte for each query head of a key head.  The loads of the
+// next keys are issued as soon as the registers of the present ones are free, about 16 KB a
+// wave, one wave to a SIMD.  Measured (MI355X, GB/s of keys and values, second launch
+// included): 131071 keys of one row, 8 heads of 128, bf16 99.8 us, 5380 GB/s (a read of as
+// many bytes 84 us); 128 rows of 2000 - 12000 keys, e4m3, 270 us, 5560 GB/s.
 #pragma once
 
 #include <type_traits>
@@ -40,6 +42,7 @@ using qmm::f32x4;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct BF16 {
+    static constexpr int kExactParts = 3;  // that hold an fp32 probability, 8 bits each
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                        0, 0);
@@ -57,6 +60,7 @@ struct BF16 {
 };
 
 struct F16 {
+    static constexpr int kExactParts = 2;  // 11 bits each
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                       0);
@@ -114,137 +118,112 @@ __device__ __forceinline__ float column_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// log(sum of exponentials) from a maximum in powers of two and the sum above it.
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l == 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
+}
+
 // 2^(a - m) for a maximum m that is -inf where nothing is seen.
 __device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ __forceinline__ float exp2_of(float a) { return __builtin_amdgcn_exp2f(a); }
 
-// The part of a row that a workgroup takes: tiles [tile0, tile1) of keys [lo, hi), part
-// `part` of `parts`, whose first sits at `place` among the parts of all split rows.
-struct Part {
-    uint32_t row, tile0, tile1, part, parts, place;
-    int32_t lo, hi;
-};
-
 struct Span {
-    int32_t lo, hi;
+    int32_t lo, hi;   // the keys that a row sees
     uint32_t tiles;
+    __device__ __forceinline__ uint32_t weight() const { return max(tiles, 1u); }
 };
 
-// The keys that row r sees: none for a request outside the tables.
+// None for a request outside the tables.
+template <uint32_t kKeys>
 __device__ __forceinline__ Span span_of(const DecodeArgs& a, uint32_t r) {
     Span s;
     s.hi = min(max(a.lens[r], 0), (int32_t)a.max_len);
     const uint32_t request = a.rows ? (uint32_t)a.rows[r] : r;
     if (request >= a.requests) s.hi = 0;
     s.lo = a.window && (int64_t)s.hi > a.window ? s.hi - (int32_t)a.window : 0;
-    s.tiles = (uint32_t)((s.hi + kTile - 1) / kTile - s.lo / kTile);  // max_len leaves room for + 31
+    s.tiles = ((uint32_t)s.hi + kKeys - 1) / kKeys - (uint32_t)s.lo / kKeys;
     return s;
 }
 
-__device__ __forceinline__ uint32_t parts_of(const Span& s, uint32_t part_tiles) {
-    return min(max((s.tiles + part_tiles - 1) / part_tiles, 1u), (uint32_t)kMaxParts);
-}
+// Where a wave starts.  The tiles of all rows stand in one line (a row without keys takes
+// the place of one, for its zeros to be written); share p of it is [p each, (p + 1) each),
+// whatever rows that is.  So every share is as long as every other, however the lengths
+// differ.
+struct Share {
+    uint32_t each, from, to;  // tiles of a share; this one's place in the line
+    uint32_t row, row_at;     // its first row, and that row's place
+    Span span;                // of that row
+};
 
-__device__ __forceinline__ void fill(Part& p, uint32_t row, const Span& s, uint32_t parts, uint32_t part, uint32_t place) {
-    const uint32_t base = (uint32_t)(s.lo / kTile);
-    p.row = row;
-    p.lo = s.lo;
-    p.hi = s.hi;
-    p.parts = parts;
-    p.part = part;
-    p.place = place;
-    // tiles spread evenly: part i has (i + 1) n / parts - i n / parts of them
-    p.tile0 = base + (uint32_t)((uint64_t)part * s.tiles / parts);
-    p.tile1 = base + (uint32_t)((uint64_t)(part + 1) * s.tiles / parts);
-}
-
-// The item-th part of the call, or false.  A part has about total / target_parts tiles: the
-// lengths of the call alone decide, so long rows beside short ones are cut into as many
-// parts as their share of the work.
-template <int W>
-__device__ __forceinline__ bool find_part(const DecodeArgs& a, uint32_t item, Part& out) {
+template <uint32_t kKeys, int W>
+__device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Share& out) {
     const uint32_t lane = threadIdx.x & 63;
+    auto place = [&](uint32_t total) {
+        out.each = (total + a.shares - 1) / a.shares;
+        out.from = min(p * out.each, total);  // below 2^32: total < 2^31, p < 2 shares but for few tiles
+        out.to = min(out.from + out.each, total);
+        return out.from < total;
+    };
     if (a.n_rows <= 64) {  // every wave by itself
         Span s = {0, 0, 0};
-        if (lane < a.n_rows) s = span_of(a, lane);
-        const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)wave_sums(s.tiles), 63);
-        const uint32_t part_tiles = max(a.min_tiles, (total + a.target_parts - 1) / a.target_parts);
-        const uint32_t n = lane < a.n_rows ? parts_of(s, part_tiles) : 0;
-        const uint32_t upto = wave_sums(n), places = wave_sums(n > 1 ? n : 0);
-        const uint64_t hit = __ballot(item >= upto - n && item < upto);
-        if (!hit) return false;
-        const int at = __ffsll((unsigned long long)hit) - 1;
-        s.lo = __builtin_amdgcn_readlane(s.lo, at);
-        s.hi = __builtin_amdgcn_readlane(s.hi, at);
-        s.tiles = (uint32_t)__builtin_amdgcn_readlane((int)s.tiles, at);
-        const uint32_t parts = (uint32_t)__builtin_amdgcn_readlane((int)n, at);
-        fill(out, (uint32_t)at, s, parts, item - ((uint32_t)__builtin_amdgcn_readlane((int)upto, at) - parts),
-             (uint32_t)__builtin_amdgcn_readlane((int)places, at) - (parts > 1 ? parts : 0));
+        uint32_t n = 0;
+        if (lane < a.n_rows) {
+            s = span_of<kKeys>(a, lane);
+            n = s.weight();
+        }
+        const uint32_t upto = wave_sums(n);
+        if (!place((uint32_t)__builtin_amdgcn_readlane((int)upto, 63))) return false;
+        const int at = __ffsll((unsigned long long)__ballot(out.from >= upto - n && out.from < upto)) - 1;
+        out.row = (uint32_t)at;
+        out.row_at = (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), at);
+        out.span.lo = __builtin_amdgcn_readlane(s.lo, at);
+        out.span.hi = __builtin_amdgcn_readlane(s.hi, at);
+        out.span.tiles = (uint32_t)__builtin_amdgcn_readlane((int)s.tiles, at);
         return true;
     }
-    __shared__ uint32_t wave_total[2][W], found[7];
+    // each thread sums some rows; the one whose rows pass a wave's start looks through them
+    __shared__ uint32_t wave_total[W], start[W], found[W][2];
     const uint32_t wave = threadIdx.x >> 6;
     const uint32_t each = (a.n_rows + 64 * W - 1) / (64 * W);
     const uint32_t r0 = min(threadIdx.x * each, a.n_rows), r1 = min(r0 + each, a.n_rows);
-    uint32_t v = 0;
-    for (uint32_t r = r0; r < r1; ++r) v += span_of(a, r).tiles;
-    uint32_t sum = wave_sums(v);
-    if (lane == 63) wave_total[0][wave] = sum;
-    if (threadIdx.x == 0) found[0] = 0xFFFFFFFFu;
+    uint32_t n = 0;
+    for (uint32_t r = r0; r < r1; ++r) n += span_of<kKeys>(a, r).weight();
+    uint32_t upto = wave_sums(n);
+    if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
     uint32_t total = 0;
-    for (int w = 0; w < W; ++w) total += wave_total[0][w];
-    const uint32_t part_tiles = max(a.min_tiles, (total + a.target_parts - 1) / a.target_parts);
-    uint32_t n = 0, split = 0;
-    for (uint32_t r = r0; r < r1; ++r) {
-        const uint32_t p = parts_of(span_of(a, r), part_tiles);
-        n += p;
-        split += p > 1 ? p : 0;
+    for (uint32_t w = 0; w < W; ++w) {
+        if (w == wave) upto += total;
+        total += wave_total[w];
     }
-    uint32_t upto = wave_sums(n), places = wave_sums(split);
+    const bool any = place(total);
+    if (lane == 0) start[wave] = out.from;
     __syncthreads();
-    if (lane == 63) {
-        wave_total[0][wave] = upto;
-        wave_total[1][wave] = places;
-    }
-    __syncthreads();
-    upto -= n;
-    places -= split;
-    for (uint32_t w = 0; w < wave; ++w) {
-        upto += wave_total[0][w];
-        places += wave_total[1][w];
-    }
-    if (item >= upto && item < upto + n) {
-        for (uint32_t r = r0; r < r1; ++r) {
-            const Span s = span_of(a, r);
-            const uint32_t p = parts_of(s, part_tiles);
-            if (item < upto + p) {
-                found[0] = r;
-                found[1] = p;
-                found[2] = item - upto;
-                found[3] = places;
-                found[4] = (uint32_t)s.lo;
-                found[5] = (uint32_t)s.hi;
-                found[6] = s.tiles;
-                break;
+    for (uint32_t w = 0; w < W; ++w) {
+        const uint32_t from = start[w];
+        if (from >= upto - n && from < upto) {
+            uint32_t at = upto - n, r = r0;
+            for (; r + 1 < r1; ++r) {
+                const uint32_t weight = span_of<kKeys>(a, r).weight();
+                if (from < at + weight) break;
+                at += weight;
             }
-            upto += p;
-            places += p > 1 ? p : 0;
+            found[w][0] = r;
+            found[w][1] = at;
         }
     }
     __syncthreads();
-    if (found[0] == 0xFFFFFFFFu) return false;
-    Span s;
-    s.lo = (int32_t)found[4];
-    s.hi = (int32_t)found[5];
-    s.tiles = found[6];
-    fill(out, found[0], s, found[1], found[2], found[3]);
+    if (!any) return false;
+    out.row = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[wave][0]);
+    out.row_at = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[wave][1]);
+    out.span = span_of<kKeys>(a, out.row);
     return true;
 }
 
-template <int D, class T, bool F8, int W>
-__global__ __launch_bounds__(64 * W) void decode_kernel(DecodeArgs a) {
+template <int D, class T, bool F8, int kSub, int W>
+__global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(DecodeArgs a) {
     constexpr int kEl = F8 ? 1 : 2;           // bytes of a cache element
+    constexpr uint32_t kKeys = 32 * kSub;     // keys of a tile, in kSub tiles of 32
     constexpr int kSteps = D / 32;            // MFMAs over head_dim of the first product
     constexpr int kTiles = D / 16;            // 16-dimension tiles of the second
     constexpr int kKWords = kSteps * 2 * kEl; // dwords of a key in a lane
@@ -252,34 +231,38 @@ __global__ __launch_bounds__(64 * W) void decode_kernel(DecodeArgs a) {
     // V in chunks of 128, 64 and 32 dimensions, of which a lane holds 8, 4 and 2
     constexpr int kFull = D / 128, kRest = D % 128;
     constexpr bool kHas64 = kRest >= 64, kHas32 = kRest % 64 != 0;
-    constexpr int kRow = D + 4;  // LDS row of a head: neighbours start four banks apart
 
-    // Two uses, one after the other: accumulators of half the waves; weights of a row's
-    // parts and the sums of their groups.
-    constexpr int kRed = W / 2 * kHeadTile * kRow;
-    constexpr int kJoin = kMaxParts * kHeadTile + 64 * W * 4;
-    __shared__ __attribute__((aligned(16))) float red[kRed > kJoin ? kRed : kJoin];
-    __shared__ float wave_m[W][kHeadTile], wave_l[W][kHeadTile], all_m[kHeadTile], all_l[kHeadTile];
-    __shared__ uint32_t is_last;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
 
-    // Workgroups go round the 8 XCDs by index; those of one key head's head tiles read the
-    // same keys and take the same XCD, whose L2 then reads them once.
-    const uint32_t y = blockIdx.x >> 3;
-    const uint32_t head_tile = y - a.by_head_tiles.div(y) * a.by_head_tiles.d;
-    const uint32_t pos = a.by_head_tiles.div(y) * 8 + (blockIdx.x & 7);
-    const uint32_t item = a.by_kv_heads.div(pos), kv = pos - item * a.by_kv_heads.d;
-    Part part;
-    if (!find_part<W>(a, item, part)) return;
+    // Waves in line: the units (key heads, or tiles of their query heads) of share 0, of
+    // share 1, ...; workgroups go round the 8 XCDs by index, and each XCD takes one eighth of
+    // the line.  So the heads of a share run side by side: in a cache of
+    // [tokens][heads][dims] they read whole stretches of memory together (537 MB of keys and
+    // values in bf16, heads of 128, loads alone: 88 us; a workgroup to a head: 95 us).
+    const uint32_t line = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const uint32_t units = (uint32_t)(a.kv_heads * a.head_tiles), w_no = line * W + (uint32_t)wave;
+    const uint32_t share_no = a.by_units.div(w_no), unit = w_no - share_no * units;
+    const uint32_t kv = a.by_head_tiles.div(unit), head_tile = unit - kv * (uint32_t)a.head_tiles;
+    Share share;
+    if (!find_share<kKeys, W>(a, share_no, share)) {
+        if (!a.by_row && unit == 0 && share_no < a.shares && lane == 0) a.split[share_no] = Split{0, 0, 0};
+        return;
+    }
     const int heads = min(kHeadTile, a.group - (int)head_tile * kHeadTile);  // columns in use
     const int head0 = (int)kv * a.group + (int)head_tile * kHeadTile;
+
+    for (;;) {
+    // the share's part of a row: tiles [tile0, tile1) of keys [part.lo, part.hi)
+    const Span part = share.span;
+    const uint32_t row = share.row, row_end = share.row_at + part.weight(), here_end = min(row_end, share.to);
+    const uint32_t tile0 = (uint32_t)part.lo / kKeys + (share.from - share.row_at);
+    const uint32_t tile1 = part.tiles ? (uint32_t)part.lo / kKeys + (here_end - share.row_at) : tile0;
 
     // q^T: lane holds column `col`, eight dimensions a step, in the order of a key's loads
     u32x4 qf[kSteps];
     {
-        const uint8_t* q = a.q + part.row * a.q_stride + (int64_t)(head0 + min(col, heads - 1)) * D * 2;
+        const uint8_t* q = a.q + row * a.q_stride + (int64_t)(head0 + min(col, heads - 1)) * D * 2;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
             const int dim = F8 && (st | 1) < kSteps ? (st >> 1) * 64 + g * 16 + (st & 1) * 8 : st * 32 + g * 8;
@@ -293,109 +276,139 @@ __global__ __launch_bounds__(64 * W) void decode_kernel(DecodeArgs a) {
     for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0;
 
-    const uint32_t request = a.rows ? (uint32_t)a.rows[part.row] : part.row;
+    const uint32_t request = a.rows ? (uint32_t)a.rows[row] : row;
     const int32_t* table = a.tables + (int64_t)request * a.table_stride;
     const int32_t first_group = part.lo & ~7, last_group = (part.hi - 1) & ~7;
     const uint8_t* k_lane = a.cache.k + kv * a.cache.head_stride + g * 16;
     const uint8_t* v_base = a.cache.v + kv * a.cache.head_stride;
     const int kg = col >> 2, k_row = col & 3;  // the lane's key of tile s: 8 kg + 4 s + k_row
 
-    // the eight keys from 8 * grp of a tile on: their page's column, kept inside [lo, hi)
-    auto group_at = [&](uint32_t tile, int grp) -> int32_t {
-        return min(max((int32_t)(tile * kTile) + 8 * grp, first_group), last_group);
+    // the eight keys from 8 * grp of a tile's 32 `sub` on, kept inside the row's keys; the
+    // column of their page, and their place in the cache
+    auto group_at = [&](uint32_t tile, int sub, int grp) -> int32_t {
+        return min(max((int32_t)(tile * kKeys) + 32 * sub + 8 * grp, first_group), last_group);
     };
-    auto page_at = [&](int32_t key) -> int32_t { return table[a.cache.page.div((uint32_t)key)]; };
+    auto page_at = [&](int32_t key) -> int32_t { return table[a.cache.page.div_by_many((uint32_t)key)]; };
     auto offset_of = [&](int32_t page, int32_t key) -> int64_t {
-        const uint32_t in_page = (uint32_t)key - a.cache.page.div((uint32_t)key) * a.cache.page.d;
+        const uint32_t in_page = (uint32_t)key - a.cache.page.div_by_many((uint32_t)key) * a.cache.page.d;
         return ((uint32_t)page < a.cache.n_pages ? (int64_t)page * a.cache.page_stride : 0) +
                (int64_t)in_page * a.cache.token_stride;
     };
+    struct Pages {
+        int32_t k[kSub], v[kSub];
+    };
+    auto pages_of = [&](uint32_t tile) {
+        Pages p;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            p.k[u] = page_at(group_at(tile, u, kg));
+            p.v[u] = page_at(group_at(tile, u, g));
+        }
+        return p;
+    };
 
-    uint32_t kraw[2][kKWords], vraw[8][kVWords];
-    auto load_k = [&](uint32_t tile, int32_t page) {
-        const uint8_t* p = k_lane + offset_of(page, group_at(tile, kg)) + k_row * a.cache.token_stride;
+    uint32_t kraw[kSub][2][kKWords], vraw[kSub][8][kVWords];
+    auto load_k = [&](uint32_t tile, const Pages& pages) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const uint8_t* ps = p + 4 * s * a.cache.token_stride;
-            if constexpr (F8) {
+        for (int u = 0; u < kSub; ++u) {
+            const uint8_t* p = k_lane + offset_of(pages.k[u], group_at(tile, u, kg)) + k_row * a.cache.token_stride;
 #pragma unroll
-                for (int c = 0; c < kSteps / 2; ++c) load<16>(ps + c * 64, &kraw[s][4 * c]);
-                if constexpr (kSteps & 1) load<8>(ps - g * 8 + (kSteps - 1) * 32, &kraw[s][2 * (kSteps - 1)]);
-            } else {
+            for (int s = 0; s < 2; ++s) {
+                const uint8_t* ps = p + 4 * s * a.cache.token_stride;
+                if constexpr (F8) {
 #pragma unroll
-                for (int st = 0; st < kSteps; ++st) load<16>(ps + st * 64, &kraw[s][4 * st]);
+                    for (int c = 0; c < kSteps / 2; ++c) load<16>(ps + c * 64, &kraw[u][s][4 * c]);
+                    if constexpr (kSteps & 1) load<8>(ps - g * 8 + (kSteps - 1) * 32, &kraw[u][s][2 * (kSteps - 1)]);
+                } else {
+#pragma unroll
+                    for (int st = 0; st < kSteps; ++st) load<16>(ps + st * 64, &kraw[u][s][4 * st]);
+                }
             }
         }
     };
-    auto load_v = [&](uint32_t tile, int32_t page) {
-        const uint8_t* p = v_base + offset_of(page, group_at(tile, g));
+    auto load_v = [&](uint32_t tile, const Pages& pages) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint8_t* pj = p + j * a.cache.token_stride;
+        for (int u = 0; u < kSub; ++u) {
+            const uint8_t* p = v_base + offset_of(pages.v[u], group_at(tile, u, g));
 #pragma unroll
-            for (int c = 0; c < kFull; ++c) load<8 * kEl>(pj + (c * 128 + col * 8) * kEl, &vraw[j][c * 2 * kEl]);
-            if constexpr (kHas64) load<4 * kEl>(pj + (kFull * 128 + col * 4) * kEl, &vraw[j][kFull * 2 * kEl]);
-            if constexpr (kHas32)
-                load<2 * kEl>(pj + (kFull * 128 + kHas64 * 64 + col * 2) * kEl, &vraw[j][kFull * 2 * kEl + kHas64 * kEl]);
+            for (int j = 0; j < 8; ++j) {
+                const uint8_t* pj = p + j * a.cache.token_stride;
+#pragma unroll
+                for (int c = 0; c < kFull; ++c) load<8 * kEl>(pj + (c * 128 + col * 8) * kEl, &vraw[u][j][c * 2 * kEl]);
+                if constexpr (kHas64) load<4 * kEl>(pj + (kFull * 128 + col * 4) * kEl, &vraw[u][j][kFull * 2 * kEl]);
+                if constexpr (kHas32)
+                    load<2 * kEl>(pj + (kFull * 128 + kHas64 * 64 + col * 2) * kEl,
+                                  &vraw[u][j][kFull * 2 * kEl + kHas64 * kEl]);
+            }
         }
     };
 
-    uint32_t tile = part.tile0 + wave;
-    if (tile < part.tile1) {
-        int32_t k_page = page_at(group_at(tile, kg)), v_page = page_at(group_at(tile, g));
-        uint32_t next = min(tile + W, part.tile1 - 1);
-        int32_t k_next = page_at(group_at(next, kg)), v_next = page_at(group_at(next, g));
-        load_k(tile, k_page);
-        load_v(tile, v_page);
+    uint32_t tile = tile0;
+    if (tile < tile1) {
+        Pages now = pages_of(tile);
+        // the tile after the last is the last again: loads without a branch around them,
+        // so that the wait for the present values need not cover them
+        uint32_t next = tile + 1 < tile1 ? tile + 1 : tile;
+        Pages then = pages_of(next);
+        load_k(tile, now);
+        load_v(tile, now);
         for (;;) {
-            const bool more = tile + W < part.tile1;
             // first product
-            f32x4 sc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+            f32x4 sc[kSub][2];
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
-                    u32x4 kf;
-                    if constexpr (F8) {
-                        const uint32_t w0 = kraw[s][2 * st], w1 = kraw[s][2 * st + 1];
-                        kf = u32x4{T::template from_f8<false>(w0), T::template from_f8<true>(w0),
-                                   T::template from_f8<false>(w1), T::template from_f8<true>(w1)};
-                    } else {
-                        kf = u32x4{kraw[s][4 * st], kraw[s][4 * st + 1], kraw[s][4 * st + 2], kraw[s][4 * st + 3]};
+                for (int s = 0; s < 2; ++s) {
+                    sc[u][s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int st = 0; st < kSteps; ++st) {
+                        u32x4 kf;
+                        if constexpr (F8) {
+                            const uint32_t w0 = kraw[u][s][2 * st], w1 = kraw[u][s][2 * st + 1];
+                            kf = u32x4{T::template from_f8<false>(w0), T::template from_f8<true>(w0),
+                                       T::template from_f8<false>(w1), T::template from_f8<true>(w1)};
+                        } else {
+                            kf = u32x4{kraw[u][s][4 * st], kraw[u][s][4 * st + 1], kraw[u][s][4 * st + 2],
+                                       kraw[u][s][4 * st + 3]};
+                        }
+                        sc[u][s] = T::mfma(kf, qf[st], sc[u][s]);
                     }
-                    sc[s] = T::mfma(kf, qf[st], sc[s]);
                 }
             // the pages of the tile after the next, then the next keys: their pages came
             // with loads that have been waited for
-            int32_t k_after = 0, v_after = 0;
-            if (more) {
-                const uint32_t after = min(tile + 2 * W, part.tile1 - 1);
-                k_after = page_at(group_at(after, kg));
-                v_after = page_at(group_at(after, g));
-                load_k(tile + W, k_next);
-            }
+            const uint32_t after = next + 1 < tile1 ? next + 1 : next;
+            const Pages later = pages_of(after);
+            load_k(next, then);
 
-            float x[8];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * s + i] = sc[s][i] * a.scale;
             // keys outside the row's or on no page of the cache: only a row's first and
             // last tiles, and broken tables, have them
-            const int32_t key0 = (int32_t)(tile * kTile) + 8 * g;
-            const bool on_page = (uint32_t)v_page < a.cache.n_pages;
-            const bool whole = on_page && key0 >= part.lo && key0 + 8 <= part.hi;
+            float x[kSub][8];
+            const int32_t key0 = (int32_t)(tile * kKeys) + 8 * g;
+            bool whole = key0 >= part.lo && key0 + (int32_t)kKeys - 24 <= part.hi;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[u][j] = sc[u][j / 4][j % 4] * a.scale;
+                whole = whole && (uint32_t)now.v[u] < a.cache.n_pages;
+            }
             if (!__all(whole)) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool seen = on_page && key0 + j >= part.lo && key0 + j < part.hi;
-                    x[j] = seen ? x[j] : -INFINITY;
+                for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                    for (int w = 0; w < kVWords; ++w) vraw[j][w] = seen ? vraw[j][w] : 0;  // 0 * NaN is NaN
-                }
+                    for (int j = 0; j < 8; ++j) {
+                        const int32_t key = key0 + 32 * u + j;
+                        const bool seen = (uint32_t)now.v[u] < a.cache.n_pages && key >= part.lo && key < part.hi;
+                        x[u][j] = seen ? x[u][j] : -INFINITY;
+#pragma unroll
+                        for (int w = 0; w < kVWords; ++w) vraw[u][j][w] = seen ? vraw[u][j][w] : 0;  // 0 * NaN is NaN
+                    }
             }
-            const float top = column_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                               fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+            float top = x[0][0];
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, x[u][j]);
+            top = column_max(top);
             if (__any(top > m)) {
                 const float to = fmaxf(m, top);
                 const float by = exp2_of(m - above(to));
@@ -405,232 +418,152 @@ __global__ __launch_bounds__(64 * W) void decode_kernel(DecodeArgs a) {
                 for (int i = 0; i < kTiles; ++i) acc[i] *= by;
             }
             const float base = above(m);
-            u32x4 p_high, p_low;
+            // second product, p as the sum of kParts 16-bit parts
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float p0 = exp2_of(x[j] - base), p1 = exp2_of(x[j + 1] - base);
-                l += p0 + p1;
-                const uint32_t h = T::pair(p0, p1);
-                p_high[j / 2] = h;
-                p_low[j / 2] = T::pair(p0 - T::low(h), p1 - T::high(h));
-            }
-            // second product
-            auto add = [&](int t, u32x4 vf) {
-                acc[t] = T::mfma(vf, p_high, acc[t]);
-                acc[t] = T::mfma(vf, p_low, acc[t]);
-            };
-            auto chunk = [&](int tile0, int word0, auto width_tag) {
-                constexpr int kWidth = decltype(width_tag)::value;
-                if constexpr (F8) {
+            for (int u = 0; u < kSub; ++u) {
+                constexpr int kParts = T::kExactParts;
+                u32x4 pf[kParts];
 #pragma unroll
-                    for (int w = 0; w < (kWidth + 3) / 4; ++w) {
-                        u32x4 f[4];
+                for (int j = 0; j < 8; j += 2) {
+                    float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
+                    l += r0 + r1;
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            const uint32_t v0 = vraw[2 * p][word0 + w], v1 = vraw[2 * p + 1][word0 + w];
-                            const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
-                            f[0][p] = T::template from_f8<false>(lo);
-                            f[1][p] = T::template from_f8<true>(lo);
-                            if constexpr (kWidth >= 4) {
-                                const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
-                                f[2][p] = T::template from_f8<false>(hi);
-                                f[3][p] = T::template from_f8<true>(hi);
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < (kWidth < 4 ? kWidth : 4); ++e) add(tile0 + 4 * w + e, f[e]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kWidth; ++e) {
-                        u32x4 f;
-#pragma unroll
-                        for (int p = 0; p < 4; ++p)
-                            f[p] = __builtin_amdgcn_perm(vraw[2 * p + 1][word0 + e / 2], vraw[2 * p][word0 + e / 2],
-                                                         e & 1 ? 0x07060302u : 0x05040100u);
-                        add(tile0 + e, f);
+                    for (int k = 0; k < kParts; ++k) {
+                        const uint32_t h = T::pair(r0, r1);
+                        pf[k][j / 2] = h;
+                        r0 -= T::low(h);
+                        r1 -= T::high(h);
                     }
                 }
-            };
+                auto add = [&](int t, u32x4 vf) {
 #pragma unroll
-            for (int c = 0; c < kFull; ++c) chunk(8 * c, c * 2 * kEl, std::integral_constant<int, 8>{});
-            if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
-            if constexpr (kHas32)
-                chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
-            if (!more) break;
-            load_v(tile + W, v_next);
-            tile += W;
-            v_page = v_next;
-            k_next = k_after;
-            v_next = v_after;
+                    for (int k = 0; k < kParts; ++k) acc[t] = T::mfma(vf, pf[k], acc[t]);
+                };
+                auto chunk = [&](int t0, int word0, auto width_tag) {
+                    constexpr int kWidth = decltype(width_tag)::value;
+                    if constexpr (F8) {
+#pragma unroll
+                        for (int w = 0; w < (kWidth + 3) / 4; ++w) {
+                            u32x4 f[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const uint32_t v0 = vraw[u][2 * q][word0 + w], v1 = vraw[u][2 * q + 1][word0 + w];
+                                const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
+                                f[0][q] = T::template from_f8<false>(lo);
+                                f[1][q] = T::template from_f8<true>(lo);
+                                if constexpr (kWidth >= 4) {
+                                    const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
+                                    f[2][q] = T::template from_f8<false>(hi);
+                                    f[3][q] = T::template from_f8<true>(hi);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < (kWidth < 4 ? kWidth : 4); ++e) add(t0 + 4 * w + e, f[e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kWidth; ++e) {
+                            u32x4 f;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                f[q] = __builtin_amdgcn_perm(vraw[u][2 * q + 1][word0 + e / 2], vraw[u][2 * q][word0 + e / 2],
+                                                             e & 1 ? 0x07060302u : 0x05040100u);
+                            add(t0 + e, f);
+                        }
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < kFull; ++c) chunk(8 * c, c * 2 * kEl, std::integral_constant<int, 8>{});
+                if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
+                if constexpr (kHas32)
+                    chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
+            }
+            if (next == tile) break;
+            load_v(next, then);
+            tile = next;
+            next = after;
+            now = then;
+            then = later;
         }
     }
 
-    // The waves' sums joined: to a common maximum, then the upper half's accumulators into
-    // the lower half's, then the lower half's over all threads.
     l = column_sum(l);
-    if (g == 0) {
-        wave_m[wave][col] = m;
-        wave_l[wave][col] = l;
-    }
-    __syncthreads();
-    float top = -INFINITY, sum = 0;
+    // accumulator i of tile t is dimension chunk + (4 g + i) * width + (t in the chunk): a
+    // lane stores the chunk's width neighbours at a time
+    auto each_run = [&](auto&& f) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, wave_m[w][col]);
-    const float base = above(top);
+        for (int c = 0; c < kTiles;) {
+            const int width = c / 8 < kFull ? 8 : kHas64 && c < 8 * kFull + 4 ? 4 : 2;
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum += exp2_of(wave_m[w][col] - base) * wave_l[w][col];
-    const float by = exp2_of(m - base);
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) acc[i] *= by;
-    if (wave == 0 && g == 0) {
-        all_m[col] = top;
-        all_l[col] = sum;
-    }
-    // accumulator i of tile t is dimension chunk + (4 g + i) * width + (t in the chunk)
-    auto each_acc = [&](auto&& f) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            const int c = t / 8 < kFull ? t / 8 * 8 : kHas64 && t < 8 * kFull + 4 ? 8 * kFull : 8 * kFull + 4 * kHas64;
-            const int width = t / 8 < kFull ? 8 : kHas64 && t < 8 * kFull + 4 ? 4 : 2;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f(t, i, c * 16 + (4 * g + i) * width + (t - c));
+            for (int i = 0; i < 4; ++i) f(c, i, width, c * 16 + (4 * g + i) * width);
+            c += width;
         }
     };
-    float* mine = red + ((wave % (W / 2)) * kHeadTile + col) * kRow;
-    if (wave >= W / 2 && col < heads) each_acc([&](int t, int i, int d) { mine[d] = acc[t][i]; });
-    __syncthreads();
-    if (wave < W / 2 && col < heads) each_acc([&](int t, int i, int d) { mine[d] += acc[t][i]; });
-    __syncthreads();
-
-    const int outs = heads * (D / 4);  // fours of the output
-    const uint32_t units = (uint32_t)(a.kv_heads * a.head_tiles), unit = kv * a.head_tiles + head_tile;
-    auto store = [&](int o, f32x4 v, float total) {
-        const int h = o / (D / 4), d = o % (D / 4) * 4;
-        const float over = total > 0 || total != total ? a.cache.v_scale / total : 0.0f;
-        v *= over;
-        const int64_t at = (int64_t)(head0 + h) * D + d;
-        if (a.out_f32)
-            *reinterpret_cast<f32x4*>(a.out + part.row * a.out_stride + at * 4) = v;
-        else
-            *reinterpret_cast<uint2*>(a.out + part.row * a.out_stride + at * 2) =
-                make_uint2(T::pair(v[0], v[1]), T::pair(v[2], v[3]));
-    };
-    auto store_lse = [&](int h, float most, float total) {
-        if (a.lse)
-            a.lse[(int64_t)part.row * a.q_heads + head0 + h] =
-                total == 0 ? -INFINITY : (most + __builtin_amdgcn_logf(total)) * 0.693147180559945309f;
-    };
-    auto waves_sum = [&](int o) {
-        const float* r = red + o / (D / 4) * kRow + o % (D / 4) * 4;
-        f32x4 v = *reinterpret_cast<const f32x4*>(r);
+    // the row's shares: all but the first begin inside it
+    const uint32_t first_share = share.row_at / share.each, parts = (row_end - 1) / share.each - first_share + 1;
+    if (a.by_row && unit == 0 && lane == 0 && share_no == first_share) a.split[row] = Split{row, first_share, parts};
+    if (col < heads) {
+        if (parts == 1) {
+            const float over = l > 0 || l != l ? a.cache.v_scale / l : 0.0f;
+            const int64_t at = (int64_t)(head0 + col) * D;
+            if (a.out_f32) {
+                float* o = reinterpret_cast<float*>(a.out + row * a.out_stride) + at;
+                each_run([&](int t, int i, int width, int d) {
+                    if (width >= 4) {
 #pragma unroll
-        for (int w = 1; w < W / 2; ++w) v += *reinterpret_cast<const f32x4*>(r + w * kHeadTile * kRow);
-        return v;
-    };
-    if (part.parts == 1) {
-        for (int o = tid; o < outs; o += 64 * W) store(o, waves_sum(o), all_l[o / (D / 4)]);
-        if (tid < heads) store_lse(tid, all_m[tid], all_l[tid]);
-        return;
-    }
-
-    // A part of a split row: its sums to the workspace, past this XCD's L2 (sc1), and the
-    // last of the row's workgroups adds the parts.  As in the batched GEMV's K split: each
-    // wave's stores are acknowledged (vmcnt 0) before the barrier that precedes the count,
-    // the loads follow the count's return and miss this XCD's L2 (sc1); no workgroup waits
-    // for another.
-    constexpr int kSc1 = 16;
-    const __amdgpu_buffer_rsrc_t acc_rsrc = qmm::make_rsrc(a.part_acc, a.part_acc_bytes);
-    const __amdgpu_buffer_rsrc_t ml_rsrc = qmm::make_rsrc(a.part_ml, a.part_ml_bytes);
-    const int tile_heads = min(kHeadTile, a.group);  // heads of a workspace entry
-    auto entry = [&](uint32_t i) { return ((part.place + i) * units + unit) * (uint32_t)tile_heads; };
-    for (int o = tid; o < outs; o += 64 * W)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, waves_sum(o)), acc_rsrc,
-                                               (int)(entry(part.part) * (D * 4) + o * 16), 0, kSc1);
-    if (tid < heads) {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(all_m[tid]), __float_as_uint(all_l[tid])}, ml_rsrc,
-                                              (int)((entry(part.part) + tid) * 8), 0, kSc1);
-    }
-    __builtin_amdgcn_s_waitcnt(qmm::vmcnt_only(0));
-    __syncthreads();
-    if (tid == 0) {
-        uint32_t* count = a.counters + (size_t)part.place * units + unit;
-        const bool last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == part.parts - 1;
-        if (last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        is_last = last;
-    }
-    __syncthreads();
-    if (!is_last) return;
-
-    // weight of part i for each head, in `red`
-    for (int h = wave; h < heads; h += W) {
-        float pm[kMaxParts / 64], pl[kMaxParts / 64], most = -INFINITY, total = 0;
+                        for (int e = 0; e < width; e += 4)
+                            *reinterpret_cast<f32x4*>(o + d + e) =
+                                f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]} * over;
+                    } else {
+                        *reinterpret_cast<float2*>(o + d) = make_float2(acc[t][i] * over, acc[t + 1][i] * over);
+                    }
+                });
+            } else {
+                uint16_t* o = reinterpret_cast<uint16_t*>(a.out + row * a.out_stride) + at;
+                each_run([&](int t, int i, int width, int d) {
+                    uint32_t w[4];
 #pragma unroll
-        for (int c = 0; c < kMaxParts / 64; ++c) {
-            const uint32_t i = c * 64 + lane;
-            pm[c] = -INFINITY;
-            pl[c] = 0;
-            if (i < part.parts) {
-                const auto v = __builtin_amdgcn_raw_buffer_load_b64(ml_rsrc, (int)((entry(i) + h) * 8), 0, kSc1);
-                pm[c] = __uint_as_float(v[0]);
-                pl[c] = __uint_as_float(v[1]);
+                    for (int e = 0; e < width; e += 2) w[e / 2] = T::pair(acc[t + e][i] * over, acc[t + e + 1][i] * over);
+                    if (width == 8)
+                        *reinterpret_cast<uint4*>(o + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                    else if (width == 4)
+                        *reinterpret_cast<uint2*>(o + d) = make_uint2(w[0], w[1]);
+                    else
+                        *reinterpret_cast<uint32_t*>(o + d) = w[0];
+                });
             }
-            most = fmaxf(most, pm[c]);
-        }
+            if (a.lse && g == 0) a.lse[(int64_t)row * a.q_heads + head0 + col] = log_sum(m, l);
+        } else {
+            // an entry of the share: 1 for a row that starts in it, 0 for one that goes on
+            const int64_t entry = ((int64_t)(2 * share_no + (share_no == first_share)) * a.q_heads + head0 + col);
+            float* o = a.part_acc + entry * D;
+            each_run([&](int t, int i, int width, int d) {
+                if (width >= 4) {
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-#pragma unroll
-        for (int c = 0; c < kMaxParts / 64; ++c) {
-            const uint32_t i = c * 64 + lane;
-            const float w = exp2_of(pm[c] - above(most));
-            if (i < part.parts) red[i * kHeadTile + h] = w;
-            total += w * pl[c];
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-        if (lane == 0) {
-            all_m[h] = most;
-            all_l[h] = total;
+                    for (int e = 0; e < width; e += 4)
+                        *reinterpret_cast<f32x4*>(o + d + e) =
+                            f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]};
+                } else {
+                    *reinterpret_cast<float2*>(o + d) = make_float2(acc[t][i], acc[t + 1][i]);
+                }
+            });
+            if (g == 0) a.part_ml[entry] = make_float2(m, l);
         }
     }
-    __syncthreads();
-    // groups of threads take every groups-th part; their sums are added in order
-    const int groups = max(64 * W / outs, 1);
-    f32x4* sums = reinterpret_cast<f32x4*>(red + kMaxParts * kHeadTile);
-    for (int o0 = 0; o0 < outs; o0 += 64 * W) {
-        const int grp = groups == 1 ? 0 : tid / outs, o = groups == 1 ? o0 + tid : tid % outs;
-        const bool active = grp < groups && o < outs;
-        f32x4 v = {0, 0, 0, 0};
-        if (active) {
-            const int h = o / (D / 4);
-#pragma unroll 8
-            for (uint32_t i = grp; i < part.parts; i += groups) {
-                const u32x4 r = __builtin_amdgcn_raw_buffer_load_b128(acc_rsrc, (int)(entry(i) * (D * 4) + o * 16), 0, kSc1);
-                v += __builtin_bit_cast(f32x4, r) * red[i * kHeadTile + h];
-            }
-        }
-        if (groups > 1) {
-            if (active) sums[tid] = v;
-            __syncthreads();
-            if (active && grp == 0)
-                for (int k = 1; k < groups; ++k) v += sums[k * outs + o];
-        }
-        if (active && grp == 0) store(o, v, all_l[o / (D / 4)]);
+    if (!a.by_row && unit == 0 && lane == 0 && here_end == share.to)
+        a.split[share_no] = here_end < row_end && share_no == first_share ? Split{row, first_share, parts} : Split{0, 0, 0};
+    if (here_end == share.to) return;
+    share.from = share.row_at = row_end;
+    share.row = row + 1;
+    share.span = span_of<kKeys>(a, row + 1);
     }
-    if (tid < heads) store_lse(tid, all_m[tid], all_l[tid]);
 }
-
-// Waves of a workgroup: eight where their registers let a CU hold two workgroups.
-template <int D>
-constexpr int decode_waves() { return D <= 128 ? 8 : 4; }
 
 template <int D, class T, bool F8>
 hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
-    constexpr int W = decode_waves<D>();
-    const uint64_t heads = (uint64_t)a.max_parts * a.kv_heads;
-    const uint64_t wgs = (heads + 7) / 8 * 8 * a.head_tiles;
-    hipLaunchKernelGGL((decode_kernel<D, T, F8, W>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a);
+    constexpr int W = kDecodeWaves, kSub = decode_subtiles(D, F8);
+    const uint64_t waves = (uint64_t)a.launch_shares * a.kv_heads * a.head_tiles, wgs = ((waves + W - 1) / W + 7) / 8 * 8;
+    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a);
     return hipGetLastError();
 }
 

@@ -22,6 +22,7 @@ struct FastDiv {
         m = (uint32_t)((((uint64_t)1 << (31 + l)) + div - 1) / div);
     }
     __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) >> shift : n; }
+    __device__ __forceinline__ uint32_t div_by_many(uint32_t n) const { return __umulhi(n, m) >> shift; }  // d > 1
 };
 
 // A cache as the kernels see it: strides in bytes.
@@ -83,12 +84,23 @@ struct RopeArgs {
 hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s);
 
 // ---- attn_decode_*.hip ---------------------------------------------------------------
-constexpr int kTile = 32;        // keys a wave takes at a time
+constexpr int kDecodeWaves = 4;  // waves of a workgroup
+// Keys that a wave takes at a time, in 32s: about 16 KB of keys and values.
+constexpr int decode_subtiles(int head_dim, bool f8) {
+    return f8 ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1) : head_dim <= 64 ? 2 : 1;
+}
 constexpr int kHeadTile = 16;    // query heads a workgroup serves (the MFMA's columns)
-constexpr int kMaxParts = 256;   // parts of one row
 constexpr int kMaxHeads = 1024;  // query heads
-constexpr int kRound = 1024;     // workgroups that decode_shape() aims at, at most
-constexpr size_t kCounters = 2 * (kRound + kMaxHeads);  // at least 2 ceil(kRound / units) units
+// Waves of a call, at most (one share each unless the units alone are more): one for each
+// SIMD.  Two or three raise the bytes in flight past what the memory needs, and then equal
+// shares end at different times (131071 keys, 8 heads of 128, bf16: the waves end between 73
+// and 104 us, the call takes 106 us instead of 99; 512 waves 117).
+constexpr int kRound = 1024;
+
+// A row of several parts (parts > 1), in shares first_share on.
+struct Split {
+    uint32_t row, first_share, parts;
+};
 
 struct DecodeArgs {
     Cache cache;
@@ -103,23 +115,23 @@ struct DecodeArgs {
     int32_t q_heads, kv_heads, group, head_tiles;
     int32_t out_f32;
     float scale;  // of a raw product, in powers of two: scale * k_scale * log2(e)
-    // The cut of long rows: parts of at least min_tiles tiles, about target_parts in all
-    // (for each of the units = kv_heads * head_tiles).
-    uint32_t target_parts, min_tiles, max_parts;
-    FastDiv by_kv_heads, by_head_tiles;
-    uint32_t* counters;  // [place of a split row's first part][units], 0 between calls
-    float* part_acc;     // [parts][units][heads of a tile][head_dim]
-    float* part_ml;      // [parts][units][heads of a tile][2]
-    uint32_t part_acc_bytes, part_ml_bytes;
+    // Shares of the call's tiles for each of the units = kv_heads * head_tiles, at most, and
+    // those that waves are launched for.
+    uint32_t shares, launch_shares;
+    FastDiv by_units, by_head_tiles;
+    // What the join reads: entries of split rows, and for each row (by_row: there are at
+    // most as many as shares) or each share the row that is split there.
+    float* part_acc;  // [shares][2][q_heads][head_dim]
+    float2* part_ml;  // [shares][2][q_heads]: maximum, sum
+    Split* split;     // [shares]
+    int32_t by_row;
 };
 
-// The cut for a call.
-struct DecodeShape {
-    uint32_t target_parts, min_tiles, max_parts;
-};
-DecodeShape decode_shape(int64_t rows, int kv_heads, int head_tiles, int head_dim, int64_t max_len);
-// Parts that the split rows of one call have at most (for each unit).
-int64_t decode_split_parts(int kv_heads, int head_tiles, int head_dim);
+// Shares of a call, at most.
+uint32_t decode_shares(int kv_heads, int head_tiles);
+
+// The parts of split rows joined into out and lse; after launch_decode_*.
+hipError_t launch_join(const DecodeArgs& a, int head_dim, int out_dtype, hipStream_t s);
 
 hipError_t launch_decode_bf16(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s);
 hipError_t launch_decode_f16(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s);

@@ -35,14 +35,16 @@ class DType(enum.IntEnum):
 
     @property
     def nbytes(self) -> int:
-        return (4, 2, 2, 1)[self]
+        return _NBYTES[self]
 
 
-def _need(buf, nbytes: int, what: str):
-    """The buffer's pointer, if it holds nbytes."""
-    if buf.nbytes < nbytes:
-        raise InvalidInput(f"{what} holds {buf.nbytes} bytes, {nbytes} are needed")
-    return buf.ptr
+# Calls build their argument structure and compare sizes in line: a step's smallest launches
+# take 3 - 4 us, which a helper call for each buffer would add half of.
+_NBYTES = (4, 2, 2, 1)  # of a DType
+
+
+def _short(what: str, buf, nbytes: int):
+    raise InvalidInput(f"{what} holds {buf.nbytes} bytes, {nbytes} are needed")
 
 
 def _rows_bytes(rows: int, stride: int, row: int, size: int) -> int:
@@ -66,9 +68,12 @@ class KVCache:
         self.d_k, self.d_v = d_k, d_v
         self.dtype, self.n_pages, self.page_size = dtype, int(n_pages), int(page_size)
         self.kv_heads, self.head_dim, self.layout = int(kv_heads), int(head_dim), layout
+        for name, buf in (("d_k", d_k), ("d_v", d_v)):
+            if buf.nbytes < nbytes:
+                _short(name, buf, nbytes)
         token, head = (kv_heads * head_dim, head_dim) if layout == "token" else (head_dim, page_size * head_dim)
-        self.desc = _native.KvCache(_need(d_k, nbytes, "d_k"), _need(d_v, nbytes, "d_v"), dtype, kv_heads, head_dim, page_size,
-                                    n_pages, page_size * kv_heads * head_dim, token, head, k_scale, v_scale)
+        self.desc = _native.KvCache(d_k.ptr, d_v.ptr, dtype, kv_heads, head_dim, page_size, n_pages,
+                                    page_size * kv_heads * head_dim, token, head, k_scale, v_scale)
 
     @classmethod
     def allocate(cls, dtype: DType, n_pages: int, page_size: int, kv_heads: int, head_dim: int, **kw) -> "KVCache":
@@ -99,8 +104,10 @@ class StepPlan:
             buf = (buffers or {}).get(name)
             if buf is None:
                 buf = DeviceBuffer(nbytes)
-            _need(buf, nbytes, name)
+            if buf.nbytes < nbytes:
+                _short(name, buf, nbytes)
             setattr(self, name, buf)
+        self._call = lib().openmini_kv_plan
 
     def run(self, d_cached, d_new, requests: int, d_tables, d_free, n_free: int, d_head=None, stream=None,
             table_stride: int | None = None) -> None:
@@ -109,12 +116,21 @@ class StepPlan:
         if requests > self.max_requests:
             raise InvalidInput(f"{requests} requests, planned for {self.max_requests}")
         stride = self.max_pages if table_stride is None else table_stride
-        a = _native.KvPlanArgs(_need(d_cached, 4 * requests, "d_cached"), _need(d_new, 4 * requests, "d_new"), requests,
-                               _need(d_free, 4 * n_free, "d_free"), n_free, d_head.ptr if d_head is not None else None,
-                               _need(d_tables, 4 * _rows_bytes(requests, stride, self.max_pages, 1), "d_tables"), stride,
-                               self.max_pages, self.page_size, self.max_tokens, self.starts.ptr, self.lens.ptr, self.rows.ptr,
-                               self.positions.ptr, self.slots.ptr, self.row_lens.ptr, self.counts.ptr)
-        check(lib().openmini_kv_plan(a, stream))
+        n, table_bytes = 4 * requests, 4 * _rows_bytes(requests, stride, self.max_pages, 1)
+        if d_cached.nbytes < n:
+            _short("d_cached", d_cached, n)
+        if d_new.nbytes < n:
+            _short("d_new", d_new, n)
+        if d_free.nbytes < 4 * n_free:
+            _short("d_free", d_free, 4 * n_free)
+        if d_tables.nbytes < table_bytes:
+            _short("d_tables", d_tables, table_bytes)
+        rc = self._call(_native.KvPlanArgs(
+            d_cached.ptr, d_new.ptr, requests, d_free.ptr, n_free, d_head.ptr if d_head is not None else None, d_tables.ptr, stride,
+            self.max_pages, self.page_size, self.max_tokens, self.starts.ptr, self.lens.ptr, self.rows.ptr, self.positions.ptr,
+            self.slots.ptr, self.row_lens.ptr, self.counts.ptr), stream)
+        if rc:
+            check(rc)
 
 
 # ---- rotary positions ------------------------------------------------------------------
@@ -157,10 +173,7 @@ class Rope:
         self.handle = ctypes.c_void_p()
         check(lib().openmini_rope_create(freq, axis, self.pairs, self.n_axes, int(pairing == "adjacent"), scale,
                                          ctypes.byref(self.handle)))
-
-    def _positions(self, d_positions, position_stride, tokens: int):
-        stride = tokens if position_stride is None else position_stride
-        return _need(d_positions, 4 * _rows_bytes(self.n_axes if tokens else 0, stride, tokens, 1), "d_positions"), stride
+        self._apply, self._append = lib().openmini_rope_apply, lib().openmini_rope_append
 
     def apply(self, d_x, x_dtype: DType, d_y, y_dtype: DType, d_positions, tokens: int, heads: int, head_dim: int,
               inverse: bool = False, stream=None, x_stride: int | None = None, y_stride: int | None = None,
@@ -169,11 +182,20 @@ class Rope:
         (d_positions [axes][tokens]); inverse: turned back, the gradient of x from y's."""
         row = heads * head_dim
         xs, ys = row if x_stride is None else x_stride, row if y_stride is None else y_stride
-        pos, ps = self._positions(d_positions, position_stride, tokens)
-        a = _native.RopeArgs(_need(d_x, _rows_bytes(tokens, xs, row, DType(x_dtype).nbytes), "d_x"),
-                             _need(d_y, _rows_bytes(tokens, ys, row, DType(y_dtype).nbytes), "d_y"), xs, ys, x_dtype, y_dtype,
-                             tokens, heads, head_dim, bool(inverse), pos, ps)
-        check(lib().openmini_rope_apply(self.handle, a, stream))
+        ps = tokens if position_stride is None else position_stride
+        n = _rows_bytes(tokens, xs, row, _NBYTES[x_dtype])
+        if d_x.nbytes < n:
+            _short("d_x", d_x, n)
+        n = _rows_bytes(tokens, ys, row, _NBYTES[y_dtype])
+        if d_y.nbytes < n:
+            _short("d_y", d_y, n)
+        n = 4 * ((self.n_axes - 1) * ps + tokens)
+        if d_positions.nbytes < n:
+            _short("d_positions", d_positions, n)
+        rc = self._apply(self.handle, _native.RopeArgs(d_x.ptr, d_y.ptr, xs, ys, x_dtype, y_dtype, tokens, heads, head_dim, inverse,
+                                                       d_positions.ptr, ps), stream)
+        if rc:
+            check(rc)
 
     def append(self, cache: KVCache, d_q, d_k, d_v, in_dtype: DType, d_q_out, q_dtype: DType, d_positions, d_slots, tokens: int,
                q_heads: int, stream=None, q_stride: int | None = None, k_stride: int | None = None,
@@ -183,14 +205,30 @@ class Rope:
         q_row, kv_row = q_heads * cache.head_dim, cache.kv_heads * cache.head_dim
         qs = q_row if q_stride is None else q_stride
         ks, vs = kv_row if k_stride is None else k_stride, kv_row if v_stride is None else v_stride
-        size = DType(in_dtype).nbytes
-        pos, ps = self._positions(d_positions, position_stride, tokens)
-        a = _native.RopeAppendArgs(_need(d_q, _rows_bytes(tokens, qs, q_row, size), "d_q"),
-                                   _need(d_k, _rows_bytes(tokens, ks, kv_row, size), "d_k"),
-                                   _need(d_v, _rows_bytes(tokens, vs, kv_row, size), "d_v"), qs, ks, vs,
-                                   _need(d_q_out, tokens * q_row * DType(q_dtype).nbytes, "d_q_out"), q_row, in_dtype, q_dtype,
-                                   tokens, q_heads, pos, ps, _need(d_slots, 4 * tokens, "d_slots"))
-        check(lib().openmini_rope_append(self.handle, cache.desc, a, stream))
+        ps = tokens if position_stride is None else position_stride
+        size = _NBYTES[in_dtype]
+        n = _rows_bytes(tokens, qs, q_row, size)
+        if d_q.nbytes < n:
+            _short("d_q", d_q, n)
+        n = _rows_bytes(tokens, ks, kv_row, size)
+        if d_k.nbytes < n:
+            _short("d_k", d_k, n)
+        n = _rows_bytes(tokens, vs, kv_row, size)
+        if d_v.nbytes < n:
+            _short("d_v", d_v, n)
+        n = tokens * q_row * _NBYTES[q_dtype]
+        if d_q_out.nbytes < n:
+            _short("d_q_out", d_q_out, n)
+        n = 4 * ((self.n_axes - 1) * ps + tokens)
+        if d_positions.nbytes < n:
+            _short("d_positions", d_positions, n)
+        if d_slots.nbytes < 4 * tokens:
+            _short("d_slots", d_slots, 4 * tokens)
+        rc = self._append(self.handle, cache.desc, _native.RopeAppendArgs(
+            d_q.ptr, d_k.ptr, d_v.ptr, qs, ks, vs, d_q_out.ptr, q_row, in_dtype, q_dtype, tokens, q_heads, d_positions.ptr, ps,
+            d_slots.ptr), stream)
+        if rc:
+            check(rc)
 
     def close(self) -> None:
         if self.handle:
@@ -221,8 +259,7 @@ class PagedAttention:
         if not nbytes:
             raise InvalidInput(f"no attention of {q_heads} query heads on {kv_heads} key heads of {head_dim}")
         self.work = DeviceBuffer(nbytes)
-        self.work.fill(0)
-        check(lib().openmini_qmm_stream_synchronize(None))  # before a call on any stream
+        self._call = lib().openmini_attn_decode
 
     def run(self, cache: KVCache, d_q, d_out, d_tables, max_pages: int, d_lens, rows: int, d_rows=None,
             requests: int | None = None, d_lse=None, stream=None, table_stride: int | None = None,
@@ -230,7 +267,7 @@ class PagedAttention:
         """d_out [rows][q_heads][head_dim]: row j attends to the first d_lens[j] keys of request
         d_rows[j] (None: of request j), whose pages are d_tables[request][:max_pages];
         d_lse [rows][q_heads] fp32, the log of the sum of exponentials."""
-        if (cache.kv_heads, cache.head_dim) != (self.kv_heads, self.head_dim):
+        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
             raise InvalidInput(f"cache of {cache.kv_heads} heads of {cache.head_dim}, expected {self.kv_heads} of {self.head_dim}")
         if requests is None:
             if d_rows is not None:
@@ -239,14 +276,28 @@ class PagedAttention:
         row = self.q_heads * self.head_dim
         qs, os_ = row if q_stride is None else q_stride, row if out_stride is None else out_stride
         ts = max_pages if table_stride is None else table_stride
-        a = _native.AttnArgs(_need(d_q, _rows_bytes(rows, qs, row, 2), "d_q"), qs,
-                             _need(d_out, _rows_bytes(rows, os_, row, self.out_dtype.nbytes), "d_out"), os_,
-                             _need(d_lse, 4 * rows * self.q_heads, "d_lse") if d_lse is not None else None, self.q_dtype,
-                             self.out_dtype, self.q_heads, self.scale, self.window, rows, _need(d_lens, 4 * rows, "d_lens"),
-                             _need(d_rows, 4 * rows, "d_rows") if d_rows is not None else None,
-                             _need(d_tables, 4 * _rows_bytes(requests, ts, max_pages, 1), "d_tables"), ts, max_pages,
-                             max(requests, 1), self.work.ptr, self.work.nbytes)
-        check(lib().openmini_attn_decode(cache.desc, a, stream))
+        n = _rows_bytes(rows, qs, row, 2)
+        if d_q.nbytes < n:
+            _short("d_q", d_q, n)
+        n = _rows_bytes(rows, os_, row, _NBYTES[self.out_dtype])
+        if d_out.nbytes < n:
+            _short("d_out", d_out, n)
+        n = 4 * rows
+        if d_lens.nbytes < n:
+            _short("d_lens", d_lens, n)
+        if d_rows is not None and d_rows.nbytes < n:
+            _short("d_rows", d_rows, n)
+        if d_lse is not None and d_lse.nbytes < n * self.q_heads:
+            _short("d_lse", d_lse, n * self.q_heads)
+        n = 4 * _rows_bytes(requests, ts, max_pages, 1)
+        if d_tables.nbytes < n:
+            _short("d_tables", d_tables, n)
+        rc = self._call(cache.desc, _native.AttnArgs(
+            d_q.ptr, qs, d_out.ptr, os_, d_lse.ptr if d_lse is not None else None, self.q_dtype, self.out_dtype, self.q_heads,
+            self.scale, self.window, rows, d_lens.ptr, d_rows.ptr if d_rows is not None else None, d_tables.ptr, ts, max_pages,
+            max(requests, 1), self.work.ptr, self.work.nbytes), stream)
+        if rc:
+            check(rc)
 
 
 __all__ = ["DType", "KVCache", "PagedAttention", "Rope", "StepPlan", "rope_axes", "rope_frequencies"]
