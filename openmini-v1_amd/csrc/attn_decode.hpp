@@ -133,13 +133,25 @@ struct Span {
     __device__ __forceinline__ uint32_t weight() const { return max(tiles, 1u); }
 };
 
-// None for a request outside the tables.
+// What the call says of a row, and the same by scalar loads (a uniform row; they are not
+// counted with a wave's loads of keys and values, and wait for none of them).
+struct Said {
+    int32_t keys, request;
+};
+__device__ __forceinline__ Said said_of(const DecodeArgs& a, uint32_t r) {
+    return {a.lens[r], a.rows ? a.rows[r] : (int32_t)r};
+}
+typedef const __attribute__((address_space(4))) int32_t ConstInt;
+__device__ __forceinline__ Said said_of_uniform(const DecodeArgs& a, uint32_t r) {
+    return {((ConstInt*)a.lens)[r], a.rows ? ((ConstInt*)a.rows)[r] : (int32_t)r};
+}
+
+// No keys for a request outside the tables.
 template <uint32_t kKeys>
-__device__ __forceinline__ Span span_of(const DecodeArgs& a, uint32_t r) {
+__device__ __forceinline__ Span span_of(const DecodeArgs& a, Said said) {
     Span s;
-    s.hi = min(max(a.lens[r], 0), (int32_t)a.max_len);
-    const uint32_t request = a.rows ? (uint32_t)a.rows[r] : r;
-    if (request >= a.requests) s.hi = 0;
+    s.hi = min(max(said.keys, 0), (int32_t)a.max_len);
+    if ((uint32_t)said.request >= a.requests) s.hi = 0;
     s.lo = a.window && (int64_t)s.hi > a.window ? s.hi - (int32_t)a.window : 0;
     s.tiles = ((uint32_t)s.hi + kKeys - 1) / kKeys - (uint32_t)s.lo / kKeys;
     return s;
@@ -152,11 +164,10 @@ __device__ __forceinline__ Span span_of(const DecodeArgs& a, uint32_t r) {
 struct Share {
     uint32_t each, from, to;  // tiles of a share; this one's place in the line
     uint32_t row, row_at;     // its first row, and that row's place
-    Span span;                // of that row
 };
 
 template <uint32_t kKeys, int W>
-__device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Share& out) {
+__device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Share& out, Said& said) {
     const uint32_t lane = threadIdx.x & 63;
     auto place = [&](uint32_t total) {
         out.each = (total + a.shares - 1) / a.shares;
@@ -165,10 +176,12 @@ __device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Shar
         return out.from < total;
     };
     if (a.n_rows <= 64) {  // every wave by itself
+        Said mine = {0, 0};
         Span s = {0, 0, 0};
         uint32_t n = 0;
         if (lane < a.n_rows) {
-            s = span_of<kKeys>(a, lane);
+            mine = said_of(a, lane);
+            s = span_of<kKeys>(a, mine);
             n = s.weight();
         }
         const uint32_t upto = wave_sums(n);
@@ -176,9 +189,8 @@ __device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Shar
         const int at = __ffsll((unsigned long long)__ballot(out.from >= upto - n && out.from < upto)) - 1;
         out.row = (uint32_t)at;
         out.row_at = (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), at);
-        out.span.lo = __builtin_amdgcn_readlane(s.lo, at);
-        out.span.hi = __builtin_amdgcn_readlane(s.hi, at);
-        out.span.tiles = (uint32_t)__builtin_amdgcn_readlane((int)s.tiles, at);
+        said.keys = __builtin_amdgcn_readlane(s.hi, at);
+        said.request = __builtin_amdgcn_readlane(mine.request, at);
         return true;
     }
     // each thread sums some rows; the one whose rows pass a wave's start looks through them
@@ -187,7 +199,7 @@ __device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Shar
     const uint32_t each = (a.n_rows + 64 * W - 1) / (64 * W);
     const uint32_t r0 = min(threadIdx.x * each, a.n_rows), r1 = min(r0 + each, a.n_rows);
     uint32_t n = 0;
-    for (uint32_t r = r0; r < r1; ++r) n += span_of<kKeys>(a, r).weight();
+    for (uint32_t r = r0; r < r1; ++r) n += span_of<kKeys>(a, said_of(a, r)).weight();
     uint32_t upto = wave_sums(n);
     if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
@@ -204,7 +216,7 @@ __device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Shar
         if (from >= upto - n && from < upto) {
             uint32_t at = upto - n, r = r0;
             for (; r + 1 < r1; ++r) {
-                const uint32_t weight = span_of<kKeys>(a, r).weight();
+                const uint32_t weight = span_of<kKeys>(a, said_of(a, r)).weight();
                 if (from < at + weight) break;
                 at += weight;
             }
@@ -216,7 +228,7 @@ __device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Shar
     if (!any) return false;
     out.row = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[wave][0]);
     out.row_at = (uint32_t)__builtin_amdgcn_readfirstlane((int)found[wave][1]);
-    out.span = span_of<kKeys>(a, out.row);
+    said = said_of_uniform(a, out.row);
     return true;
 }
 
@@ -245,50 +257,62 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     const uint32_t share_no = a.by_units.div(w_no), unit = w_no - share_no * units;
     const uint32_t kv = a.by_head_tiles.div(unit), head_tile = unit - kv * (uint32_t)a.head_tiles;
     Share share;
-    if (!find_share<kKeys, W>(a, share_no, share)) {
+    Said said;
+    if (!find_share<kKeys, W>(a, share_no, share, said)) {
         if (!a.by_row && unit == 0 && share_no < a.shares && lane == 0) a.split[share_no] = Split{0, 0, 0};
         return;
     }
     const int heads = min(kHeadTile, a.group - (int)head_tile * kHeadTile);  // columns in use
     const int head0 = (int)kv * a.group + (int)head_tile * kHeadTile;
 
-    for (;;) {
-    // the share's part of a row: tiles [tile0, tile1) of keys [part.lo, part.hi)
-    const Span part = share.span;
-    const uint32_t row = share.row, row_end = share.row_at + part.weight(), here_end = min(row_end, share.to);
-    const uint32_t tile0 = (uint32_t)part.lo / kKeys + (share.from - share.row_at);
-    const uint32_t tile1 = part.tiles ? (uint32_t)part.lo / kKeys + (here_end - share.row_at) : tile0;
+    // A row's stretch of the share: tiles [tile0, tile1) of its keys [lo, hi).
+    struct Row {
+        uint32_t row, at, end;  // its places in the line: [at, end)
+        uint32_t tile0, tile1;
+        int32_t lo, hi;
+        const int32_t* table;
+    };
+    auto row_of = [&](uint32_t row, uint32_t at, uint32_t from, Said said) {
+        const Span s = span_of<kKeys>(a, said);
+        Row r;
+        r.row = row;
+        r.at = at;
+        r.end = at + s.weight();
+        r.tile0 = (uint32_t)s.lo / kKeys + (from - at);
+        r.tile1 = s.tiles ? (uint32_t)s.lo / kKeys + (min(r.end, share.to) - at) : r.tile0;
+        r.lo = s.lo;
+        r.hi = s.hi;
+        r.table = a.tables + (int64_t)said.request * a.table_stride;
+        return r;
+    };
 
-    // q^T: lane holds column `col`, eight dimensions a step, in the order of a key's loads
+    // q^T: lane holds column `col`, eight dimensions a step, in the order of a key's loads;
+    // columns past the heads in use hold the last of them again
     u32x4 qf[kSteps];
-    {
+    auto load_q = [&](uint32_t row) {
         const uint8_t* q = a.q + row * a.q_stride + (int64_t)(head0 + min(col, heads - 1)) * D * 2;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
             const int dim = F8 && (st | 1) < kSteps ? (st >> 1) * 64 + g * 16 + (st & 1) * 8 : st * 32 + g * 8;
             qf[st] = *reinterpret_cast<const u32x4*>(q + dim * 2);
-            if (col >= heads) qf[st] = u32x4{0, 0, 0, 0};
         }
-    }
+    };
 
-    f32x4 acc[kTiles];
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0;
-
-    const uint32_t request = a.rows ? (uint32_t)a.rows[row] : row;
-    const int32_t* table = a.tables + (int64_t)request * a.table_stride;
-    const int32_t first_group = part.lo & ~7, last_group = (part.hi - 1) & ~7;
     const uint8_t* k_lane = a.cache.k + kv * a.cache.head_stride + g * 16;
     const uint8_t* v_base = a.cache.v + kv * a.cache.head_stride;
     const int kg = col >> 2, k_row = col & 3;  // the lane's key of tile s: 8 kg + 4 s + k_row
 
-    // the eight keys from 8 * grp of a tile's 32 `sub` on, kept inside the row's keys; the
-    // column of their page, and their place in the cache
-    auto group_at = [&](uint32_t tile, int sub, int grp) -> int32_t {
-        return min(max((int32_t)(tile * kKeys) + 32 * sub + 8 * grp, first_group), last_group);
+    // A tile of some row; the eight keys from 8 * grp of its 32 `sub` on, kept inside the
+    // row's keys; the column of their page, and their place in the cache.
+    struct Tile {
+        uint32_t no;
+        int32_t first_group, last_group;
+        const int32_t* table;
     };
-    auto page_at = [&](int32_t key) -> int32_t { return table[a.cache.page.div_by_many((uint32_t)key)]; };
+    auto tile_of = [](const Row& r, uint32_t no) { return Tile{no, r.lo & ~7, (r.hi - 1) & ~7, r.table}; };
+    auto group_at = [&](const Tile& t, int sub, int grp) -> int32_t {
+        return min(max((int32_t)(t.no * kKeys) + 32 * sub + 8 * grp, t.first_group), t.last_group);
+    };
     auto offset_of = [&](int32_t page, int32_t key) -> int64_t {
         const uint32_t in_page = (uint32_t)key - a.cache.page.div_by_many((uint32_t)key) * a.cache.page.d;
         return ((uint32_t)page < a.cache.n_pages ? (int64_t)page * a.cache.page_stride : 0) +
@@ -297,21 +321,21 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     struct Pages {
         int32_t k[kSub], v[kSub];
     };
-    auto pages_of = [&](uint32_t tile) {
+    auto pages_of = [&](const Tile& t) {
         Pages p;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            p.k[u] = page_at(group_at(tile, u, kg));
-            p.v[u] = page_at(group_at(tile, u, g));
+            p.k[u] = t.table[a.cache.page.div_by_many((uint32_t)group_at(t, u, kg))];
+            p.v[u] = t.table[a.cache.page.div_by_many((uint32_t)group_at(t, u, g))];
         }
         return p;
     };
 
     uint32_t kraw[kSub][2][kKWords], vraw[kSub][8][kVWords];
-    auto load_k = [&](uint32_t tile, const Pages& pages) {
+    auto load_k = [&](const Tile& t, const Pages& pages) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            const uint8_t* p = k_lane + offset_of(pages.k[u], group_at(tile, u, kg)) + k_row * a.cache.token_stride;
+            const uint8_t* p = k_lane + offset_of(pages.k[u], group_at(t, u, kg)) + k_row * a.cache.token_stride;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const uint8_t* ps = p + 4 * s * a.cache.token_stride;
@@ -326,10 +350,10 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
             }
         }
     };
-    auto load_v = [&](uint32_t tile, const Pages& pages) {
+    auto load_v = [&](const Tile& t, const Pages& pages) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            const uint8_t* p = v_base + offset_of(pages.v[u], group_at(tile, u, g));
+            const uint8_t* p = v_base + offset_of(pages.v[u], group_at(t, u, g));
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint8_t* pj = p + j * a.cache.token_stride;
@@ -343,219 +367,254 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         }
     };
 
-    uint32_t tile = tile0;
-    if (tile < tile1) {
-        Pages now = pages_of(tile);
-        // the tile after the last is the last again: loads without a branch around them,
-        // so that the wait for the present values need not cover them
-        uint32_t next = tile + 1 < tile1 ? tile + 1 : tile;
-        Pages then = pages_of(next);
-        load_k(tile, now);
-        load_v(tile, now);
-        for (;;) {
-            // first product
-            f32x4 sc[kSub][2];
+    Pages now, then;  // of the present tile and the next
+    f32x4 acc[kTiles], sc[kSub][2];
+    float m, l;
+    auto scores = [&] {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                sc[u][s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int st = 0; st < kSteps; ++st) {
+                    u32x4 kf;
+                    if constexpr (F8) {
+                        const uint32_t w0 = kraw[u][s][2 * st], w1 = kraw[u][s][2 * st + 1];
+                        kf = u32x4{T::template from_f8<false>(w0), T::template from_f8<true>(w0),
+                                   T::template from_f8<false>(w1), T::template from_f8<true>(w1)};
+                    } else {
+                        kf = u32x4{kraw[u][s][4 * st], kraw[u][s][4 * st + 1], kraw[u][s][4 * st + 2],
+                                   kraw[u][s][4 * st + 3]};
+                    }
+                    sc[u][s] = T::mfma(kf, qf[st], sc[u][s]);
+                }
+            }
+    };
+    auto outputs = [&](const Row& cur, uint32_t tile) {
+        // keys outside the row's or on no page of the cache: only a row's first and
+        // last tiles, and broken tables, have them
+        float x[kSub][8];
+        const int32_t key0 = (int32_t)(tile * kKeys) + 8 * g;
+        bool whole = key0 >= cur.lo && key0 + (int32_t)kKeys - 24 <= cur.hi;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[u][j] = sc[u][j / 4][j % 4] * a.scale;
+            whole = whole && (uint32_t)now.v[u] < a.cache.n_pages;
+        }
+        if (!__all(whole)) {
 #pragma unroll
             for (int u = 0; u < kSub; ++u)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    sc[u][s] = f32x4{0, 0, 0, 0};
+                for (int j = 0; j < 8; ++j) {
+                    const int32_t key = key0 + 32 * u + j;
+                    const bool seen = (uint32_t)now.v[u] < a.cache.n_pages && key >= cur.lo && key < cur.hi;
+                    x[u][j] = seen ? x[u][j] : -INFINITY;
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st) {
-                        u32x4 kf;
-                        if constexpr (F8) {
-                            const uint32_t w0 = kraw[u][s][2 * st], w1 = kraw[u][s][2 * st + 1];
-                            kf = u32x4{T::template from_f8<false>(w0), T::template from_f8<true>(w0),
-                                       T::template from_f8<false>(w1), T::template from_f8<true>(w1)};
-                        } else {
-                            kf = u32x4{kraw[u][s][4 * st], kraw[u][s][4 * st + 1], kraw[u][s][4 * st + 2],
-                                       kraw[u][s][4 * st + 3]};
+                    for (int w = 0; w < kVWords; ++w) vraw[u][j][w] = seen ? vraw[u][j][w] : 0;  // 0 * NaN is NaN
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, x[u][j]);
+        top = column_max(top);
+        if (__any(top > m)) {
+            const float to = fmaxf(m, top);
+            const float by = exp2_of(m - above(to));
+            m = to;
+            l *= by;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) acc[i] *= by;
+        }
+        const float base = above(m);
+        // second product, p as the sum of kParts 16-bit parts
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            constexpr int kParts = T::kExactParts;
+            u32x4 pf[kParts];
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
+                l += r0 + r1;
+#pragma unroll
+                for (int k = 0; k < kParts; ++k) {
+                    const uint32_t h = T::pair(r0, r1);
+                    pf[k][j / 2] = h;
+                    r0 -= T::low(h);
+                    r1 -= T::high(h);
+                }
+            }
+            auto add = [&](int t, u32x4 vf) {
+#pragma unroll
+                for (int k = 0; k < kParts; ++k) acc[t] = T::mfma(vf, pf[k], acc[t]);
+            };
+            auto chunk = [&](int t0, int word0, auto width_tag) {
+                constexpr int kWidth = decltype(width_tag)::value;
+                if constexpr (F8) {
+#pragma unroll
+                    for (int w = 0; w < (kWidth + 3) / 4; ++w) {
+                        u32x4 f[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t v0 = vraw[u][2 * q][word0 + w], v1 = vraw[u][2 * q + 1][word0 + w];
+                            const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
+                            f[0][q] = T::template from_f8<false>(lo);
+                            f[1][q] = T::template from_f8<true>(lo);
+                            if constexpr (kWidth >= 4) {
+                                const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
+                                f[2][q] = T::template from_f8<false>(hi);
+                                f[3][q] = T::template from_f8<true>(hi);
+                            }
                         }
-                        sc[u][s] = T::mfma(kf, qf[st], sc[u][s]);
+#pragma unroll
+                        for (int e = 0; e < (kWidth < 4 ? kWidth : 4); ++e) add(t0 + 4 * w + e, f[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kWidth; ++e) {
+                        u32x4 f;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            f[q] = __builtin_amdgcn_perm(vraw[u][2 * q + 1][word0 + e / 2], vraw[u][2 * q][word0 + e / 2],
+                                                         e & 1 ? 0x07060302u : 0x05040100u);
+                        add(t0 + e, f);
                     }
                 }
+            };
+#pragma unroll
+            for (int c = 0; c < kFull; ++c) chunk(8 * c, c * 2 * kEl, std::integral_constant<int, 8>{});
+            if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
+            if constexpr (kHas32)
+                chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
+        }
+    };
+
+    // The share's tiles, row after row.  The loads run a tile ahead and the pages two, from
+    // a row into the next: a row's last products are behind the next row's first loads.
+    Row cur = row_of(share.row, share.row_at, share.from, said);
+    bool loaded = false;  // cur's first tile is on its way
+    for (;;) {
+        const bool more = cur.end < share.to;
+        if (more) said = said_of_uniform(a, cur.row + 1);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0, 0, 0, 0};
+        m = -INFINITY;
+        l = 0;
+        uint32_t tile = cur.tile0;
+        if (!loaded && tile < cur.tile1) {
+            const Tile first = tile_of(cur, tile), second = tile_of(cur, min(tile + 1, cur.tile1 - 1));
+            now = pages_of(first);
+            load_q(cur.row);
+            then = pages_of(second);
+            load_k(first, now);
+            load_v(first, now);
+        }
+        for (; tile + 2 < cur.tile1; ++tile) {
+            scores();
             // the pages of the tile after the next, then the next keys: their pages came
             // with loads that have been waited for
-            const uint32_t after = next + 1 < tile1 ? next + 1 : next;
-            const Pages later = pages_of(after);
-            load_k(next, then);
-
-            // keys outside the row's or on no page of the cache: only a row's first and
-            // last tiles, and broken tables, have them
-            float x[kSub][8];
-            const int32_t key0 = (int32_t)(tile * kKeys) + 8 * g;
-            bool whole = key0 >= part.lo && key0 + (int32_t)kKeys - 24 <= part.hi;
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[u][j] = sc[u][j / 4][j % 4] * a.scale;
-                whole = whole && (uint32_t)now.v[u] < a.cache.n_pages;
-            }
-            if (!__all(whole)) {
-#pragma unroll
-                for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int32_t key = key0 + 32 * u + j;
-                        const bool seen = (uint32_t)now.v[u] < a.cache.n_pages && key >= part.lo && key < part.hi;
-                        x[u][j] = seen ? x[u][j] : -INFINITY;
-#pragma unroll
-                        for (int w = 0; w < kVWords; ++w) vraw[u][j][w] = seen ? vraw[u][j][w] : 0;  // 0 * NaN is NaN
-                    }
-            }
-            float top = x[0][0];
-#pragma unroll
-            for (int u = 0; u < kSub; ++u)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, x[u][j]);
-            top = column_max(top);
-            if (__any(top > m)) {
-                const float to = fmaxf(m, top);
-                const float by = exp2_of(m - above(to));
-                m = to;
-                l *= by;
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) acc[i] *= by;
-            }
-            const float base = above(m);
-            // second product, p as the sum of kParts 16-bit parts
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                constexpr int kParts = T::kExactParts;
-                u32x4 pf[kParts];
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
-                    l += r0 + r1;
-#pragma unroll
-                    for (int k = 0; k < kParts; ++k) {
-                        const uint32_t h = T::pair(r0, r1);
-                        pf[k][j / 2] = h;
-                        r0 -= T::low(h);
-                        r1 -= T::high(h);
-                    }
-                }
-                auto add = [&](int t, u32x4 vf) {
-#pragma unroll
-                    for (int k = 0; k < kParts; ++k) acc[t] = T::mfma(vf, pf[k], acc[t]);
-                };
-                auto chunk = [&](int t0, int word0, auto width_tag) {
-                    constexpr int kWidth = decltype(width_tag)::value;
-                    if constexpr (F8) {
-#pragma unroll
-                        for (int w = 0; w < (kWidth + 3) / 4; ++w) {
-                            u32x4 f[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const uint32_t v0 = vraw[u][2 * q][word0 + w], v1 = vraw[u][2 * q + 1][word0 + w];
-                                const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
-                                f[0][q] = T::template from_f8<false>(lo);
-                                f[1][q] = T::template from_f8<true>(lo);
-                                if constexpr (kWidth >= 4) {
-                                    const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
-                                    f[2][q] = T::template from_f8<false>(hi);
-                                    f[3][q] = T::template from_f8<true>(hi);
-                                }
-                            }
-#pragma unroll
-                            for (int e = 0; e < (kWidth < 4 ? kWidth : 4); ++e) add(t0 + 4 * w + e, f[e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < kWidth; ++e) {
-                            u32x4 f;
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                f[q] = __builtin_amdgcn_perm(vraw[u][2 * q + 1][word0 + e / 2], vraw[u][2 * q][word0 + e / 2],
-                                                             e & 1 ? 0x07060302u : 0x05040100u);
-                            add(t0 + e, f);
-                        }
-                    }
-                };
-#pragma unroll
-                for (int c = 0; c < kFull; ++c) chunk(8 * c, c * 2 * kEl, std::integral_constant<int, 8>{});
-                if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
-                if constexpr (kHas32)
-                    chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
-            }
-            if (next == tile) break;
-            load_v(next, then);
-            tile = next;
-            next = after;
+            const Pages later = pages_of(tile_of(cur, tile + 2));
+            load_k(tile_of(cur, tile + 1), then);
+            outputs(cur, tile);
+            load_v(tile_of(cur, tile + 1), then);
             now = then;
             then = later;
         }
-    }
-
-    l = column_sum(l);
-    // accumulator i of tile t is dimension chunk + (4 g + i) * width + (t in the chunk): a
-    // lane stores the chunk's width neighbours at a time
-    auto each_run = [&](auto&& f) {
-#pragma unroll
-        for (int c = 0; c < kTiles;) {
-            const int width = c / 8 < kFull ? 8 : kHas64 && c < 8 * kFull + 4 ? 4 : 2;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f(c, i, width, c * 16 + (4 * g + i) * width);
-            c += width;
+        // The row's last two tiles, before which come the next row's first.  At the share's
+        // end (or before a row without keys) the next tile is the present one again: loads
+        // without a branch around them, so that the wait for the present values need not
+        // cover them.
+        Row following = cur;
+        if (more) following = row_of(cur.row + 1, cur.end, cur.end, said);
+        loaded = tile < cur.tile1 && more && following.tile0 < following.tile1;
+        for (; tile < cur.tile1; ++tile) {
+            const bool last = tile + 1 == cur.tile1, cross = last && loaded;
+            scores();
+            const Tile next = cross ? tile_of(following, following.tile0) : tile_of(cur, last ? tile : tile + 1);
+            const Tile after = loaded ? tile_of(following, min(following.tile0 + (last ? 1u : 0u), following.tile1 - 1)) : next;
+            const Pages later = pages_of(after);
+            if (cross && cur.tile1 - cur.tile0 == 1) then = pages_of(next);  // no tile before looked them up
+            load_k(next, then);
+            if (cross) load_q(following.row);
+            outputs(cur, tile);
+            if (last && !cross) break;
+            load_v(next, then);
+            now = then;
+            then = later;
         }
-    };
-    // the row's shares: all but the first begin inside it
-    const uint32_t first_share = share.row_at / share.each, parts = (row_end - 1) / share.each - first_share + 1;
-    if (a.by_row && unit == 0 && lane == 0 && share_no == first_share) a.split[row] = Split{row, first_share, parts};
-    if (col < heads) {
-        if (parts == 1) {
-            const float over = l > 0 || l != l ? a.cache.v_scale / l : 0.0f;
-            const int64_t at = (int64_t)(head0 + col) * D;
-            if (a.out_f32) {
-                float* o = reinterpret_cast<float*>(a.out + row * a.out_stride) + at;
+
+        l = column_sum(l);
+        // accumulator i of tile t is dimension chunk + (4 g + i) * width + (t in the chunk): a
+        // lane stores the chunk's width neighbours at a time
+        auto each_run = [&](auto&& f) {
+#pragma unroll
+            for (int c = 0; c < kTiles;) {
+                const int width = c / 8 < kFull ? 8 : kHas64 && c < 8 * kFull + 4 ? 4 : 2;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f(c, i, width, c * 16 + (4 * g + i) * width);
+                c += width;
+            }
+        };
+        // the row's shares: all but the first begin inside it
+        const uint32_t row = cur.row, first_share = cur.at / share.each, parts = (cur.end - 1) / share.each - first_share + 1;
+        if (a.by_row && unit == 0 && lane == 0 && share_no == first_share) a.split[row] = Split{row, first_share, parts};
+        if (col < heads) {
+            if (parts == 1) {
+                const float over = l > 0 || l != l ? a.cache.v_scale / l : 0.0f;
+                const int64_t at = (int64_t)(head0 + col) * D;
+                if (a.out_f32) {
+                    float* o = reinterpret_cast<float*>(a.out + row * a.out_stride) + at;
+                    each_run([&](int t, int i, int width, int d) {
+                        if (width >= 4) {
+#pragma unroll
+                            for (int e = 0; e < width; e += 4)
+                                *reinterpret_cast<f32x4*>(o + d + e) =
+                                    f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]} * over;
+                        } else {
+                            *reinterpret_cast<float2*>(o + d) = make_float2(acc[t][i] * over, acc[t + 1][i] * over);
+                        }
+                    });
+                } else {
+                    uint16_t* o = reinterpret_cast<uint16_t*>(a.out + row * a.out_stride) + at;
+                    each_run([&](int t, int i, int width, int d) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < width; e += 2) w[e / 2] = T::pair(acc[t + e][i] * over, acc[t + e + 1][i] * over);
+                        if (width == 8)
+                            *reinterpret_cast<uint4*>(o + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                        else if (width == 4)
+                            *reinterpret_cast<uint2*>(o + d) = make_uint2(w[0], w[1]);
+                        else
+                            *reinterpret_cast<uint32_t*>(o + d) = w[0];
+                    });
+                }
+                if (a.lse && g == 0) a.lse[(int64_t)row * a.q_heads + head0 + col] = log_sum(m, l);
+            } else {
+                // an entry of the share: 1 for a row that starts in it, 0 for one that goes on
+                const int64_t entry = ((int64_t)(2 * share_no + (share_no == first_share)) * a.q_heads + head0 + col);
+                float* o = a.part_acc + entry * D;
                 each_run([&](int t, int i, int width, int d) {
                     if (width >= 4) {
 #pragma unroll
                         for (int e = 0; e < width; e += 4)
                             *reinterpret_cast<f32x4*>(o + d + e) =
-                                f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]} * over;
+                                f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]};
                     } else {
-                        *reinterpret_cast<float2*>(o + d) = make_float2(acc[t][i] * over, acc[t + 1][i] * over);
+                        *reinterpret_cast<float2*>(o + d) = make_float2(acc[t][i], acc[t + 1][i]);
                     }
                 });
-            } else {
-                uint16_t* o = reinterpret_cast<uint16_t*>(a.out + row * a.out_stride) + at;
-                each_run([&](int t, int i, int width, int d) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < width; e += 2) w[e / 2] = T::pair(acc[t + e][i] * over, acc[t + e + 1][i] * over);
-                    if (width == 8)
-                        *reinterpret_cast<uint4*>(o + d) = make_uint4(w[0], w[1], w[2], w[3]);
-                    else if (width == 4)
-                        *reinterpret_cast<uint2*>(o + d) = make_uint2(w[0], w[1]);
-                    else
-                        *reinterpret_cast<uint32_t*>(o + d) = w[0];
-                });
+                if (g == 0) a.part_ml[entry] = make_float2(m, l);
             }
-            if (a.lse && g == 0) a.lse[(int64_t)row * a.q_heads + head0 + col] = log_sum(m, l);
-        } else {
-            // an entry of the share: 1 for a row that starts in it, 0 for one that goes on
-            const int64_t entry = ((int64_t)(2 * share_no + (share_no == first_share)) * a.q_heads + head0 + col);
-            float* o = a.part_acc + entry * D;
-            each_run([&](int t, int i, int width, int d) {
-                if (width >= 4) {
-#pragma unroll
-                    for (int e = 0; e < width; e += 4)
-                        *reinterpret_cast<f32x4*>(o + d + e) =
-                            f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]};
-                } else {
-                    *reinterpret_cast<float2*>(o + d) = make_float2(acc[t][i], acc[t + 1][i]);
-                }
-            });
-            if (g == 0) a.part_ml[entry] = make_float2(m, l);
         }
-    }
-    if (!a.by_row && unit == 0 && lane == 0 && here_end == share.to)
-        a.split[share_no] = here_end < row_end && share_no == first_share ? Split{row, first_share, parts} : Split{0, 0, 0};
-    if (here_end == share.to) return;
-    share.from = share.row_at = row_end;
-    share.row = row + 1;
-    share.span = span_of<kKeys>(a, row + 1);
+        if (!more) {
+            if (!a.by_row && unit == 0 && lane == 0)
+                a.split[share_no] = cur.end > share.to && share_no == first_share ? Split{row, first_share, parts} : Split{0, 0, 0};
+            return;
+        }
+        cur = following;
     }
 }
 
