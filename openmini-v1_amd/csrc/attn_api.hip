@@ -409,7 +409,7 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     a.q_stride = p->q_stride * 2;
     a.out_stride = p->out_stride * out_size;
     a.table_stride = p->table_stride;
-    a.window = p->window;
+    a.window = p->window && p->window < max_len ? (uint32_t)p->window : (uint32_t)max_len;
     a.n_rows = (uint32_t)p->rows;
     a.requests = (uint32_t)p->requests;
     a.max_len = (uint32_t)max_len;

@@ -133,26 +133,33 @@ struct Span {
     __device__ __forceinline__ uint32_t weight() const { return max(tiles, 1u); }
 };
 
+// What a wave needs first.  These are kernel arguments of their own, in front: the first 14
+// dwords of them are in SGPRs when a wave starts, while the others are still to be loaded.
+struct First {
+    const int32_t *lens, *rows;
+    uint32_t n_rows, requests, max_len, window, shares;
+};
+
 // What the call says of a row, and the same by scalar loads (a uniform row; they are not
 // counted with a wave's loads of keys and values, and wait for none of them).
 struct Said {
     int32_t keys, request;
 };
-__device__ __forceinline__ Said said_of(const DecodeArgs& a, uint32_t r) {
+__device__ __forceinline__ Said said_of(const First& a, uint32_t r) {
     return {a.lens[r], a.rows ? a.rows[r] : (int32_t)r};
 }
 typedef const __attribute__((address_space(4))) int32_t ConstInt;
-__device__ __forceinline__ Said said_of_uniform(const DecodeArgs& a, uint32_t r) {
+__device__ __forceinline__ Said said_of_uniform(const First& a, uint32_t r) {
     return {((ConstInt*)a.lens)[r], a.rows ? ((ConstInt*)a.rows)[r] : (int32_t)r};
 }
 
 // No keys for a request outside the tables.
 template <uint32_t kKeys>
-__device__ __forceinline__ Span span_of(const DecodeArgs& a, Said said) {
+__device__ __forceinline__ Span span_of(const First& a, Said said) {
     Span s;
     s.hi = min(max(said.keys, 0), (int32_t)a.max_len);
     if ((uint32_t)said.request >= a.requests) s.hi = 0;
-    s.lo = a.window && (int64_t)s.hi > a.window ? s.hi - (int32_t)a.window : 0;
+    s.lo = (int32_t)max((uint32_t)s.hi, a.window) - (int32_t)a.window;  // window: at least 1
     s.tiles = ((uint32_t)s.hi + kKeys - 1) / kKeys - (uint32_t)s.lo / kKeys;
     return s;
 }
@@ -167,7 +174,7 @@ struct Share {
 };
 
 template <uint32_t kKeys, int W>
-__device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Share& out, Said& said) {
+__device__ __forceinline__ bool find_share(const First& a, uint32_t p, Share& out, Said& said) {
     const uint32_t lane = threadIdx.x & 63;
     auto place = [&](uint32_t total) {
         out.each = (total + a.shares - 1) / a.shares;
@@ -233,7 +240,13 @@ __device__ __forceinline__ bool find_share(const DecodeArgs& a, uint32_t p, Shar
 }
 
 template <int D, class T, bool F8, int kSub, int W>
-__global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(const int32_t* lens, const int32_t* rows,
+                                                                                 uint32_t n_rows, uint32_t requests,
+                                                                                 uint32_t max_len, uint32_t window,
+                                                                                 uint32_t shares, uint32_t units,
+                                                                                 uint32_t units_m, uint32_t units_shift,
+                                                                                 DecodeArgs a) {
+    const First f = {lens, rows, n_rows, requests, max_len, window, shares};
     constexpr int kEl = F8 ? 1 : 2;           // bytes of a cache element
     constexpr uint32_t kKeys = 32 * kSub;     // keys of a tile, in kSub tiles of 32
     constexpr int kSteps = D / 32;            // MFMAs over head_dim of the first product
@@ -253,13 +266,13 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     // [tokens][heads][dims] they read whole stretches of memory together (537 MB of keys and
     // values in bf16, heads of 128, loads alone: 88 us; a workgroup to a head: 95 us).
     const uint32_t line = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    const uint32_t units = (uint32_t)(a.kv_heads * a.head_tiles), w_no = line * W + (uint32_t)wave;
-    const uint32_t share_no = a.by_units.div(w_no), unit = w_no - share_no * units;
+    const uint32_t w_no = line * W + (uint32_t)wave;
+    const uint32_t share_no = units_m ? __umulhi(w_no, units_m) >> units_shift : w_no, unit = w_no - share_no * units;
     const uint32_t kv = a.by_head_tiles.div(unit), head_tile = unit - kv * (uint32_t)a.head_tiles;
     Share share;
     Said said;
-    if (!find_share<kKeys, W>(a, share_no, share, said)) {
-        if (!a.by_row && unit == 0 && share_no < a.shares && lane == 0) a.split[share_no] = Split{0, 0, 0};
+    if (!find_share<kKeys, W>(f, share_no, share, said)) {
+        if (!a.by_row && unit == 0 && share_no < shares && lane == 0) a.split[share_no] = Split{0, 0, 0};
         return;
     }
     const int heads = min(kHeadTile, a.group - (int)head_tile * kHeadTile);  // columns in use
@@ -273,7 +286,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         const int32_t* table;
     };
     auto row_of = [&](uint32_t row, uint32_t at, uint32_t from, Said said) {
-        const Span s = span_of<kKeys>(a, said);
+        const Span s = span_of<kKeys>(f, said);
         Row r;
         r.row = row;
         r.at = at;
@@ -498,7 +511,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     bool loaded = false;  // cur's first tile is on its way
     for (;;) {
         const bool more = cur.end < share.to;
-        if (more) said = said_of_uniform(a, cur.row + 1);
+        if (more) said = said_of_uniform(f, cur.row + 1);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0, 0, 0, 0};
         m = -INFINITY;
@@ -622,7 +635,8 @@ template <int D, class T, bool F8>
 hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
     constexpr int W = kDecodeWaves, kSub = decode_subtiles(D, F8);
     const uint64_t waves = (uint64_t)a.launch_shares * a.kv_heads * a.head_tiles, wgs = ((waves + W - 1) / W + 7) / 8 * 8;
-    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows, a.n_rows,
+                       a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift, a);
     return hipGetLastError();
 }
 

@@ -110,8 +110,8 @@ struct DecodeArgs {
     const int32_t *lens, *rows, *tables;
     int64_t q_stride, out_stride;  // bytes
     int64_t table_stride;
-    int64_t window;
     uint32_t n_rows, requests, max_len;  // max_len = max_pages * page_size
+    uint32_t window;                     // keys that a row sees at most
     int32_t q_heads, kv_heads, group, head_tiles;
     int32_t out_f32;
     float scale;  // of a raw product, in powers of two: scale * k_scale * log2(e)
