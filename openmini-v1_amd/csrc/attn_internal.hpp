@@ -36,7 +36,7 @@ struct Cache {
 };
 
 // ---- attn_plan.hip -------------------------------------------------------------------
-constexpr int kMaxPlanRequests = 4096;  // two words a request in a workgroup's LDS
+constexpr int kMaxPlanRequests = 4096;  // three words a request in a workgroup's LDS
 
 struct PlanArgs {
     const int32_t *cached, *fresh, *free, *head;

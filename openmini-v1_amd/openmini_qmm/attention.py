@@ -116,7 +116,7 @@ class StepPlan:
         if requests > self.max_requests:
             raise InvalidInput(f"{requests} requests, planned for {self.max_requests}")
         stride = self.max_pages if table_stride is None else table_stride
-        n, table_bytes = 4 * requests, 4 * _rows_bytes(requests, stride, self.max_pages, 1)
+        n, table_bytes = 4 * requests, 4 * ((requests - 1) * stride + self.max_pages)
         if d_cached.nbytes < n:
             _short("d_cached", d_cached, n)
         if d_new.nbytes < n:
