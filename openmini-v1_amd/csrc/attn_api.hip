@@ -388,6 +388,7 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     TRY(check_range("table_stride", p->table_stride, p->max_pages, (int64_t)1 << 40));
     TRY(check_range("requests", p->requests, 1, kMaxI32));
     if (p->rows == 0) return ok();
+    const attn::Cache& c = a.cache;
     const int64_t held = p->max_pages * cache->page_size, max_len = held < kMostKeys ? held : kMostKeys;
     const uint32_t shares = attn::decode_shares(cache->kv_heads, head_tiles);
     // tiles of the call at most
@@ -418,6 +419,10 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     a.group = p->q_heads / cache->kv_heads;
     a.head_tiles = head_tiles;
     a.out_f32 = p->out_dtype == OPENMINI_ATTN_F32;
+    // the last byte that a lane's own offset reaches (heads and the eight keys of a group are
+    // added to the scalar address)
+    a.wide = (double)(c.n_pages - 1) * (double)c.page_stride + (double)(cache->page_size + 8) * (double)c.token_stride + 1024 >=
+             4294967296.0;
     a.scale = (float)((double)p->scale * cache->k_scale * 1.44269504088896340736);
     a.shares = shares;
     a.launch_shares = tiles < (int64_t)shares ? (uint32_t)tiles : shares;

@@ -239,7 +239,9 @@ __device__ __forceinline__ bool find_share(const First& a, uint32_t p, Share& ou
     return true;
 }
 
-template <int D, class T, bool F8, int kSub, int W>
+// kWide: a key's place in the cache takes 64 bits (caches of 4 GiB and more); else 32, which
+// the loads add to a scalar address by themselves.
+template <int D, class T, bool F8, int kSub, int W, bool kWide>
 __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(const int32_t* lens, const int32_t* rows,
                                                                                  uint32_t n_rows, uint32_t requests,
                                                                                  uint32_t max_len, uint32_t window,
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         }
     };
 
-    const uint8_t* k_lane = a.cache.k + kv * a.cache.head_stride + g * 16;
+    const uint8_t* k_base = a.cache.k + kv * a.cache.head_stride;
     const uint8_t* v_base = a.cache.v + kv * a.cache.head_stride;
     const int kg = col >> 2, k_row = col & 3;  // the lane's key of tile s: 8 kg + 4 s + k_row
 
@@ -326,57 +328,60 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     auto group_at = [&](const Tile& t, int sub, int grp) -> int32_t {
         return min(max((int32_t)(t.no * kKeys) + 32 * sub + 8 * grp, t.first_group), t.last_group);
     };
-    auto offset_of = [&](int32_t page, int32_t key) -> int64_t {
-        const uint32_t in_page = (uint32_t)key - a.cache.page.div_by_many((uint32_t)key) * a.cache.page.d;
-        return ((uint32_t)page < a.cache.n_pages ? (int64_t)page * a.cache.page_stride : 0) +
-               (int64_t)in_page * a.cache.token_stride;
-    };
-    struct Pages {
+    using Place = std::conditional_t<kWide, uint64_t, uint32_t>;
+    struct Pages {  // of a tile's K and V groups, and the groups' places in them
         int32_t k[kSub], v[kSub];
+        uint32_t k_in[kSub], v_in[kSub];
+    };
+    auto page_of = [&](const Tile& t, int32_t key, int32_t* page, uint32_t* in_page) {
+        const uint32_t at = a.cache.page.div_by_many((uint32_t)key);
+        *page = t.table[at];
+        *in_page = (uint32_t)key - at * a.cache.page.d;
     };
     auto pages_of = [&](const Tile& t) {
         Pages p;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            p.k[u] = t.table[a.cache.page.div_by_many((uint32_t)group_at(t, u, kg))];
-            p.v[u] = t.table[a.cache.page.div_by_many((uint32_t)group_at(t, u, g))];
+            page_of(t, group_at(t, u, kg), &p.k[u], &p.k_in[u]);
+            page_of(t, group_at(t, u, g), &p.v[u], &p.v_in[u]);
         }
         return p;
     };
+    auto place_of = [&](int32_t page, uint32_t in_page) -> Place {
+        return ((uint32_t)page < a.cache.n_pages ? (Place)(uint32_t)page * (Place)a.cache.page_stride : 0) +
+               (Place)in_page * (Place)a.cache.token_stride;
+    };
 
     uint32_t kraw[kSub][2][kKWords], vraw[kSub][8][kVWords];
-    auto load_k = [&](const Tile& t, const Pages& pages) {
+    auto load_k = [&](const Pages& pages) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            const uint8_t* p = k_lane + offset_of(pages.k[u], group_at(t, u, kg)) + k_row * a.cache.token_stride;
+            const Place at = place_of(pages.k[u], pages.k_in[u] + k_row) + g * 16;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const uint8_t* ps = p + 4 * s * a.cache.token_stride;
+                const uint8_t* p = k_base + 4 * s * a.cache.token_stride;
                 if constexpr (F8) {
 #pragma unroll
-                    for (int c = 0; c < kSteps / 2; ++c) load<16>(ps + c * 64, &kraw[u][s][4 * c]);
-                    if constexpr (kSteps & 1) load<8>(ps - g * 8 + (kSteps - 1) * 32, &kraw[u][s][2 * (kSteps - 1)]);
+                    for (int c = 0; c < kSteps / 2; ++c) load<16>(p + at + c * 64, &kraw[u][s][4 * c]);
+                    if constexpr (kSteps & 1) load<8>(p + (at - g * 8) + (kSteps - 1) * 32, &kraw[u][s][2 * (kSteps - 1)]);
                 } else {
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st) load<16>(ps + st * 64, &kraw[u][s][4 * st]);
+                    for (int st = 0; st < kSteps; ++st) load<16>(p + at + st * 64, &kraw[u][s][4 * st]);
                 }
             }
         }
     };
-    auto load_v = [&](const Tile& t, const Pages& pages) {
+    auto load_v = [&](const Pages& pages, int u) {
+        const Place at = place_of(pages.v[u], pages.v_in[u]);
+        const Place at128 = at + col * 8 * kEl, at64 = at + col * 4 * kEl, at32 = at + col * 2 * kEl;
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-            const uint8_t* p = v_base + offset_of(pages.v[u], group_at(t, u, g));
+        for (int j = 0; j < 8; ++j) {
+            const uint8_t* p = v_base + j * a.cache.token_stride;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint8_t* pj = p + j * a.cache.token_stride;
-#pragma unroll
-                for (int c = 0; c < kFull; ++c) load<8 * kEl>(pj + (c * 128 + col * 8) * kEl, &vraw[u][j][c * 2 * kEl]);
-                if constexpr (kHas64) load<4 * kEl>(pj + (kFull * 128 + col * 4) * kEl, &vraw[u][j][kFull * 2 * kEl]);
-                if constexpr (kHas32)
-                    load<2 * kEl>(pj + (kFull * 128 + kHas64 * 64 + col * 2) * kEl,
-                                  &vraw[u][j][kFull * 2 * kEl + kHas64 * kEl]);
-            }
+            for (int c = 0; c < kFull; ++c) load<8 * kEl>(p + at128 + c * 128 * kEl, &vraw[u][j][c * 2 * kEl]);
+            if constexpr (kHas64) load<4 * kEl>(p + at64 + kFull * 128 * kEl, &vraw[u][j][kFull * 2 * kEl]);
+            if constexpr (kHas32)
+                load<2 * kEl>(p + at32 + (kFull * 128 + kHas64 * 64) * kEl, &vraw[u][j][kFull * 2 * kEl + kHas64 * kEl]);
         }
     };
 
@@ -502,6 +507,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
             if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
             if constexpr (kHas32)
                 chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
+            load_v(then, u);  // the next tile's, into the registers that are free
         }
     };
 
@@ -522,17 +528,17 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
             now = pages_of(first);
             load_q(cur.row);
             then = pages_of(second);
-            load_k(first, now);
-            load_v(first, now);
+            load_k(now);
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) load_v(now, u);
         }
         for (; tile + 2 < cur.tile1; ++tile) {
             scores();
             // the pages of the tile after the next, then the next keys: their pages came
             // with loads that have been waited for
             const Pages later = pages_of(tile_of(cur, tile + 2));
-            load_k(tile_of(cur, tile + 1), then);
+            load_k(then);
             outputs(cur, tile);
-            load_v(tile_of(cur, tile + 1), then);
             now = then;
             then = later;
         }
@@ -550,11 +556,10 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
             const Tile after = loaded ? tile_of(following, min(following.tile0 + (last ? 1u : 0u), following.tile1 - 1)) : next;
             const Pages later = pages_of(after);
             if (cross && cur.tile1 - cur.tile0 == 1) then = pages_of(next);  // no tile before looked them up
-            load_k(next, then);
+            load_k(then);
             if (cross) load_q(following.row);
             outputs(cur, tile);
             if (last && !cross) break;
-            load_v(next, then);
             now = then;
             then = later;
         }
@@ -631,23 +636,29 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     }
 }
 
-template <int D, class T, bool F8>
+template <int D, class T, bool F8, bool kWide>
 hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
     constexpr int W = kDecodeWaves, kSub = decode_subtiles(D, F8);
     const uint64_t waves = (uint64_t)a.launch_shares * a.kv_heads * a.head_tiles, wgs = ((waves + W - 1) / W + 7) / 8 * 8;
-    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows, a.n_rows,
-                       a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift, a);
+    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
+                       a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift, a);
     return hipGetLastError();
+}
+
+template <int D, class T>
+hipError_t launch_dim(const DecodeArgs& a, bool f8, hipStream_t s) {
+    if (a.wide) return f8 ? launch_one<D, T, true, true>(a, s) : launch_one<D, T, false, true>(a, s);
+    return f8 ? launch_one<D, T, true, false>(a, s) : launch_one<D, T, false, false>(a, s);
 }
 
 template <class T>
 hipError_t launch_type(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s) {
     switch (head_dim) {
-    case 64: return f8 ? launch_one<64, T, true>(a, s) : launch_one<64, T, false>(a, s);
-    case 96: return f8 ? launch_one<96, T, true>(a, s) : launch_one<96, T, false>(a, s);
-    case 128: return f8 ? launch_one<128, T, true>(a, s) : launch_one<128, T, false>(a, s);
-    case 192: return f8 ? launch_one<192, T, true>(a, s) : launch_one<192, T, false>(a, s);
-    case 256: return f8 ? launch_one<256, T, true>(a, s) : launch_one<256, T, false>(a, s);
+    case 64: return launch_dim<64, T>(a, f8, s);
+    case 96: return launch_dim<96, T>(a, f8, s);
+    case 128: return launch_dim<128, T>(a, f8, s);
+    case 192: return launch_dim<192, T>(a, f8, s);
+    case 256: return launch_dim<256, T>(a, f8, s);
     default: return hipErrorInvalidValue;
     }
 }

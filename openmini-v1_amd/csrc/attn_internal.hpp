@@ -114,6 +114,7 @@ struct DecodeArgs {
     uint32_t window;                     // keys that a row sees at most
     int32_t q_heads, kv_heads, group, head_tiles;
     int32_t out_f32;
+    int32_t wide;  // a key's place in the cache takes more than 32 bits
     float scale;  // of a raw product, in powers of two: scale * k_scale * log2(e)
     // Shares of the call's tiles for each of the units = kv_heads * head_tiles, at most, and
     // those that waves are launched for.
