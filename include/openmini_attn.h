@@ -8,7 +8,7 @@
  * codes these calls return: no call aborts, a failing one leaves its message in
  * openmini_qmm_last_error() and goes to the log callback; d_* are device pointers that
  * stay valid until the stream reaches the call; `stream` NULL is the null stream.  Every
- * call only enqueues work (one kernel launch, attention two; no allocation, no copy, no
+ * call only enqueues work (one kernel launch, attention at most two; no allocation, no copy, no
  * synchronisation), so a stream capture may hold them.
  *
  * All numbers of tokens, slots and pages are int32 on the device.  What a call reads from
@@ -177,15 +177,17 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
  *
  * Types: q F16 or BF16 and the cache the same type, or F8_E4M3, which is converted to q's
  * (exactly); out q's type or F32.  Products are of 16-bit operands with 32-bit sums; the
- * probabilities enter the second product as the sum of two 16-bit parts, so an F32 output
- * keeps about 2^-17 of its size.  head_dim: 64, 96, 128, 192 or 256; page_size: a multiple
+ * probabilities enter the second product as the sum of two (F16) or three (BF16) 16-bit
+ * parts, which hold 22 or 24 bits of them.  head_dim: 64, 96, 128, 192 or 256; page_size: a multiple
  * of 8; q_heads: a multiple of kv_heads, at most 1024.
  *
  * Long rows are cut into parts that separate waves take, and a second launch joins a row's
- * parts in their order.  How they are cut depends on all lengths of the call, so the last
- * bits of a row may differ between calls with other rows beside it; equal calls give equal
- * bits.  d_work: openmini_attn_workspace_bytes bytes, 256-byte aligned, of any content;
- * two calls that share it must not overlap in time. */
+ * parts in their order; where the tables and the window leave only short rows, a workgroup
+ * takes a row and there is no second launch (so max_pages is best no more than the call's
+ * longest row needs; table_stride is free).  How rows are cut depends on all lengths of the
+ * call and on max_pages, so the last bits of a row may differ between calls with other rows
+ * beside it; equal calls give equal bits.  d_work: openmini_attn_workspace_bytes bytes,
+ * 256-byte aligned, of any content; two calls that share it must not overlap in time. */
 typedef struct {
     const void* d_q;
     int64_t q_stride; /* elements from a row to the next; a row is [q_heads][head_dim] */

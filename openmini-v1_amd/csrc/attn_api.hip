@@ -433,10 +433,13 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     a.part_ml = reinterpret_cast<float2*>(work + w.ml_at);
     a.part_acc = reinterpret_cast<float*>(work + w.acc_at);
     a.by_row = p->rows <= (int64_t)shares;
+    const int64_t keys = max_len < (int64_t)a.window ? max_len : (int64_t)a.window, tile = 32 * attn::decode_subtiles(cache->head_dim, f8);
+    // a window's first tile need not begin with it
+    a.whole = attn::decode_whole((keys + tile - 1) / tile + (keys < max_len), p->rows * cache->kv_heads * head_tiles);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = p->q_dtype == OPENMINI_ATTN_BF16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)
                                                     : attn::launch_decode_f16(a, cache->head_dim, f8, s);
-    if (e == hipSuccess && a.launch_shares > 1) e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
+    if (e == hipSuccess && !a.whole && a.launch_shares > 1) e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
     return launched(e, "attention launch");
 }
 

@@ -241,7 +241,11 @@ __device__ __forceinline__ bool find_share(const First& a, uint32_t p, Share& ou
 
 // kWide: a key's place in the cache takes 64 bits (caches of 4 GiB and more); else 32, which
 // the loads add to a scalar address by themselves.
-template <int D, class T, bool F8, int kSub, int W, bool kWide>
+// kWhole: a workgroup takes a row of one unit, its waves equal runs of the row's tiles, and
+// they are joined in LDS: one launch, and no wave that looks for its share, but as many CUs
+// as there are rows and units, and a CU reads about 50 GB/s.  For short rows (decode_whole);
+// the last tile of a wave is most of its work then, so no loads of a next one are behind it.
+template <int D, class T, bool F8, int kSub, int W, bool kWide, bool kWhole>
 __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(const int32_t* lens, const int32_t* rows,
                                                                                  uint32_t n_rows, uint32_t requests,
                                                                                  uint32_t max_len, uint32_t window,
@@ -269,11 +273,21 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     // values in bf16, heads of 128, loads alone: 88 us; a workgroup to a head: 95 us).
     const uint32_t line = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const uint32_t w_no = line * W + (uint32_t)wave;
-    const uint32_t share_no = units_m ? __umulhi(w_no, units_m) >> units_shift : w_no, unit = w_no - share_no * units;
+    const uint32_t at = kWhole ? line : w_no;  // share_no: the row, kWhole
+    const uint32_t share_no = units_m ? __umulhi(at, units_m) >> units_shift : at, unit = at - share_no * units;
     const uint32_t kv = a.by_head_tiles.div(unit), head_tile = unit - kv * (uint32_t)a.head_tiles;
     Share share;
     Said said;
-    if (!find_share<kKeys, W>(f, share_no, share, said)) {
+    if constexpr (kWhole) {
+        if (share_no >= n_rows) return;
+        said = said_of_uniform(f, share_no);
+        const uint32_t weight = span_of<kKeys>(f, said).weight();
+        share.each = (weight + W - 1) / W;
+        share.from = min(share.each * wave, weight);
+        share.to = min(share.from + share.each, weight);
+        share.row = share_no;
+        share.row_at = 0;
+    } else if (!find_share<kKeys, W>(f, share_no, share, said)) {
         if (!a.by_row && unit == 0 && share_no < shares && lane == 0) a.split[share_no] = Split{0, 0, 0};
         return;
     }
@@ -409,7 +423,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                 }
             }
     };
-    auto outputs = [&](const Row& cur, uint32_t tile) {
+    auto outputs = [&](const Row& cur, uint32_t tile, auto next_tag) {
         // keys outside the row's or on no page of the cache: only a row's first and
         // last tiles, and broken tables, have them
         float x[kSub][8];
@@ -507,7 +521,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
             if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
             if constexpr (kHas32)
                 chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
-            load_v(then, u);  // the next tile's, into the registers that are free
+            // the next tile's, into the registers that are free
+            if constexpr (decltype(next_tag)::value) load_v(then, u);
         }
     };
 
@@ -516,13 +531,14 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     Row cur = row_of(share.row, share.row_at, share.from, said);
     bool loaded = false;  // cur's first tile is on its way
     for (;;) {
-        const bool more = cur.end < share.to;
+        const bool more = !kWhole && cur.end < share.to;
         if (more) said = said_of_uniform(f, cur.row + 1);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0, 0, 0, 0};
         m = -INFINITY;
         l = 0;
         uint32_t tile = cur.tile0;
+        Row following = cur;
         if (!loaded && tile < cur.tile1) {
             const Tile first = tile_of(cur, tile), second = tile_of(cur, min(tile + 1, cur.tile1 - 1));
             now = pages_of(first);
@@ -532,36 +548,50 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
 #pragma unroll
             for (int u = 0; u < kSub; ++u) load_v(now, u);
         }
-        for (; tile + 2 < cur.tile1; ++tile) {
-            scores();
-            // the pages of the tile after the next, then the next keys: their pages came
-            // with loads that have been waited for
-            const Pages later = pages_of(tile_of(cur, tile + 2));
-            load_k(then);
-            outputs(cur, tile);
-            now = then;
-            then = later;
-        }
-        // The row's last two tiles, before which come the next row's first.  At the share's
-        // end (or before a row without keys) the next tile is the present one again: loads
-        // without a branch around them, so that the wait for the present values need not
-        // cover them.
-        Row following = cur;
-        if (more) following = row_of(cur.row + 1, cur.end, cur.end, said);
-        loaded = tile < cur.tile1 && more && following.tile0 < following.tile1;
-        for (; tile < cur.tile1; ++tile) {
-            const bool last = tile + 1 == cur.tile1, cross = last && loaded;
-            scores();
-            const Tile next = cross ? tile_of(following, following.tile0) : tile_of(cur, last ? tile : tile + 1);
-            const Tile after = loaded ? tile_of(following, min(following.tile0 + (last ? 1u : 0u), following.tile1 - 1)) : next;
-            const Pages later = pages_of(after);
-            if (cross && cur.tile1 - cur.tile0 == 1) then = pages_of(next);  // no tile before looked them up
-            load_k(then);
-            if (cross) load_q(following.row);
-            outputs(cur, tile);
-            if (last && !cross) break;
-            now = then;
-            then = later;
+        if constexpr (kWhole) {
+            for (; tile + 1 < cur.tile1; ++tile) {
+                scores();
+                const Pages later = pages_of(tile_of(cur, min(tile + 2, cur.tile1 - 1)));
+                load_k(then);
+                outputs(cur, tile, std::true_type{});
+                now = then;
+                then = later;
+            }
+            if (tile < cur.tile1) {
+                scores();
+                outputs(cur, tile, std::false_type{});
+            }
+        } else {
+            for (; tile + 2 < cur.tile1; ++tile) {
+                scores();
+                // the pages of the tile after the next, then the next keys: their pages came
+                // with loads that have been waited for
+                const Pages later = pages_of(tile_of(cur, tile + 2));
+                load_k(then);
+                outputs(cur, tile, std::true_type{});
+                now = then;
+                then = later;
+            }
+            // The row's last two tiles, before which come the next row's first.  At the share's
+            // end (or before a row without keys) the next tile is the present one again: loads
+            // without a branch around them, so that the wait for the present values need not
+            // cover them.
+            if (more) following = row_of(cur.row + 1, cur.end, cur.end, said);
+            loaded = tile < cur.tile1 && more && following.tile0 < following.tile1;
+            for (; tile < cur.tile1; ++tile) {
+                const bool last = tile + 1 == cur.tile1, cross = last && loaded;
+                scores();
+                const Tile next = cross ? tile_of(following, following.tile0) : tile_of(cur, last ? tile : tile + 1);
+                const Tile after = loaded ? tile_of(following, min(following.tile0 + (last ? 1u : 0u), following.tile1 - 1)) : next;
+                const Pages later = pages_of(after);
+                if (cross && cur.tile1 - cur.tile0 == 1) then = pages_of(next);  // no tile before looked them up
+                load_k(then);
+                if (cross) load_q(following.row);
+                outputs(cur, tile, std::true_type{});
+                if (last && !cross) break;
+                now = then;
+                then = later;
+            }
         }
 
         l = column_sum(l);
@@ -576,6 +606,52 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                 c += width;
             }
         };
+        if constexpr (kWhole) {
+            // a wave past the row's tiles has seen nothing: maximum -inf, sum 0
+            __shared__ __attribute__((aligned(16))) float part[W][kHeadTile][D + 4];
+            __shared__ float2 part_ml[W][kHeadTile];
+            if (col < heads) {
+                each_run([&](int t, int i, int width, int d) {
+                    float* o = &part[wave][col][d];
+                    if (width >= 4) {
+#pragma unroll
+                        for (int e = 0; e < width; e += 4)
+                            *reinterpret_cast<f32x4*>(o + e) =
+                                f32x4{acc[t + e][i], acc[t + e + 1][i], acc[t + e + 2][i], acc[t + e + 3][i]};
+                    } else {
+                        *reinterpret_cast<float2*>(o) = make_float2(acc[t][i], acc[t + 1][i]);
+                    }
+                });
+                if (g == 0) part_ml[wave][col] = make_float2(m, l);
+            }
+            __syncthreads();
+            for (int at = (int)threadIdx.x; at < heads * (D / 4); at += 64 * W) {
+                const int h = at / (D / 4), d = at % (D / 4) * 4;
+                float2 ml[W];
+                float top = -INFINITY, sum = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    ml[w] = part_ml[w][h];
+                    top = fmaxf(top, ml[w].x);
+                }
+                f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float by = exp2_of(ml[w].x - above(top));
+                    sum += ml[w].y * by;
+                    v += *reinterpret_cast<const f32x4*>(&part[w][h][d]) * by;
+                }
+                v *= sum > 0 || sum != sum ? a.cache.v_scale / sum : 0.0f;
+                const int64_t to = (int64_t)(head0 + h) * D + d;
+                uint8_t* out = a.out + cur.row * a.out_stride;
+                if (a.out_f32)
+                    *reinterpret_cast<f32x4*>(out + to * 4) = v;
+                else
+                    *reinterpret_cast<uint2*>(out + to * 2) = make_uint2(T::pair(v[0], v[1]), T::pair(v[2], v[3]));
+                if (a.lse && d == 0) a.lse[(int64_t)cur.row * a.q_heads + head0 + h] = log_sum(top, sum);
+            }
+            return;
+        }
         // the row's shares: all but the first begin inside it
         const uint32_t row = cur.row, first_share = cur.at / share.each, parts = (cur.end - 1) / share.each - first_share + 1;
         if (a.by_row && unit == 0 && lane == 0 && share_no == first_share) a.split[row] = Split{row, first_share, parts};
@@ -636,19 +712,25 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     }
 }
 
-template <int D, class T, bool F8, bool kWide>
+template <int D, class T, bool F8, bool kWide, bool kWhole>
 hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
-    constexpr int W = kDecodeWaves, kSub = decode_subtiles(D, F8);
-    const uint64_t waves = (uint64_t)a.launch_shares * a.kv_heads * a.head_tiles, wgs = ((waves + W - 1) / W + 7) / 8 * 8;
-    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
+    constexpr int W = kWhole && !(D == 256 && !F8) ? 2 * kDecodeWaves : kDecodeWaves, kSub = decode_subtiles(D, F8);
+    const uint64_t units = (uint64_t)a.kv_heads * a.head_tiles;
+    const uint64_t all = kWhole ? a.n_rows * units : (a.launch_shares * units + W - 1) / W, wgs = (all + 7) / 8 * 8;
+    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide, kWhole>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
                        a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift, a);
     return hipGetLastError();
 }
 
+template <int D, class T, bool F8>
+hipError_t launch_f8(const DecodeArgs& a, hipStream_t s) {
+    if (a.whole) return launch_one<D, T, F8, true, true>(a, s);
+    return a.wide ? launch_one<D, T, F8, true, false>(a, s) : launch_one<D, T, F8, false, false>(a, s);
+}
+
 template <int D, class T>
 hipError_t launch_dim(const DecodeArgs& a, bool f8, hipStream_t s) {
-    if (a.wide) return f8 ? launch_one<D, T, true, true>(a, s) : launch_one<D, T, false, true>(a, s);
-    return f8 ? launch_one<D, T, true, false>(a, s) : launch_one<D, T, false, false>(a, s);
+    return f8 ? launch_f8<D, T, true>(a, s) : launch_f8<D, T, false>(a, s);
 }
 
 template <class T>

@@ -97,6 +97,15 @@ constexpr int kMaxHeads = 1024;  // query heads
 // and 104 us, the call takes 106 us instead of 99; 512 waves 117).
 constexpr int kRound = 1024;
 
+// Whether workgroups take whole rows: `most` tiles in a row at most, by the table's columns
+// and the window, and `pairs` of a row and a unit.  Up to two workgroups for each CU, and rows
+// of up to two tiles a wave, or four where the shares are no more than 16 for each pair
+// either.  Measured, whole rows against shares (us): 8 pairs of 300 keys, heads of 128, bf16
+// 7.0 / 9.4, of 700 9.8 / 10.7, of 1000 12.5 / 10.9; 64 pairs of 1000 13.5 / 16.2, of 2000
+// 22.6 / 18.5; 512 pairs of 400 15.1 / 20.4; 1024 pairs of 200, e4m3 16.6 / 16.3, of 60
+// 14.3 / 9.5.
+inline bool decode_whole(int64_t most, int64_t pairs) { return pairs <= 512 && most <= (pairs < 64 ? 16 : 32); }
+
 // A row of several parts (parts > 1), in shares first_share on.
 struct Split {
     uint32_t row, first_share, parts;
@@ -126,6 +135,7 @@ struct DecodeArgs {
     float2* part_ml;  // [shares][2][q_heads]: maximum, sum
     Split* split;     // [shares]
     int32_t by_row;
+    int32_t whole;  // a row of a unit to a workgroup, and no join
 };
 
 // Shares of a call, at most.

@@ -202,18 +202,23 @@ class CachedAttention:
         self.d_q16, self.d_attn = DeviceBuffer(max_tokens * q * 2), DeviceBuffer(max_tokens * q * 4)
 
     def forward_device(self, d_x: DeviceBuffer, plan: StepPlan, d_tables, requests: int, tokens: int, d_out: DeviceBuffer,
-                       d_positions=None, stream=None) -> None:
+                       d_positions=None, stream=None, max_pages: int | None = None) -> None:
         """d_out [tokens, hidden] for the step that `plan` laid out (plan.run on the same
         stream before the first layer): d_x [tokens, hidden] fp32, d_tables the tables that
-        the plan filled.  d_positions [axes][tokens]: None takes the plan's (one axis)."""
+        the plan filled.  d_positions [axes][tokens]: None takes the plan's (one axis).
+        max_pages: columns that the step's longest request needs, where that is known (None:
+        the tables' width); attention of short rows is faster for it."""
+        most = plan.max_pages if max_pages is None else int(max_pages)
+        if not 0 < most <= plan.max_pages:
+            raise InvalidInput(f"max_pages {most}, tables of {plan.max_pages}")
         if tokens > min(self.max_tokens, plan.max_tokens):
             raise InvalidInput(f"{tokens} tokens, planned for {min(self.max_tokens, plan.max_tokens)}")
         w = self.weights
         w.project_qkv_device(d_x, self.d_q, self.d_k, self.d_v, tokens, stream)
         self.rope.append(self.cache, self.d_q, self.d_k, self.d_v, DType.F32, self.d_q16, self.q_dtype,
                          plan.positions if d_positions is None else d_positions, plan.slots, tokens, self.q_heads, stream)
-        self.attention.run(self.cache, self.d_q16, self.d_attn, d_tables, plan.max_pages, plan.row_lens, tokens,
-                           d_rows=plan.rows, requests=requests, stream=stream)
+        self.attention.run(self.cache, self.d_q16, self.d_attn, d_tables, most, plan.row_lens, tokens,
+                           d_rows=plan.rows, requests=requests, table_stride=plan.max_pages, stream=stream)
         w.o_proj.gemv(self.d_attn, d_out, tokens, stream)
 
 

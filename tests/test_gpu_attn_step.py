@@ -118,3 +118,21 @@ def test_refusals(qmm, orc):
         qmm.StepPlan(PAGE, 1, 8, 4, buffers={"slot": d})
     with pytest.raises(qmm.InvalidInput):
         plan.run(d, d, 2, d, d, 4)
+
+
+def test_max_pages(qmm, orc):
+    """Fewer columns of the same tables, as many as the step needs: the same outputs, to
+    2^-16 of the largest: fp32 sums of the same products in other orders, then a sum of 512."""
+    layer = Layer(qmm, orc, 0xF00, F16, 1)
+    width, buf = 400, qmm.DeviceBuffer.from_numpy
+    plan, tables = qmm.StepPlan(PAGE, 2, 64, width), qmm.DeviceBuffer(2 * width * 4)
+    plan.run(buf(np.zeros(2, np.int32)), buf(np.array([20, 33], np.int32)), 2, tables, buf(np.arange(24, dtype=np.int32)), 24)
+    d_x, outs = buf(np.random.default_rng(10).standard_normal((53, HIDDEN)).astype(np.float32)), []
+    for max_pages in (None, 3):
+        d_out = qmm.DeviceBuffer(53 * HIDDEN * 4)
+        layer.step.forward_device(d_x, plan, tables, 2, 53, d_out, max_pages=max_pages)
+        outs.append(d_out.download(np.float32, (53, HIDDEN)))
+    assert np.max(np.abs(outs[0] - outs[1])) <= 2.0 ** -16 * np.max(np.abs(outs[0]))
+    for bad in (0, width + 1):
+        with pytest.raises(qmm.InvalidInput, match="max_pages"):
+            layer.step.forward_device(d_x, plan, tables, 2, 53, d_out, max_pages=bad)
