@@ -22,11 +22,16 @@
 // output, to two 2^-18 (1.2e-6 measured, against 4e-7 for fp32 arithmetic throughout).
 // Sums, maxima and the joined parts are fp32.
 //
-// Bound by memory: 4 operations a byte for each query head of a key head.  The loads of the
-// next keys are issued as soon as the registers of the present ones are free, about 16 KB a
-// wave, one wave to a SIMD.  Measured (MI355X, GB/s of keys and values, second launch
-// included): 131071 keys of one row, 8 heads of 128, bf16 99.8 us, 5380 GB/s (a read of as
-// many bytes 84 us); 128 rows of 2000 - 12000 keys, e4m3, 270 us, 5560 GB/s.
+// Bound by memory: one operation a byte (e4m3: two) for each query head of a key head.  A tile
+// of 32, 64 or 128 keys is about 16 KB; the loads of the next tile are issued as soon as the
+// registers of the present one are free, one wave to a SIMD, a row's first behind the last
+// products of the row before.  Measured (MI355X, us with the second launch, which is 4 to 6
+// of them; in brackets a read of as many bytes): 131071 keys of one row, 8 heads of 128, bf16
+// 98 (84), the kernel alone 92, 5.8 TB/s; 16 rows of 700 - 2100 keys, 32 heads of 128, fp16 60
+// (50); 64 rows of up to 4096 keys in a window, 4 heads of 64, bf16 28 (17); 128 rows of 2000 -
+// 12000 keys, 8 heads of 128, e4m3 271 (230).  One row of 300 keys, in one launch, 6.9 (2.4, a
+// launch).  Heads of 64 in e4m3 are bound by the issue of instructions instead (183 vector
+// instructions for 32 keys): 100 rows of 1000 - 8000 keys, 8 heads, 84 us, 4.4 TB/s.
 #pragma once
 
 #include <type_traits>

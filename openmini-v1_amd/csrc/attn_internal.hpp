@@ -102,8 +102,8 @@ constexpr int kRound = 1024;
 // of up to two tiles a wave, or four where the shares are no more than 16 for each pair
 // either.  Measured, whole rows against shares (us): 8 pairs of 300 keys, heads of 128, bf16
 // 7.0 / 9.4, of 700 9.8 / 10.7, of 1000 12.5 / 10.9; 64 pairs of 1000 13.5 / 16.2, of 2000
-// 22.6 / 18.5; 512 pairs of 400 15.1 / 20.4; 1024 pairs of 200, e4m3 16.6 / 16.3, of 60
-// 14.3 / 9.5.
+// 22.6 / 18.5; 256 of up to 4000, heads of 64, 46.8 / 36.4; 512 of 400 15.1 / 20.4; 1024 of
+// 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.
 inline bool decode_whole(int64_t most, int64_t pairs) { return pairs <= 512 && most <= (pairs < 64 ? 16 : 32); }
 
 // A row of several parts (parts > 1), in shares first_share on.

@@ -12,6 +12,9 @@
 // and two stores of four; neighbouring lanes take neighbouring items.  Bound by memory for
 // prompts and by latency for single tokens, whose heads are spread over workgroups (each
 // making the token's sines again); the first items' loads are issued before the sines.
+// Measured (MI355X): 16128 tokens of 16 heads of 128, fp32 to bf16 37 us, 5.3 TB/s read and
+// written (a plain copy of as many bytes that converts alike 30 us); 8191 tokens of 32 + 64
+// heads of 128 into an fp16 cache, all of it, 112 us, 5.4 TB/s; one token 2.8 - 3.4 us.
 #include "attn_internal.hpp"
 
 namespace attn {
