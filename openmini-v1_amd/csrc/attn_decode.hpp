@@ -255,7 +255,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                                                                                  uint32_t n_rows, uint32_t requests,
                                                                                  uint32_t max_len, uint32_t window,
                                                                                  uint32_t shares, uint32_t units,
-                                                                                 uint32_t units_m, uint32_t units_shift,
+                                                                                 uint32_t units_m, uint32_t units_shift, uint32_t eighth,
                                                                                  DecodeArgs a) {
     const First f = {lens, rows, n_rows, requests, max_len, window, shares};
     constexpr int kEl = F8 ? 1 : 2;           // bytes of a cache element
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     // the line.  So the heads of a share run side by side: in a cache of
     // [tokens][heads][dims] they read whole stretches of memory together (537 MB of keys and
     // values in bf16, heads of 128, loads alone: 88 us; a workgroup to a head: 95 us).
-    const uint32_t line = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const uint32_t line = (blockIdx.x & 7) * eighth + (blockIdx.x >> 3);
     const uint32_t w_no = line * W + (uint32_t)wave;
     const uint32_t at = kWhole ? line : w_no;  // share_no: the row, kWhole
     const uint32_t share_no = units_m ? __umulhi(at, units_m) >> units_shift : at, unit = at - share_no * units;
@@ -723,7 +723,8 @@ hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
     const uint64_t units = (uint64_t)a.kv_heads * a.head_tiles;
     const uint64_t all = kWhole ? a.n_rows * units : (a.launch_shares * units + W - 1) / W, wgs = (all + 7) / 8 * 8;
     hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide, kWhole>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
-                       a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift, a);
+                       a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift,
+                       (uint32_t)(wgs / 8), a);
     return hipGetLastError();
 }
 

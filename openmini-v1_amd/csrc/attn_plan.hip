@@ -69,7 +69,7 @@ constexpr uint32_t kRefused = 0x80000000u;  // in `before`, whose sums stay belo
 __global__ __launch_bounds__(kThreads) void plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ fresh,
                                                         const int32_t* __restrict__ free, uint32_t requests, uint32_t max_held,
                                                         uint32_t max_tokens, uint32_t page_d, uint32_t page_m,
-                                                        uint32_t page_shift, PlanArgs a) {
+                                                        uint32_t page_shift, uint32_t threads, PlanArgs a) {
     extern __shared__ uint32_t lds[];  // [requests] first tokens, [requests] pages before, [requests] cached tokens
     __shared__ uint32_t wave_tokens[kThreads / 64], wave_pages[kThreads / 64];
     __shared__ uint32_t taken, refused;
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const int32_t* __restric
     }
 
     const uint32_t most = max(max(max_tokens, requests + 1), total_pages);
-    for (uint64_t at = (uint64_t)blockIdx.x * kThreads + tid; at < most; at += (uint64_t)gridDim.x * kThreads) {
+    for (uint64_t at = (uint64_t)blockIdx.x * kThreads + tid; at < most; at += threads) {
         const uint32_t i = (uint32_t)at;
         if (i < requests) {
             a.starts[i] = (int32_t)first[i];
@@ -179,9 +179,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const int32_t* __restric
 
 hipError_t launch_plan(const PlanArgs& a, hipStream_t s) {
     const uint64_t most = a.max_tokens > a.requests + 1 ? a.max_tokens : a.requests + 1;
-    const uint64_t wgs = (most + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(plan_kernel, dim3((unsigned)(wgs < 1024 ? wgs : 1024)), dim3(kThreads), 3 * 4 * (size_t)a.requests,
-                       s, a.cached, a.fresh, a.free, a.requests, a.max_held, a.max_tokens, a.page.d, a.page.m, a.page.shift, a);
+    const uint64_t all = (most + kThreads - 1) / kThreads;
+    const unsigned wgs = (unsigned)(all < 1024 ? all : 1024);
+    hipLaunchKernelGGL(plan_kernel, dim3(wgs), dim3(kThreads), 3 * 4 * (size_t)a.requests,
+                       s, a.cached, a.fresh, a.free, a.requests, a.max_held, a.max_tokens, a.page.d, a.page.m, a.page.shift, wgs * kThreads, a);
     return hipGetLastError();
 }
 

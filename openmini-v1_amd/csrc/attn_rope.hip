@@ -137,7 +137,7 @@ __device__ __forceinline__ Item item_of(const RopeArgs& a, uint32_t i) {
 }
 
 template <int kIn, bool kStream>
-__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim, int wg_tokens) {
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim, int wg_tokens, uint32_t step) {
     __shared__ __attribute__((aligned(16))) float sines[kMaxTokens * kMaxPairs], cosines[kMaxTokens * kMaxPairs];
     __shared__ int64_t places[kMaxTokens];  // byte offset of a token's slot, or -1
     constexpr int kSize = kIn == OPENMINI_ATTN_F32 ? 4 : 2;
@@ -146,7 +146,6 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim
     const uint32_t mine = (uint32_t)min((int64_t)wg_tokens, a.tokens - token0);
     const uint32_t total = mine * a.per_token.d;
     const int y_size = size_of(a.y_dtype), c_size = size_of(a.cache_dtype);
-    const uint32_t step = gridDim.y * kThreads;
 
     bool first_round = true;
     for (uint32_t i0 = blockIdx.y * kThreads; i0 < total; i0 += kBatch * step) {
@@ -228,9 +227,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim
 template <int kIn>
 static void launch_type(const RopeArgs& a, int head_dim, dim3 grid, int wg_tokens, bool stream, hipStream_t s) {
     if (stream)
-        hipLaunchKernelGGL((rope_kernel<kIn, true>), grid, dim3(kThreads), 0, s, a, head_dim, wg_tokens);
+        hipLaunchKernelGGL((rope_kernel<kIn, true>), grid, dim3(kThreads), 0, s, a, head_dim, wg_tokens, grid.y * kThreads);
     else
-        hipLaunchKernelGGL((rope_kernel<kIn, false>), grid, dim3(kThreads), 0, s, a, head_dim, wg_tokens);
+        hipLaunchKernelGGL((rope_kernel<kIn, false>), grid, dim3(kThreads), 0, s, a, head_dim, wg_tokens, grid.y * kThreads);
 }
 
 hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s) {
