@@ -9,12 +9,13 @@
 // series.  A workgroup makes the sines of its tokens once, in LDS, for all their heads.
 //
 // An item is eight elements of a head (four pairs, or eight that pass through), two loads
-// and two stores of four; neighbouring lanes take neighbouring items.  Bound by memory for
+// and two stores of four; neighbouring lanes take neighbouring items.  A thread takes the
+// same item of its tokens, so what an item is, is worked out once.  Bound by memory for
 // prompts and by latency for single tokens, whose heads are spread over workgroups (each
-// making the token's sines again); the first items' loads are issued before the sines.
-// Measured (MI355X): 16128 tokens of 16 heads of 128, fp32 to bf16 37 us, 5.3 TB/s read and
-// written (a plain copy of as many bytes that converts alike 30 us); 8191 tokens of 32 + 64
-// heads of 128 into an fp16 cache, all of it, 112 us, 5.4 TB/s; one token 2.8 - 3.4 us.
+// making the token's sines again); the loads are issued before the sines.
+// Measured (MI355X): 16128 tokens of 16 heads of 128, fp32 to bf16 35 us, 5.6 TB/s read and
+// written (a copy alone that converts alike, in the same pieces, 31); 8191 tokens of 32 + 64
+// heads of 128 into an fp16 cache 114 us, 5.3 TB/s (the copy 93); one token 2.8 - 3.4 us.
 #include "attn_internal.hpp"
 
 namespace attn {
@@ -24,8 +25,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 3;      // items a thread loads before it stores
-constexpr int kMaxTokens = 8;  // tokens of a workgroup
+// Tokens of a thread where a call streams: 64 bytes of loads.
+constexpr int batch_of(int in) { return in == OPENMINI_ATTN_F32 ? 2 : 4; }
+constexpr uint32_t kMostBeside = 32;  // tokens side by side in a workgroup
+static_assert(4 * kMostBeside <= kThreads, "a thread to each token's slot");
 
 // sin and cos of `phase` / 2^64 revolutions.  Series on [-pi/4, pi/4]: the first term left
 // out is below 2e-9 (sine, x^11 / 11!) and 2e-10 (cosine, x^12 / 12!).
@@ -108,16 +111,14 @@ __device__ __forceinline__ float4 scaled(float4 v, float f) { return make_float4
 
 // What an item is: its head (of q, k or v), and where its two fours of elements are.
 struct Item {
-    int32_t token, head, first, second, pair;  // token of the workgroup; pair < 0: passes through
-    int32_t part;                              // 0 q, 1 k, 2 v
+    int32_t head, first, second, pair;  // pair < 0: passes through
+    int32_t part;                       // 0 q, 1 k, 2 v
 };
 
 __device__ __forceinline__ Item item_of(const RopeArgs& a, uint32_t i) {
     Item t;
-    t.token = (int32_t)a.per_token.div(i);
-    const uint32_t in_token = i - (uint32_t)t.token * a.per_token.d;
-    const uint32_t h = a.per_head.div(in_token);
-    const int32_t u = (int32_t)(in_token - h * a.per_head.d);
+    const uint32_t h = a.per_head.div(i);
+    const int32_t u = (int32_t)(i - h * a.per_head.d);
     t.head = (int32_t)h;
     t.part = 0;
     if (t.head >= a.heads) {
@@ -136,88 +137,81 @@ __device__ __forceinline__ Item item_of(const RopeArgs& a, uint32_t i) {
     return t;
 }
 
-template <int kIn, bool kStream>
-__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim, int wg_tokens, uint32_t step) {
-    __shared__ __attribute__((aligned(16))) float sines[kMaxTokens * kMaxPairs], cosines[kMaxTokens * kMaxPairs];
-    __shared__ int64_t places[kMaxTokens];  // byte offset of a token's slot, or -1
+// A workgroup takes kThreads items of kTokens tokens, or where a token has fewer all of
+// kTokens * beside tokens; a thread one item, of kTokens tokens.
+template <int kIn, bool kStream, int kTokens>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim, uint32_t beside) {
+    extern __shared__ __attribute__((aligned(16))) float sines[];  // [tokens][pairs], and as many cosines
+    __shared__ int64_t places[kTokens * kMostBeside];              // byte offset of a token's slot, or -1
     constexpr int kSize = kIn == OPENMINI_ATTN_F32 ? 4 : 2;
-    const uint32_t tid = threadIdx.x;
-    const int64_t token0 = (int64_t)blockIdx.x * wg_tokens;
-    const uint32_t mine = (uint32_t)min((int64_t)wg_tokens, a.tokens - token0);
-    const uint32_t total = mine * a.per_token.d;
+    const uint32_t tid = threadIdx.x, items = a.per_token.d;
+    const int64_t token0 = (int64_t)blockIdx.x * (kTokens * beside);
+    const uint32_t mine = (uint32_t)min((int64_t)(kTokens * beside), a.tokens - token0);
     const int y_size = size_of(a.y_dtype), c_size = size_of(a.cache_dtype);
+    float* cosines = sines + kTokens * beside * a.n_pairs;
 
-    bool first_round = true;
-    for (uint32_t i0 = blockIdx.y * kThreads; i0 < total; i0 += kBatch * step) {
-        Item items[kBatch];
-        float4 lo[kBatch], hi[kBatch];
+    const uint32_t sub = beside > 1 ? a.per_token.div(tid) : 0, item = blockIdx.y * kThreads + tid - sub * items;
+    const bool active = sub < beside && item < items;
+    Item t = {};
+    float4 lo[kTokens], hi[kTokens];
+    if (active) {
+        t = item_of(a, item);
+        const int64_t stride = t.part == 0 ? a.x_stride : t.part == 1 ? a.k_stride : a.v_stride;
+        const uint8_t* src = (t.part == 0 ? a.x : t.part == 1 ? a.k : a.v) + (token0 + sub) * stride + (int64_t)t.head * head_dim * kSize;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const uint32_t i = i0 + (uint32_t)b * step + tid;
-            if (i >= total) continue;
-            const Item t = items[b] = item_of(a, i);
-            const int64_t token = token0 + t.token;
-            const uint8_t* src = t.part == 0 ? a.x + token * a.x_stride : t.part == 1 ? a.k + token * a.k_stride
-                                                                                       : a.v + token * a.v_stride;
-            src += (int64_t)t.head * head_dim * kSize;
+        for (int b = 0; b < kTokens; ++b, src += beside * stride) {
+            if (b * beside + sub >= mine) break;
             lo[b] = load4<kIn, kStream>(src + t.first * kSize);
             hi[b] = load4<kIn, kStream>(src + t.second * kSize);
         }
-        if (first_round) {
-            first_round = false;
-            for (uint32_t j = tid; j < mine * (uint32_t)a.n_pairs; j += kThreads) {
-                const uint32_t t = a.by_pairs.div(j), i = j - t * a.by_pairs.d;
-                const RopePair pair = a.pairs[i];
-                const int32_t p = a.positions[pair.axis * a.position_stride + token0 + t];
-                float s, c;
-                sin_cos((uint64_t)(int64_t)p * pair.step, &s, &c);
-                sines[t * kMaxPairs + i] = (a.inverse ? -s : s) * a.scale;
-                cosines[t * kMaxPairs + i] = c * a.scale;
-            }
-            if (a.slots && tid < mine) {
-                const int32_t s = a.slots[token0 + tid];
-                int64_t place = -1;
-                if (s >= 0 && (uint32_t)s < a.cache.slots) {
-                    const uint32_t page = a.cache.page.div((uint32_t)s);
-                    place = (int64_t)page * a.cache.page_stride +
-                            (int64_t)((uint32_t)s - page * a.cache.page.d) * a.cache.token_stride;
-                }
-                places[tid] = place;
-            }
-            __syncthreads();
+    }
+    for (uint32_t j = tid; j < mine * (uint32_t)a.n_pairs; j += kThreads) {
+        const uint32_t token = a.by_pairs.div(j), i = j - token * a.by_pairs.d;
+        const RopePair pair = a.pairs[i];
+        const int32_t p = a.positions[pair.axis * a.position_stride + token0 + token];
+        float s, c;
+        sin_cos((uint64_t)(int64_t)p * pair.step, &s, &c);
+        sines[j] = (a.inverse ? -s : s) * a.scale;
+        cosines[j] = c * a.scale;
+    }
+    if (a.slots && tid < mine) {
+        const int32_t s = a.slots[token0 + tid];
+        int64_t place = -1;
+        if (s >= 0 && (uint32_t)s < a.cache.slots) {
+            const uint32_t page = a.cache.page.div((uint32_t)s);
+            place = (int64_t)page * a.cache.page_stride + (int64_t)((uint32_t)s - page * a.cache.page.d) * a.cache.token_stride;
         }
+        places[tid] = place;
+    }
+    __syncthreads();
+    if (!active) return;
+    uint8_t* y_row = a.y + (token0 + sub) * a.y_stride + (int64_t)t.head * head_dim * y_size;
+    uint8_t* c_row = (t.part == 1 ? a.cache.k : a.cache.v) + t.head * a.cache.head_stride;
+    const float over = t.part == 1 ? a.k_over : a.v_over;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            if (i0 + (uint32_t)b * step + tid >= total) continue;
-            const Item t = items[b];
-            float4 x = lo[b], y = hi[b];
-            if (t.pair >= 0) {
-                const float4 s = *reinterpret_cast<const float4*>(&sines[t.token * kMaxPairs + t.pair]);
-                const float4 c = *reinterpret_cast<const float4*>(&cosines[t.token * kMaxPairs + t.pair]);
-                if (a.adjacent) {
-                    const float4 p = x, q = y;
-                    x = make_float4(p.x * c.x - p.y * s.x, p.x * s.x + p.y * c.x, p.z * c.y - p.w * s.y,
-                                    p.z * s.y + p.w * c.y);
-                    y = make_float4(q.x * c.z - q.y * s.z, q.x * s.z + q.y * c.z, q.z * c.w - q.w * s.w,
-                                    q.z * s.w + q.w * c.w);
-                } else {
-                    const float4 p = x, q = y;
-                    x = make_float4(p.x * c.x - q.x * s.x, p.y * c.y - q.y * s.y, p.z * c.z - q.z * s.z,
-                                    p.w * c.w - q.w * s.w);
-                    y = make_float4(p.x * s.x + q.x * c.x, p.y * s.y + q.y * c.y, p.z * s.z + q.z * c.z,
-                                    p.w * s.w + q.w * c.w);
-                }
+    for (int b = 0; b < kTokens; ++b, y_row += beside * a.y_stride) {
+        const uint32_t token = b * beside + sub;
+        if (token >= mine) break;
+        float4 x = lo[b], y = hi[b];
+        if (t.pair >= 0) {
+            const uint32_t at = token * (uint32_t)a.n_pairs + (uint32_t)t.pair;
+            const float4 s = *reinterpret_cast<const float4*>(sines + at), c = *reinterpret_cast<const float4*>(cosines + at);
+            const float4 p = x, q = y;
+            if (a.adjacent) {
+                x = make_float4(p.x * c.x - p.y * s.x, p.x * s.x + p.y * c.x, p.z * c.y - p.w * s.y, p.z * s.y + p.w * c.y);
+                y = make_float4(q.x * c.z - q.y * s.z, q.x * s.z + q.y * c.z, q.z * c.w - q.w * s.w, q.z * s.w + q.w * c.w);
+            } else {
+                x = make_float4(p.x * c.x - q.x * s.x, p.y * c.y - q.y * s.y, p.z * c.z - q.z * s.z, p.w * c.w - q.w * s.w);
+                y = make_float4(p.x * s.x + q.x * c.x, p.y * s.y + q.y * c.y, p.z * s.z + q.z * c.z, p.w * s.w + q.w * c.w);
             }
-            if (t.part == 0) {
-                uint8_t* dst = a.y + (token0 + t.token) * a.y_stride + (int64_t)t.head * head_dim * y_size;
-                store4<kStream>(dst + t.first * y_size, a.y_dtype, x);
-                store4<kStream>(dst + t.second * y_size, a.y_dtype, y);
-            } else if (places[t.token] >= 0) {
-                uint8_t* dst = (t.part == 1 ? a.cache.k : a.cache.v) + places[t.token] + t.head * a.cache.head_stride;
-                const float over = t.part == 1 ? a.k_over : a.v_over;
-                store4<false>(dst + t.first * c_size, a.cache_dtype, scaled(x, over));
-                store4<false>(dst + t.second * c_size, a.cache_dtype, scaled(y, over));
-            }
+        }
+        if (t.part == 0) {
+            store4<kStream>(y_row + t.first * y_size, a.y_dtype, x);
+            store4<kStream>(y_row + t.second * y_size, a.y_dtype, y);
+        } else if (places[token] >= 0) {
+            uint8_t* dst = c_row + places[token];
+            store4<false>(dst + t.first * c_size, a.cache_dtype, scaled(x, over));
+            store4<false>(dst + t.second * c_size, a.cache_dtype, scaled(y, over));
         }
     }
 }
@@ -225,34 +219,34 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a, int head_dim
 }  // namespace
 
 template <int kIn>
-static void launch_type(const RopeArgs& a, int head_dim, dim3 grid, int wg_tokens, bool stream, hipStream_t s) {
+static void launch_type(const RopeArgs& a, int head_dim, dim3 grid, uint32_t beside, bool stream, hipStream_t s) {
+    const size_t lds = 2 * 4 * (size_t)beside * a.n_pairs;
     if (stream)
-        hipLaunchKernelGGL((rope_kernel<kIn, true>), grid, dim3(kThreads), 0, s, a, head_dim, wg_tokens, grid.y * kThreads);
+        hipLaunchKernelGGL((rope_kernel<kIn, true, batch_of(kIn)>), grid, dim3(kThreads), batch_of(kIn) * lds, s, a, head_dim,
+                           beside);
     else
-        hipLaunchKernelGGL((rope_kernel<kIn, false>), grid, dim3(kThreads), 0, s, a, head_dim, wg_tokens, grid.y * kThreads);
+        hipLaunchKernelGGL((rope_kernel<kIn, false, 1>), grid, dim3(kThreads), lds, s, a, head_dim, beside);
 }
 
 hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s) {
-    // Up to 2048 workgroups of one item a thread (single tokens: least latency), else
-    // workgroups of about kBatch items a thread that stream.  MI355X, fp32 to bf16, plain
-    // and four items against streaming and three: 16128 tokens of 16 heads 45.7 and 38.0 us
-    // (5.2 TB/s), 4096 of 64 + 16 heads into an e4m3 cache 55.3 and 46.4, 8191 of 96 heads
-    // into an fp16 cache 120 both (5.0 TB/s).
-    const int64_t items = a.per_token.d;
-    int64_t wg_tokens = 1, split = (items + kThreads - 1) / kThreads;
-    const bool stream = a.tokens * split > 2048;
-    if (stream) {
-        wg_tokens = kBatch * kThreads / items;
-        wg_tokens = wg_tokens < 1 ? 1 : wg_tokens > kMaxTokens ? kMaxTokens : wg_tokens;
-        split = (items * wg_tokens + kBatch * kThreads - 1) / (kBatch * kThreads);
-    }
-    const dim3 grid((unsigned)((a.tokens + wg_tokens - 1) / wg_tokens), (unsigned)split);
+    // Up to 2048 workgroups of one token (or of those side by side) a thread, for the least
+    // latency; else batch_of tokens a thread, past the caches.  MI355X, us, the latter with 1,
+    // 2, 3 and 4 tokens: 16128 tokens of 16 heads, fp32 to bf16 38.4, 35.1, 35.8, 34.8, from
+    // bf16 29.1, 26.6, 24.3, 23.2; 8191 of 96 heads into an fp16 cache 118.3, 113.8, 113.9,
+    // 117.0 (the cache's lines past the caches too: 127); 128 threads 119, 512 112.
+    const uint32_t items = a.per_token.d, slices = (items + kThreads - 1) / kThreads;
+    uint32_t beside = 1;
+    if (items < kThreads) beside = kThreads / items < kMostBeside ? kThreads / items : kMostBeside;
+    const bool stream = (a.tokens + beside - 1) / beside * slices > 2048;
+    const int64_t tokens = stream ? (int64_t)batch_of(a.x_dtype) * beside : beside;
+    const unsigned groups = (unsigned)((a.tokens + tokens - 1) / tokens);
+    const dim3 grid(groups, slices);
     if (a.x_dtype == OPENMINI_ATTN_F32)
-        launch_type<OPENMINI_ATTN_F32>(a, head_dim, grid, (int)wg_tokens, stream, s);
+        launch_type<OPENMINI_ATTN_F32>(a, head_dim, grid, beside, stream, s);
     else if (a.x_dtype == OPENMINI_ATTN_F16)
-        launch_type<OPENMINI_ATTN_F16>(a, head_dim, grid, (int)wg_tokens, stream, s);
+        launch_type<OPENMINI_ATTN_F16>(a, head_dim, grid, beside, stream, s);
     else
-        launch_type<OPENMINI_ATTN_BF16>(a, head_dim, grid, (int)wg_tokens, stream, s);
+        launch_type<OPENMINI_ATTN_BF16>(a, head_dim, grid, beside, stream, s);
     return hipGetLastError();
 }
 
