@@ -434,6 +434,8 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     a.part_acc = reinterpret_cast<float*>(work + w.acc_at);
     a.by_row = p->rows <= (int64_t)shares;
     const int64_t keys = max_len < (int64_t)a.window ? max_len : (int64_t)a.window, tile = 32 * attn::decode_subtiles(cache->head_dim, f8);
+    a.stream = head_tiles == 1 && p->rows <= p->requests &&
+               attn::decode_streams(c, cache->kv_heads, cache->head_dim, f8, p->rows * keys);
     // a window's first tile need not begin with it
     a.whole = attn::decode_whole((keys + tile - 1) / tile + (keys < max_len), p->rows * cache->kv_heads * head_tiles);
     const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -45,6 +45,7 @@ using qmm::bf16x8;
 using qmm::f16x8;
 using qmm::f32x4;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct BF16 {
     static constexpr int kExactParts = 3;  // that hold an fp32 probability, 8 bits each
@@ -81,20 +82,26 @@ struct F16 {
     }
 };
 
-template <int kBytes>
+// kStream: loads that leave the caches to others (decode_streams).
+template <bool kStream, class V>
+__device__ __forceinline__ V load_as(const uint8_t* p) {
+    if constexpr (kStream) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    return *reinterpret_cast<const V*>(p);
+}
+template <int kBytes, bool kStream>
 __device__ __forceinline__ void load(const uint8_t* p, uint32_t* d) {
     if constexpr (kBytes == 16) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+        const u32x4 v = load_as<kStream, u32x4>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[i] = v[i];
     } else if constexpr (kBytes == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        d[0] = v.x;
-        d[1] = v.y;
+        const u32x2 v = load_as<kStream, u32x2>(p);
+        d[0] = v[0];
+        d[1] = v[1];
     } else if constexpr (kBytes == 4) {
-        d[0] = *reinterpret_cast<const uint32_t*>(p);
+        d[0] = load_as<kStream, uint32_t>(p);
     } else {
-        d[0] = *reinterpret_cast<const uint16_t*>(p);
+        d[0] = load_as<kStream, uint16_t>(p);
     }
 }
 
@@ -250,7 +257,7 @@ __device__ __forceinline__ bool find_share(const First& a, uint32_t p, Share& ou
 // they are joined in LDS: one launch, and no wave that looks for its share, but as many CUs
 // as there are rows and units, and a CU reads about 50 GB/s.  For short rows (decode_whole);
 // the last tile of a wave is most of its work then, so no loads of a next one are behind it.
-template <int D, class T, bool F8, int kSub, int W, bool kWide, bool kWhole>
+template <int D, class T, bool F8, int kSub, int W, bool kWide, bool kWhole, bool kStream>
 __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(const int32_t* lens, const int32_t* rows,
                                                                                  uint32_t n_rows, uint32_t requests,
                                                                                  uint32_t max_len, uint32_t window,
@@ -347,6 +354,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     auto group_at = [&](const Tile& t, int sub, int grp) -> int32_t {
         return min(max((int32_t)(t.no * kKeys) + 32 * sub + 8 * grp, t.first_group), t.last_group);
     };
+    // Eight keys of a tile, for all its groups.
+    auto one_group = [&](const Row& r, uint32_t no) {
+        Tile t = tile_of(r, no);
+        t.first_group = t.last_group = min(max((int32_t)(no * kKeys), t.first_group), t.last_group);
+        return t;
+    };
     using Place = std::conditional_t<kWide, uint64_t, uint32_t>;
     struct Pages {  // of a tile's K and V groups, and the groups' places in them
         int32_t k[kSub], v[kSub];
@@ -381,11 +394,11 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                 const uint8_t* p = k_base + 4 * s * a.cache.token_stride;
                 if constexpr (F8) {
 #pragma unroll
-                    for (int c = 0; c < kSteps / 2; ++c) load<16>(p + at + c * 64, &kraw[u][s][4 * c]);
-                    if constexpr (kSteps & 1) load<8>(p + (at - g * 8) + (kSteps - 1) * 32, &kraw[u][s][2 * (kSteps - 1)]);
+                    for (int c = 0; c < kSteps / 2; ++c) load<16, kStream>(p + at + c * 64, &kraw[u][s][4 * c]);
+                    if constexpr (kSteps & 1) load<8, kStream>(p + (at - g * 8) + (kSteps - 1) * 32, &kraw[u][s][2 * (kSteps - 1)]);
                 } else {
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st) load<16>(p + at + st * 64, &kraw[u][s][4 * st]);
+                    for (int st = 0; st < kSteps; ++st) load<16, kStream>(p + at + st * 64, &kraw[u][s][4 * st]);
                 }
             }
         }
@@ -397,10 +410,10 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         for (int j = 0; j < 8; ++j) {
             const uint8_t* p = v_base + j * a.cache.token_stride;
 #pragma unroll
-            for (int c = 0; c < kFull; ++c) load<8 * kEl>(p + at128 + c * 128 * kEl, &vraw[u][j][c * 2 * kEl]);
-            if constexpr (kHas64) load<4 * kEl>(p + at64 + kFull * 128 * kEl, &vraw[u][j][kFull * 2 * kEl]);
+            for (int c = 0; c < kFull; ++c) load<8 * kEl, kStream>(p + at128 + c * 128 * kEl, &vraw[u][j][c * 2 * kEl]);
+            if constexpr (kHas64) load<4 * kEl, kStream>(p + at64 + kFull * 128 * kEl, &vraw[u][j][kFull * 2 * kEl]);
             if constexpr (kHas32)
-                load<2 * kEl>(p + at32 + (kFull * 128 + kHas64 * 64) * kEl, &vraw[u][j][kFull * 2 * kEl + kHas64 * kEl]);
+                load<2 * kEl, kStream>(p + at32 + (kFull * 128 + kHas64 * 64) * kEl, &vraw[u][j][kFull * 2 * kEl + kHas64 * kEl]);
         }
     };
 
@@ -545,7 +558,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         uint32_t tile = cur.tile0;
         Row following = cur;
         if (!loaded && tile < cur.tile1) {
-            const Tile first = tile_of(cur, tile), second = tile_of(cur, min(tile + 1, cur.tile1 - 1));
+            const Tile first = tile_of(cur, tile), second = tile + 1 < cur.tile1 ? tile_of(cur, tile + 1) : one_group(cur, tile);
             now = pages_of(first);
             load_q(cur.row);
             then = pages_of(second);
@@ -578,18 +591,19 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                 then = later;
             }
             // The row's last two tiles, before which come the next row's first.  At the share's
-            // end (or before a row without keys) the next tile is the present one again: loads
-            // without a branch around them, so that the wait for the present values need not
-            // cover them.
+            // end (or before a row without keys) it is eight keys of the present one again, for
+            // the whole tile: loads without a branch around them, so that the wait for the present
+            // values need not cover them.
             if (more) following = row_of(cur.row + 1, cur.end, cur.end, said);
             loaded = tile < cur.tile1 && more && following.tile0 < following.tile1;
             for (; tile < cur.tile1; ++tile) {
                 const bool last = tile + 1 == cur.tile1, cross = last && loaded;
                 scores();
-                const Tile next = cross ? tile_of(following, following.tile0) : tile_of(cur, last ? tile : tile + 1);
-                const Tile after = loaded ? tile_of(following, min(following.tile0 + (last ? 1u : 0u), following.tile1 - 1)) : next;
+                const Tile after = loaded ? tile_of(following, min(following.tile0 + (last ? 1u : 0u), following.tile1 - 1))
+                                          : one_group(cur, cur.tile1 - 1);
                 const Pages later = pages_of(after);
-                if (cross && cur.tile1 - cur.tile0 == 1) then = pages_of(next);  // no tile before looked them up
+                if (cross && cur.tile1 - cur.tile0 == 1)  // no tile before looked them up
+                    then = pages_of(tile_of(following, following.tile0));
                 load_k(then);
                 if (cross) load_q(following.row);
                 outputs(cur, tile, std::true_type{});
@@ -717,12 +731,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     }
 }
 
-template <int D, class T, bool F8, bool kWide, bool kWhole>
+template <int D, class T, bool F8, bool kWide, bool kWhole, bool kStream>
 hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
     constexpr int W = kWhole && !(D == 256 && !F8) ? 2 * kDecodeWaves : kDecodeWaves, kSub = decode_subtiles(D, F8);
     const uint64_t units = (uint64_t)a.kv_heads * a.head_tiles;
     const uint64_t all = kWhole ? a.n_rows * units : (a.launch_shares * units + W - 1) / W, wgs = (all + 7) / 8 * 8;
-    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide, kWhole>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
+    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide, kWhole, kStream>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
                        a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift,
                        (uint32_t)(wgs / 8), a);
     return hipGetLastError();
@@ -730,8 +744,11 @@ hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
 
 template <int D, class T, bool F8>
 hipError_t launch_f8(const DecodeArgs& a, hipStream_t s) {
-    if (a.whole) return launch_one<D, T, F8, true, true>(a, s);
-    return a.wide ? launch_one<D, T, F8, true, false>(a, s) : launch_one<D, T, F8, false, false>(a, s);
+    if (a.whole) return launch_one<D, T, F8, true, true, false>(a, s);
+    if constexpr (D % 64 == 0)  // decode_streams takes no others
+        if (a.stream)
+            return a.wide ? launch_one<D, T, F8, true, false, true>(a, s) : launch_one<D, T, F8, false, false, true>(a, s);
+    return a.wide ? launch_one<D, T, F8, true, false, false>(a, s) : launch_one<D, T, F8, false, false, false>(a, s);
 }
 
 template <int D, class T>

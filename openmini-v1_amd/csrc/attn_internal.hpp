@@ -106,6 +106,23 @@ constexpr int kRound = 1024;
 // 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.
 inline bool decode_whole(int64_t most, int64_t pairs) { return pairs <= 512 && most <= (pairs < 64 ? 16 : 32); }
 
+// Whether a call reads keys and values past the caches (loads marked as not used again),
+// with `keys` of each key head at most: where these are 128 MiB or more, which the caches (256 MB, and a
+// step's weights between two calls) would not hold for the next, and where lines of 128
+// bytes are not shared by heads, whose waves read them each at its own time.  Nor where
+// several rows, or tiles of heads, read the same keys.  Measured, with and without (us): one
+// row of 131071 keys, 8 heads of 128, bf16 92.3 / 98.4; 128 rows of up to 12000, e4m3 248 /
+// 271; 16 of up to 4000 (196 MB) 40.4 / 42.6, of 2000 27.7 / 27.4; of heads of 64 in e4m3,
+// token after token of a head 68.7 / 74.1, head after head (64 bytes each) 96.0 / 85.0;
+// 32 heads of one key head 33.2 / 24.8.
+inline bool decode_streams(const Cache& c, int kv_heads, int head_dim, bool f8, int64_t keys) {
+    const int row_bytes = head_dim * (f8 ? 1 : 2);
+    const bool whole_lines = row_bytes % 128 == 0 ? c.token_stride % 128 == 0 : head_dim % 64 == 0 && c.token_stride == row_bytes;
+    const bool aligned = (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.head_stride | (uintptr_t)c.page_stride) & 127) == 0;
+    const int64_t most = keys < (int64_t)c.slots ? keys : (int64_t)c.slots;
+    return whole_lines && aligned && 2 * most * kv_heads * row_bytes >= 128 << 20;
+}
+
 // A row of several parts (parts > 1), in shares first_share on.
 struct Split {
     uint32_t row, first_share, parts;
@@ -135,7 +152,8 @@ struct DecodeArgs {
     float2* part_ml;  // [shares][2][q_heads]: maximum, sum
     Split* split;     // [shares]
     int32_t by_row;
-    int32_t whole;  // a row of a unit to a workgroup, and no join
+    int32_t whole;   // a row of a unit to a workgroup, and no join
+    int32_t stream;  // keys and values are read past the caches
 };
 
 // Shares of a call, at most.
