@@ -107,11 +107,11 @@ constexpr int kRound = 1024;
 inline bool decode_whole(int64_t most, int64_t pairs) { return pairs <= 512 && most <= (pairs < 64 ? 16 : 32); }
 
 // Whether a call reads keys and values past the caches (loads marked as not used again),
-// with `keys` of each key head at most: where these are 128 MiB or more, which the caches (256 MB, and a
-// step's weights between two calls) would not hold for the next, and where lines of 128
-// bytes are not shared by heads, whose waves read them each at its own time.  Nor where
+// with `keys` of each key head at most: where these are 128 MiB or more, which the caches (256
+// MB, and a step's weights between two calls) would not hold for the next, and where lines of
+// 128 bytes are not shared by heads, whose waves read them each at its own time.  Nor where
 // several rows, or tiles of heads, read the same keys.  Measured, with and without (us): one
-// row of 131071 keys, 8 heads of 128, bf16 92.3 / 98.4; 128 rows of up to 12000, e4m3 248 /
+// row of 131071 keys, 8 heads of 128, bf16 90.3 / 98.4; 128 rows of up to 12000, e4m3 245 /
 // 271; 16 of up to 4000 (196 MB) 40.4 / 42.6, of 2000 27.7 / 27.4; of heads of 64 in e4m3,
 // token after token of a head 68.7 / 74.1, head after head (64 bytes each) 96.0 / 85.0;
 // 32 heads of one key head 33.2 / 24.8.

@@ -6,7 +6,7 @@
 // dimensions, kDeep loads in flight, and the groups are joined in order.
 //
 // Bound by latency: a launch and two loads one after the other, of lines that other XCDs
-// wrote; 4 to 6 us (131071 keys of one row, 128 parts of 64 heads of 128: 6.0).  A launch of
+// wrote; 4 to 6 us (131071 keys of one row, 128 parts of 64 heads of 128: 5.6).  A launch of
 // its own and not the end of the first: there, waves that joined by pairs as they ended,
 // through device-scope stores and loads, took longer on every call (one row of 300 keys 13.2
 // against 9.3 us, of 131071 105 against 99.7, 64 rows in a window 33.8 against 30.8).
