@@ -93,8 +93,8 @@ constexpr int kHeadTile = 16;    // query heads a workgroup serves (the MFMA's c
 constexpr int kMaxHeads = 1024;  // query heads
 // Waves of a call, at most (one share each unless the units alone are more): one for each
 // SIMD.  Two or three raise the bytes in flight past what the memory needs, and then equal
-// shares end at different times (131071 keys, 8 heads of 128, bf16: the waves end between 73
-// and 104 us, the call takes 106 us instead of 99; 512 waves 117).
+// shares end at different times (131071 keys, 8 heads of 128, bf16: 2048 waves 103 us, 1536
+// 116, 1024 93).
 constexpr int kRound = 1024;
 
 // Whether workgroups take whole rows: `most` tiles in a row at most, by the table's columns
