@@ -183,7 +183,7 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
  *
  * Long rows are cut into parts that separate waves take, and a second launch joins a row's
  * parts in their order; where the tables and the window leave only short rows, a workgroup
- * takes a row and there is no second launch (so max_pages is best no more than the call's
+ * takes a row, or a wave several, and there is no second launch (so max_pages is best no more than the call's
  * longest row needs; table_stride is free).  How rows are cut depends on all lengths of the
  * call and on max_pages, so the last bits of a row may differ between calls with other rows
  * beside it; equal calls give equal bits.  d_work: openmini_attn_workspace_bytes bytes,

@@ -437,11 +437,15 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     a.stream = head_tiles == 1 && p->rows <= p->requests &&
                attn::decode_streams(c, cache->kv_heads, cache->head_dim, f8, p->rows * keys);
     // a window's first tile need not begin with it
-    a.whole = attn::decode_whole((keys + tile - 1) / tile + (keys < max_len), p->rows * cache->kv_heads * head_tiles);
+    const int64_t most = (keys + tile - 1) / tile + (keys < max_len), pairs = p->rows * cache->kv_heads * head_tiles;
+    a.whole = attn::decode_whole(most, pairs);
+    a.uncut = attn::decode_uncut(most, pairs);
+    if (a.uncut) a.launch_shares = p->rows < (int64_t)shares ? (uint32_t)p->rows : shares;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = p->q_dtype == OPENMINI_ATTN_BF16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)
                                                     : attn::launch_decode_f16(a, cache->head_dim, f8, s);
-    if (e == hipSuccess && !a.whole && a.launch_shares > 1) e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
+    if (e == hipSuccess && !a.whole && !a.uncut && a.launch_shares > 1)
+        e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
     return launched(e, "attention launch");
 }
 

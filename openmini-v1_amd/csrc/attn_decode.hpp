@@ -150,6 +150,7 @@ struct Span {
 struct First {
     const int32_t *lens, *rows;
     uint32_t n_rows, requests, max_len, window, shares;
+    uint32_t uncut;  // the shares are rows (decode_uncut)
 };
 
 // What the call says of a row, and the same by scalar loads (a uniform row; they are not
@@ -194,6 +195,12 @@ __device__ __forceinline__ bool find_share(const First& a, uint32_t p, Share& ou
         out.to = min(out.from + out.each, total);
         return out.from < total;
     };
+    if (a.uncut) {  // rows are its places
+        if (!place(a.n_rows)) return false;
+        out.row = out.row_at = out.from;
+        said = said_of_uniform(a, out.row);
+        return true;
+    }
     if (a.n_rows <= 64) {  // every wave by itself
         Said mine = {0, 0};
         Span s = {0, 0, 0};
@@ -263,8 +270,9 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                                                                                  uint32_t max_len, uint32_t window,
                                                                                  uint32_t shares, uint32_t units,
                                                                                  uint32_t units_m, uint32_t units_shift, uint32_t eighth,
+                                                                                 uint32_t uncut,
                                                                                  DecodeArgs a) {
-    const First f = {lens, rows, n_rows, requests, max_len, window, shares};
+    const First f = {lens, rows, n_rows, requests, max_len, window, shares, uncut};
     constexpr int kEl = F8 ? 1 : 2;           // bytes of a cache element
     constexpr uint32_t kKeys = 32 * kSub;     // keys of a tile, in kSub tiles of 32
     constexpr int kSteps = D / 32;            // MFMAs over head_dim of the first product
@@ -318,9 +326,9 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         Row r;
         r.row = row;
         r.at = at;
-        r.end = at + s.weight();
+        r.end = at + (f.uncut ? 1 : s.weight());
         r.tile0 = (uint32_t)s.lo / kKeys + (from - at);
-        r.tile1 = s.tiles ? (uint32_t)s.lo / kKeys + (min(r.end, share.to) - at) : r.tile0;
+        r.tile1 = f.uncut ? r.tile0 + s.tiles : s.tiles ? (uint32_t)s.lo / kKeys + (min(r.end, share.to) - at) : r.tile0;
         r.lo = s.lo;
         r.hi = s.hi;
         r.table = a.tables + (int64_t)said.request * a.table_stride;
@@ -738,7 +746,7 @@ hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
     const uint64_t all = kWhole ? a.n_rows * units : (a.launch_shares * units + W - 1) / W, wgs = (all + 7) / 8 * 8;
     hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide, kWhole, kStream>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
                        a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift,
-                       (uint32_t)(wgs / 8), a);
+                       (uint32_t)(wgs / 8), (uint32_t)a.uncut, a);
     return hipGetLastError();
 }
 

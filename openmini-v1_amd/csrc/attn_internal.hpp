@@ -104,7 +104,20 @@ constexpr int kRound = 1024;
 // 7.0 / 9.4, of 700 9.8 / 10.7, of 1000 12.5 / 10.9; 64 pairs of 1000 13.5 / 16.2, of 2000
 // 22.6 / 18.5; 256 of up to 4000, heads of 64, 46.8 / 36.4; 512 of 400 15.1 / 20.4; 1024 of
 // 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.
-inline bool decode_whole(int64_t most, int64_t pairs) { return pairs <= 512 && most <= (pairs < 64 ? 16 : 32); }
+inline bool decode_whole(int64_t most, int64_t pairs) {
+    return most == 1 ? pairs <= 256 : pairs <= 512 && most <= (pairs < 64 ? 16 : 32);
+}
+
+// Whether the shares are rows, as many to a wave as to any other whatever their lengths, so
+// that no row is cut and there is no join: more pairs than workgroups take whole, of so few
+// tiles that lengths do not differ by much.  Measured, uncut against shares of tiles (us):
+// 1024 pairs of half to all of 4 tiles, heads of 128, bf16 11.3 / 16.9, of a twentieth to all
+// 9.6 / 13.0; 2048 the same 20.8 / 27.7 and 15.1 / 17.1; of 8 tiles 39.2 / 43.1 and 23.5 / 23.7,
+// in heads of 256 77.3 / 81.4 and 63.9 / 46.7; 6000 of a twentieth to all of 4 tiles 40.3 / 39.9.
+// 264 of one tile against whole rows 5.3 / 5.8, 128 5.2 / 5.3.
+inline bool decode_uncut(int64_t most, int64_t pairs) {
+    return most == 1 ? pairs > 256 : pairs > 512 && most <= (pairs <= 4096 ? 4 : 2);
+}
 
 // Whether a call reads keys and values past the caches (loads marked as not used again),
 // with `keys` of each key head at most: where these are 128 MiB or more, which the caches (256
@@ -152,6 +165,7 @@ struct DecodeArgs {
     float2* part_ml;  // [shares][2][q_heads]: maximum, sum
     Split* split;     // [shares]
     int32_t by_row;
+    int32_t uncut;   // shares are rows, whatever their lengths, and there is no join
     int32_t whole;   // a row of a unit to a workgroup, and no join
     int32_t stream;  // keys and values are read past the caches
 };

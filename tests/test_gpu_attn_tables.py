@@ -113,3 +113,27 @@ def test_graph_replays_of_short_rows(qmm):
         got = do.download(np.uint32, (3, 8, 128)), dlse.download(np.float32, (3, 8))
         c.check(got)
         assert np.array_equal(c.run(qmm, attn=attn)[0], got[0])
+
+
+@pytest.mark.parametrize("R,kv,most", [(257, 1, 32), (130, 2, 31), (300, 2, 100), (513, 1, 128), (1030, 1, 60), (2100, 2, 64), (400, 4, 33)])
+@pytest.mark.parametrize("dim,c_t", [(128, BF16), (64, F8), (256, BF16)])
+def test_many_short_rows(qmm, R, kv, most, dim, c_t):
+    """Rows of a few tiles, more than workgroups take whole: empty ones, whole ones, one key."""
+    rng = np.random.default_rng(R + most)
+    lens = rng.integers(0, most + 1, R)
+    lens[rng.random(R) < 0.1] = 0
+    lens[0], lens[R // 2], lens[R - 1] = 1, most, 0
+    c = Case(qmm, [int(n) for n in lens], 4, kv, dim, BF16, c_t, seed=R)
+    c.check(c.run(qmm))
+
+
+def test_many_short_rows_of_requests_and_windows(qmm):
+    """The same for rows that share requests, lie outside them, or see a window."""
+    rng = np.random.default_rng(5)
+    reqs = [int(r) for r in rng.integers(-1, 4, 700)]
+    lens = [70, 3, 128, 40]
+    row_lens = [int(rng.integers(-2, (lens[r] if r >= 0 else 128) + 1)) for r in reqs]
+    c = Case(qmm, lens, 8, 1, 128, reqs=reqs, row_lens=row_lens, seed=6)
+    c.check(c.run(qmm))
+    c = Case(qmm, [int(n) for n in rng.integers(0, 900, 520)], 8, 1, 64, window=60, seed=7)
+    c.check(c.run(qmm))
