@@ -177,8 +177,9 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
  *
  * Types: q F16 or BF16 and the cache the same type, or F8_E4M3, which is converted to q's
  * (exactly); out q's type or F32.  Products are of 16-bit operands with 32-bit sums; the
- * probabilities enter the second product as the sum of two (F16) or three (BF16) 16-bit
- * parts, which hold 22 or 24 bits of them.  head_dim: 64, 96, 128, 192 or 256; page_size: a multiple
+ * probabilities enter the second product as the sum of three bf16 parts, which hold 24 bits of
+ * them, or on an F16 cache of fp16 parts, which hold 22 bits of them down to 2^-57 of a row's
+ * largest and all of them to 2^-79 of it.  head_dim: 64, 96, 128, 192 or 256; page_size: a multiple
  * of 8; q_heads: a multiple of kv_heads, at most 1024.
  *
  * Long rows are cut into parts that separate waves take, and a second launch joins a row's

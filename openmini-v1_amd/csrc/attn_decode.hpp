@@ -17,10 +17,13 @@
 // neighbouring lanes, whole) and transposes them in registers, two keys to a dword, one
 // byte permutation each; tile e of a chunk is then dimensions e, e + width, ...
 //
-// The probabilities enter the second product as the sum of two (fp16) or three (bf16) 16-bit
-// parts, together all of fp32 or nearly: their rounding to one bf16 would be 2^-9 of an fp32
-// output, to two 2^-18 (1.2e-6 measured, against 4e-7 for fp32 arithmetic throughout).
-// Sums, maxima and the joined parts are fp32.
+// The probabilities enter the second product as the sum of three bf16 or two fp16 parts (fp16
+// caches), together all of fp32 or nearly: their rounding to one bf16 would be 2^-9 of an fp32
+// output, to two 2^-18 (1.2e-6 measured, against 4e-7 for fp32 arithmetic throughout).  bf16 has
+// the range of fp32.  fp16 has a least unit of 2^-24, so there p is 2^15 at the maximum, and
+// where a tile has keys whose two parts hold less than 22 bits (p below 2^-17 of the largest: a
+// first key that draws most of the weight leaves the others there), what the two leave is
+// added too, as two parts 2^39 up.  Sums, maxima and the joined parts are fp32.
 //
 // Bound by memory: one operation a byte (e4m3: two) for each query head of a key head.  A tile
 // of 32, 64 or 128 keys is about 16 KB; the loads of the next tile are issued as soon as the
@@ -49,6 +52,9 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct BF16 {
     static constexpr int kExactParts = 3;  // that hold an fp32 probability, 8 bits each
+    static constexpr bool kNarrow = false;  // parts have the range of fp32
+    // The base m of p = 2^(s - m) for a largest s.
+    static __device__ __forceinline__ float base_of(float top) { return top; }
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                        0, 0);
@@ -66,7 +72,11 @@ struct BF16 {
 };
 
 struct F16 {
-    static constexpr int kExactParts = 2;  // 11 bits each
+    static constexpr int kExactParts = 2;  // 11 bits each, for p from 2^-2 on
+    static constexpr bool kNarrow = true;
+    // p of at most 2^15, below the largest fp16.  From 2^23 on the difference need not be
+    // exact and could round to 2^16: there p is at most 1, and scores are 1 apart at least.
+    static __device__ __forceinline__ float base_of(float top) { return fabsf(top) < 8388608.0f ? top - 15.0f : top; }
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                       0);
@@ -130,10 +140,6 @@ __device__ __forceinline__ float column_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// log(sum of exponentials) from a maximum in powers of two and the sum above it.
-__device__ __forceinline__ float log_sum(float m, float l) {
-    return l == 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
-}
 
 // 2^(a - m) for a maximum m that is -inf where nothing is seen.
 __device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -273,6 +279,7 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                                                                                  uint32_t uncut,
                                                                                  DecodeArgs a) {
     const First f = {lens, rows, n_rows, requests, max_len, window, shares, uncut};
+    using P = std::conditional_t<F8, BF16, T>;  // of the second product's parts: both hold e4m3
     constexpr int kEl = F8 ? 1 : 2;           // bytes of a cache element
     constexpr uint32_t kKeys = 32 * kSub;     // keys of a tile, in kSub tiles of 32
     constexpr int kSteps = D / 32;            // MFMAs over head_dim of the first product
@@ -452,13 +459,16 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     auto outputs = [&](const Row& cur, uint32_t tile, auto next_tag) {
         // keys outside the row's or on no page of the cache: only a row's first and
         // last tiles, and broken tables, have them
-        float x[kSub][8];
+        float x[kSub][8], least = INFINITY;  // least before the mask: a tile's edge is not low
         const int32_t key0 = (int32_t)(tile * kKeys) + 8 * g;
         bool whole = key0 >= cur.lo && key0 + (int32_t)kKeys - 24 <= cur.hi;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[u][j] = sc[u][j / 4][j % 4] * a.scale;
+            for (int j = 0; j < 8; ++j) {
+                x[u][j] = sc[u][j / 4][j % 4] * a.scale;
+                if constexpr (P::kNarrow) least = fminf(least, x[u][j]);
+            }
             whole = whole && (uint32_t)now.v[u] < a.cache.n_pages;
         }
         if (!__all(whole)) {
@@ -478,75 +488,105 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         for (int u = 0; u < kSub; ++u)
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, x[u][j]);
-        top = column_max(top);
-        if (__any(top > m)) {
-            const float to = fmaxf(m, top);
-            const float by = exp2_of(m - above(to));
+        const float lift = P::base_of(column_max(top)), to = fmaxf(m, lift), base = above(to);
+        constexpr float kUp = 549755813888.0f;  // 2^39
+        bool low = false;
+        if constexpr (P::kNarrow) low = __any(least < base - 2.0f);
+        if (low || __any(lift > m)) {
+            float by = exp2_of(m - base);
             m = to;
             l *= by;
+            if (low) by *= kUp;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) acc[i] *= by;
         }
-        const float base = above(m);
         // second product, p as the sum of kParts 16-bit parts
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            constexpr int kParts = T::kExactParts;
+            constexpr int kParts = P::kExactParts;
             u32x4 pf[kParts];
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
-                l += r0 + r1;
+            auto split = [&](float r0, float r1, int j) {
 #pragma unroll
                 for (int k = 0; k < kParts; ++k) {
-                    const uint32_t h = T::pair(r0, r1);
+                    const uint32_t h = P::pair(r0, r1);
                     pf[k][j / 2] = h;
-                    r0 -= T::low(h);
-                    r1 -= T::high(h);
+                    r0 -= P::low(h);
+                    r1 -= P::high(h);
                 }
-            }
-            auto add = [&](int t, u32x4 vf) {
-#pragma unroll
-                for (int k = 0; k < kParts; ++k) acc[t] = T::mfma(vf, pf[k], acc[t]);
+                return make_float2(r0, r1);
             };
-            auto chunk = [&](int t0, int word0, auto width_tag) {
-                constexpr int kWidth = decltype(width_tag)::value;
-                if constexpr (F8) {
+            // a low tile's first time round: what the parts leave of p < 2^-2, at most 2^-25, is
+            // added to the accumulators 2^39 up.  All tiles low against none: 131071 keys of one
+            // row 90.4 / 90.3 us, 64 rows of heads of 64 31.0 / 29.9, one row of 300 keys 8.2 / 7.4.
+            for (bool rest = low;; rest = false) {
+                if (rest) {
 #pragma unroll
-                    for (int w = 0; w < (kWidth + 3) / 4; ++w) {
-                        u32x4 f[4];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const uint32_t v0 = vraw[u][2 * q][word0 + w], v1 = vraw[u][2 * q + 1][word0 + w];
-                            const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
-                            f[0][q] = T::template from_f8<false>(lo);
-                            f[1][q] = T::template from_f8<true>(lo);
-                            if constexpr (kWidth >= 4) {
-                                const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
-                                f[2][q] = T::template from_f8<false>(hi);
-                                f[3][q] = T::template from_f8<true>(hi);
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < (kWidth < 4 ? kWidth : 4); ++e) add(t0 + 4 * w + e, f[e]);
+                    for (int j = 0; j < 8; j += 2) {
+                        const float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
+                        const float2 r = split(r0, r1, j);
+                        split(r0 < 0.25f ? r.x * kUp : 0.0f, r1 < 0.25f ? r.y * kUp : 0.0f, j);
                     }
+                    if (u > 0)
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) acc[t] *= kUp;
                 } else {
 #pragma unroll
-                    for (int e = 0; e < kWidth; ++e) {
-                        u32x4 f;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            f[q] = __builtin_amdgcn_perm(vraw[u][2 * q + 1][word0 + e / 2], vraw[u][2 * q][word0 + e / 2],
-                                                         e & 1 ? 0x07060302u : 0x05040100u);
-                        add(t0 + e, f);
+                    for (int j = 0; j < 8; j += 2) {
+                        const float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
+                        l += r0 + r1;
+                        split(r0, r1, j);
                     }
                 }
-            };
+                // a zero that is not known to be one: else V's fragments are made before the loop
+                // and kept (up to 60 registers)
+                uint32_t zero = 0;
+                if constexpr (P::kNarrow) asm volatile("" : "+s"(zero));
+                auto add = [&](int t, u32x4 vf) {
 #pragma unroll
-            for (int c = 0; c < kFull; ++c) chunk(8 * c, c * 2 * kEl, std::integral_constant<int, 8>{});
-            if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
-            if constexpr (kHas32)
-                chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
+                    for (int k = 0; k < kParts; ++k) acc[t] = P::mfma(vf, pf[k], acc[t]);
+                };
+                auto chunk = [&](int t0, int word0, auto width_tag) {
+                    constexpr int kWidth = decltype(width_tag)::value;
+                    if constexpr (F8) {
+#pragma unroll
+                        for (int w = 0; w < (kWidth + 3) / 4; ++w) {
+                            u32x4 f[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const uint32_t v0 = vraw[u][2 * q][word0 + w], v1 = vraw[u][2 * q + 1][word0 + w];
+                                const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
+                                f[0][q] = P::template from_f8<false>(lo);
+                                f[1][q] = P::template from_f8<true>(lo);
+                                if constexpr (kWidth >= 4) {
+                                    const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
+                                    f[2][q] = P::template from_f8<false>(hi);
+                                    f[3][q] = P::template from_f8<true>(hi);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < (kWidth < 4 ? kWidth : 4); ++e) add(t0 + 4 * w + e, f[e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kWidth; ++e) {
+                            u32x4 f;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                f[q] = __builtin_amdgcn_perm(vraw[u][2 * q + 1][word0 + e / 2], vraw[u][2 * q][word0 + e / 2],
+                                                             (e & 1 ? 0x07060302u : 0x05040100u) + zero);
+                            add(t0 + e, f);
+                        }
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < kFull; ++c) chunk(8 * c, c * 2 * kEl, std::integral_constant<int, 8>{});
+                if constexpr (kHas64) chunk(8 * kFull, kFull * 2 * kEl, std::integral_constant<int, 4>{});
+                if constexpr (kHas32)
+                    chunk(8 * kFull + 4 * kHas64, kFull * 2 * kEl + kHas64 * kEl, std::integral_constant<int, 2>{});
+                if (!rest) break;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) acc[t] *= 1.0f / kUp;
+            }
             // the next tile's, into the registers that are free
             if constexpr (decltype(next_tag)::value) load_v(then, u);
         }

@@ -170,6 +170,13 @@ struct DecodeArgs {
     int32_t stream;  // keys and values are read past the caches
 };
 
+// log(sum of exponentials) from a base in powers of two and the sum above it, whose exponent
+// joins the base first (fp16's sums are 2^15 up: the two nearly cancel).
+__device__ __forceinline__ float log_sum(float m, float l) {
+    const float e = (float)(__builtin_amdgcn_frexp_expf(l) - 1);
+    return l == 0 ? -INFINITY : (m + e + __builtin_amdgcn_logf(2.0f * __builtin_amdgcn_frexp_mantf(l))) * 0.693147180559945309f;
+}
+
 // Shares of a call, at most.
 uint32_t decode_shares(int kv_heads, int head_tiles);
 

@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Split* __restrict_
         *reinterpret_cast<v4*>(to + at * 2) = v4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
     }
     if (lse && d == 0)
-        lse[(int64_t)row.row * q_heads + head] = j.l == 0 ? -INFINITY : (j.m + __builtin_amdgcn_logf(j.l)) * 0.693147180559945309f;
+        lse[(int64_t)row.row * q_heads + head] = log_sum(j.m, j.l);
 }
 
 }  // namespace
