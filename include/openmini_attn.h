@@ -77,7 +77,8 @@ typedef struct {
  *   d_row_lens[j]           position + 1, the keys that a causal query of it sees (refused: 0)
  *   d_counts[4]             tokens, pages taken, requests refused, the next *d_head
  * A step of more than max_tokens tokens keeps its first max_tokens (counts[0] tells).  No
- * output may be one of the inputs.  1 <= requests <= 4096. */
+ * output may share memory with an input: d_head is not &d_counts[3] of the same call (copy it
+ * on the stream, or let the steps take turns with two counts).  1 <= requests <= 4096. */
 typedef struct {
     const int32_t* d_cached;
     const int32_t* d_new;

@@ -68,6 +68,16 @@ int check_stride(const char* what, int64_t v, int64_t least, int size) {
     return OPENMINI_QMM_OK;
 }
 
+// Whether `count` elements of 4 bytes from p on share memory with an array of rows of `row`
+// elements, `stride` from one to the next, from q on.
+bool shares_memory(const void* p, int64_t count, const void* q, int64_t rows, int64_t row, int64_t stride) {
+    if (!p || count <= 0) return false;
+    const int64_t from = ((int64_t)(uintptr_t)p - (int64_t)(uintptr_t)q) / 4, to = from + count;  // both 4-byte aligned
+    if (to <= 0 || from >= (rows - 1) * stride + row) return false;
+    const int64_t r = from < 0 ? 0 : from / stride;  // the row that begins at `from` or before it
+    return from < r * stride + row || (r + 1 < rows && to > (r + 1) * stride);
+}
+
 bool dense_type(int t) { return t == OPENMINI_ATTN_F32 || t == OPENMINI_ATTN_F16 || t == OPENMINI_ATTN_BF16; }
 bool half_type(int t) { return t == OPENMINI_ATTN_F16 || t == OPENMINI_ATTN_BF16; }
 int size_of(int t) { return t == OPENMINI_ATTN_F32 ? 4 : t == OPENMINI_ATTN_F8_E4M3 ? 1 : 2; }
@@ -202,11 +212,23 @@ int openmini_kv_plan(const openmini_kv_plan_args_t* p, void* stream) {
     for (const auto& n : need) TRY(check_pointer(n.name, n.p, 4));
     if (p->n_free || p->d_free) TRY(check_pointer("d_free", p->d_free, 4));
     if (p->d_head) TRY(check_pointer("d_head", p->d_head, 4));
-    const void* in[] = {p->d_cached, p->d_new, p->d_free, p->d_head};
-    const void* out[] = {p->d_tables, p->d_starts, p->d_lens, p->d_rows, p->d_positions, p->d_slots, p->d_row_lens, p->d_counts};
-    for (const void* i : in)
-        for (const void* o : out)
-            if (i && i == o) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "an output of the plan is one of its inputs");
+    // Every workgroup reads the inputs for itself, at its own time.
+    const struct {
+        const char* name;
+        const void* p;
+        int64_t count;
+    } in[] = {{"d_cached", p->d_cached, p->requests}, {"d_new", p->d_new, p->requests}, {"d_free", p->d_free, p->n_free},
+              {"d_head", p->d_head, 1}},
+      out[] = {{"d_starts", p->d_starts, p->requests + 1}, {"d_lens", p->d_lens, p->requests}, {"d_rows", p->d_rows, p->max_tokens},
+               {"d_positions", p->d_positions, p->max_tokens}, {"d_slots", p->d_slots, p->max_tokens},
+               {"d_row_lens", p->d_row_lens, p->max_tokens}, {"d_counts", p->d_counts, 4}};
+    for (const auto& i : in) {
+        const char* with = shares_memory(i.p, i.count, p->d_tables, p->requests, p->max_pages, p->table_stride) ? "d_tables" : nullptr;
+        for (const auto& o : out)
+            if (shares_memory(i.p, i.count, o.p, 1, o.count, o.count)) with = o.name;
+        if (with)
+            return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "an output of the plan is one of its inputs: %s and %s share memory", i.name, with);
+    }
     TRY(qmm::current_device(nullptr));
     attn::PlanArgs a;
     a.cached = p->d_cached;

@@ -110,6 +110,29 @@ def test_plan_refusals(kw, word):
     _refused(_native.lib().openmini_kv_plan(_plan_args(**kw), None), BAD, word)
 
 
+@pytest.mark.parametrize("kw,word", [
+    (dict(d_head=11 * P + 12), "d_head and d_counts"), (dict(d_head=6 * P + 4), "d_head and d_lens"),
+    (dict(d_cached=5 * P + 8), "d_cached and d_starts"), (dict(d_cached=5 * P - 4), "d_cached and d_starts"),
+    (dict(d_new=10 * P + 36), "d_new and d_row_lens"), (dict(d_free=9 * P - 12), "d_free and d_slots"),
+    (dict(d_free=4 * P + 60), "d_free and d_tables"), (dict(d_head=4 * P + 4 * 9, table_stride=9), "d_head and d_tables"),
+    (dict(d_free=4 * P + 4 * 8, table_stride=9), "d_free and d_tables")])
+def test_plan_refuses_overlaps(kw, word):
+    """Any element of an output that is one of an input's, not the first alone."""
+    _refused(_native.lib().openmini_kv_plan(_plan_args(**kw), None), BAD, word)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(d_head=11 * P + 16), dict(d_head=11 * P - 4), dict(d_head=4 * P + 4 * 8, table_stride=9), dict(d_cached=5 * P + 12),
+    dict(d_new=4 * P + 64), dict(d_free=9 * P, n_free=0), dict(d_head=4 * P + 4 * 17, table_stride=9), dict(d_head=None)])
+def test_plan_takes_neighbours(kw):
+    """Arrays beside each other, a word in the gap after a row of the tables, no list at all: what
+    stops the call is that this machine has no GPU."""
+    if _native.lib().openmini_qmm_is_available():
+        pytest.skip("the pointers are not memory")
+    rc = _native.lib().openmini_kv_plan(_plan_args(**kw), None)
+    assert rc == _native.ERR_HIP, (rc, _native.last_error())
+
+
 def test_null_arguments():
     L = _native.lib()
     _refused(L.openmini_kv_plan(None, None), BAD, "null arguments")
