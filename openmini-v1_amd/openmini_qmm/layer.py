@@ -195,11 +195,22 @@ class CachedAttention:
         self.weights, self.rope, self.cache = weights, rope, cache
         self.q_heads, self.max_tokens, self.q_dtype = int(q_heads), int(max_tokens), DType(q_dtype)
         self.attention = attention or PagedAttention(q_heads, cache.kv_heads, head_dim, q_dtype, DType.F32)
-        if self.attention.q_dtype != self.q_dtype or self.attention.out_dtype != DType.F32:
-            raise InvalidInput("the shared attention has other types")
         q, kv = q_heads * head_dim, cache.kv_heads * head_dim
         self.d_q, self.d_k, self.d_v = (DeviceBuffer(max_tokens * n * 4) for n in (q, kv, kv))
         self.d_q16, self.d_attn = DeviceBuffer(max_tokens * q * 2), DeviceBuffer(max_tokens * q * 4)
+
+    @property
+    def attention(self) -> PagedAttention:
+        return self._attention
+
+    @attention.setter
+    def attention(self, shared: PagedAttention) -> None:
+        if shared.q_dtype != self.q_dtype or shared.out_dtype != DType.F32:
+            raise InvalidInput("the shared attention has other types")
+        theirs, ours = (shared.q_heads, shared.kv_heads, shared.head_dim), (self.q_heads, self.cache.kv_heads, self.cache.head_dim)
+        if theirs != ours:
+            raise InvalidInput(f"the shared attention has heads {theirs}, the layer {ours}")
+        self._attention = shared
 
     def forward_device(self, d_x: DeviceBuffer, plan: StepPlan, d_tables, requests: int, tokens: int, d_out: DeviceBuffer,
                        d_positions=None, stream=None, max_pages: int | None = None) -> None:

@@ -1,0 +1,26 @@
+"""What CachedAttention and PagedAttention refuse: arguments whose buffers are all long enough
+and whose results would be those of other tokens."""
+import numpy as np
+import pytest
+
+from attn_ref import F16
+from test_gpu_attn_step import DIM, HEADS, KV, MAX_PAGES, PAGE, Layer
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def layer(qmm, orc):
+    return Layer(qmm, orc, 0x1100, F16, 1)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(HEADS // 2, KV, DIM), (HEADS * 2, KV, DIM), (HEADS, KV * 2, DIM), (HEADS, KV, 128)])
+def test_shared_attention_of_other_heads(qmm, layer, heads, kv, dim):
+    """Fewer query heads: every size check of a call passes, rows are read at another stride."""
+    other = qmm.PagedAttention(heads, kv, dim, F16)
+    with pytest.raises(qmm.InvalidInput, match="shared attention has heads"):
+        qmm.CachedAttention(layer.weights, qmm.Rope(layer.freq), layer.cache, HEADS, 64, F16, attention=other)
+    step = qmm.CachedAttention(layer.weights, qmm.Rope(layer.freq), layer.cache, HEADS, 64, F16,
+                               attention=qmm.PagedAttention(HEADS, KV, DIM, F16))
+    with pytest.raises(qmm.InvalidInput, match="shared attention has heads"):
+        step.attention = other
