@@ -224,6 +224,8 @@ class CachedAttention:
             raise InvalidInput(f"max_pages {most}, tables of {plan.max_pages}")
         if tokens > min(self.max_tokens, plan.max_tokens):
             raise InvalidInput(f"{tokens} tokens, planned for {min(self.max_tokens, plan.max_tokens)}")
+        if plan.page_size != self.cache.page_size:
+            raise InvalidInput(f"plan for pages of {plan.page_size} tokens, the cache's have {self.cache.page_size}")
         w = self.weights
         w.project_qkv_device(d_x, self.d_q, self.d_k, self.d_v, tokens, stream)
         self.rope.append(self.cache, self.d_q, self.d_k, self.d_v, DType.F32, self.d_q16, self.q_dtype,

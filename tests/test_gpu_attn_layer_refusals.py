@@ -1,6 +1,5 @@
 """What CachedAttention and PagedAttention refuse: arguments whose buffers are all long enough
 and whose results would be those of other tokens."""
-import numpy as np
 import pytest
 
 from attn_ref import F16
@@ -24,3 +23,12 @@ def test_shared_attention_of_other_heads(qmm, layer, heads, kv, dim):
                                attention=qmm.PagedAttention(HEADS, KV, DIM, F16))
     with pytest.raises(qmm.InvalidInput, match="shared attention has heads"):
         step.attention = other
+
+
+@pytest.mark.parametrize("page", [8, 32, 64])
+def test_plan_of_another_page_size(qmm, layer, page):
+    """Its slots and table columns would be other tokens' in the layer's cache."""
+    plan = qmm.StepPlan(page, 1, 64, MAX_PAGES)
+    d = qmm.DeviceBuffer(1 << 18)
+    with pytest.raises(qmm.InvalidInput, match="pages of"):
+        layer.step.forward_device(d, plan, d, 1, 3, d)
