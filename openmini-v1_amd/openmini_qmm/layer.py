@@ -216,7 +216,8 @@ class CachedAttention:
                        d_positions=None, stream=None, max_pages: int | None = None) -> None:
         """d_out [tokens, hidden] for the step that `plan` laid out (plan.run on the same
         stream before the first layer): d_x [tokens, hidden] fp32, d_tables the tables that
-        the plan filled.  d_positions [axes][tokens]: None takes the plan's (one axis).
+        the plan filled.  d_positions [axes][tokens]: None takes the plan's, for a rope of one
+        axis (of several, text too has its position on each).
         max_pages: columns that the step's longest request needs, where that is known (None:
         the tables' width); attention of short rows is faster for it."""
         most = plan.max_pages if max_pages is None else int(max_pages)
@@ -226,6 +227,8 @@ class CachedAttention:
             raise InvalidInput(f"{tokens} tokens, planned for {min(self.max_tokens, plan.max_tokens)}")
         if plan.page_size != self.cache.page_size:
             raise InvalidInput(f"plan for pages of {plan.page_size} tokens, the cache's have {self.cache.page_size}")
+        if d_positions is None and self.rope.n_axes > 1:
+            raise InvalidInput(f"the plan's positions are for one axis, the rope has {self.rope.n_axes}")
         w = self.weights
         w.project_qkv_device(d_x, self.d_q, self.d_k, self.d_v, tokens, stream)
         self.rope.append(self.cache, self.d_q, self.d_k, self.d_v, DType.F32, self.d_q16, self.q_dtype,

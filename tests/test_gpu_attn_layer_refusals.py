@@ -32,3 +32,12 @@ def test_plan_of_another_page_size(qmm, layer, page):
     d = qmm.DeviceBuffer(1 << 18)
     with pytest.raises(qmm.InvalidInput, match="pages of"):
         layer.step.forward_device(d, plan, d, 1, 3, d)
+
+
+def test_positions_of_several_axes_are_needed(qmm, orc):
+    """The plan's one row of positions is no [axes][tokens], long enough as it may be."""
+    layer = Layer(qmm, orc, 0x1200, F16, 3)
+    plan = qmm.StepPlan(PAGE, 1, 64, MAX_PAGES)
+    d = qmm.DeviceBuffer(1 << 18)
+    with pytest.raises(qmm.InvalidInput, match="the rope has 3"):
+        layer.step.forward_device(d, plan, d, 1, 3, d)
