@@ -273,6 +273,8 @@ class PagedAttention:
             if d_rows is not None:
                 raise InvalidInput("requests is needed with d_rows")
             requests = rows
+        if requests < 1 and rows > 0:
+            raise InvalidInput(f"{rows} rows of {requests} requests")
         row = self.q_heads * self.head_dim
         qs, os_ = row if q_stride is None else q_stride, row if out_stride is None else out_stride
         ts = max_pages if table_stride is None else table_stride

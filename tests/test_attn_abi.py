@@ -9,7 +9,7 @@ import subprocess
 import numpy as np
 import pytest
 
-from openmini_qmm import DType, InvalidInput, KVCache, Rope, _native, rope_axes, rope_frequencies
+from openmini_qmm import DType, InvalidInput, KVCache, PagedAttention, Rope, _native, rope_axes, rope_frequencies
 import attn_ref as ref
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -211,6 +211,22 @@ def test_mirror_refusals():
     with pytest.raises(InvalidInput):
         Rope([1.0] * 8, pairing="thirds")
     assert DType.of("f8").nbytes == 1 and DType.of("f32").nbytes == 4
+
+
+@pytest.mark.parametrize("requests", [0, -1])
+def test_rows_need_a_request(requests):
+    """Rows that name request 0 of none: the tables' size was not checked for it."""
+    class Buf:
+        ptr, nbytes = ctypes.c_void_p(P), 1 << 20
+
+    class NoTables:
+        ptr, nbytes = ctypes.c_void_p(2 * P), 0
+    attn = PagedAttention.__new__(PagedAttention)
+    attn.q_heads, attn.kv_heads, attn.head_dim, attn.window, attn.scale = 4, 2, 128, 0, 0.1
+    attn.q_dtype, attn.out_dtype, attn.work, attn._call = DType.BF16, DType.F32, Buf, None
+    cache = KVCache(Buf, Buf, DType.BF16, 1, 16, 2, 128)
+    with pytest.raises(InvalidInput, match="1 rows"):
+        attn.run(cache, Buf, Buf, NoTables, 4, Buf, 1, d_rows=Buf, requests=requests)
 
 
 def test_frequencies_and_axes():
