@@ -141,8 +141,8 @@ typedef struct {
 
 int openmini_rope_apply(const openmini_rope_t* rope, const openmini_rope_args_t* args, void* stream);
 
-/* One step of a layer: q rotated to d_q_out; k rotated, and v as it is, each divided by its
- * scale, rounded to the cache's type (F8: to the nearest even, values past +-448 to +-448,
+/* One step of a layer: q rotated to d_q_out; k rotated, and v as it is, each times the
+ * reciprocal of its scale (which is above 2^-128), rounded to the cache's type (F8: to the nearest even, values past +-448 to +-448,
  * NaN stays) and written at the tokens' slots.  A token whose slot is negative or past the
  * cache writes q alone.  Two tokens with one slot: either is written.  d_q, d_k and d_v are
  * [tokens][heads | kv_heads][head_dim] of one type, token strides in elements (slices of

@@ -349,6 +349,11 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
     TRY(check_stride("k_stride", p->k_stride, kv_row, in));
     TRY(check_stride("v_stride", p->v_stride, kv_row, in));
     TRY(check_stride("q_out_stride", p->q_out_stride, q_row, 2));
+    a.k_over = 1.0f / cache->k_scale;
+    a.v_over = 1.0f / cache->v_scale;
+    if (!std::isfinite(a.k_over) || !std::isfinite(a.v_over))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "cache scales %g, %g: below 2^-128 they have no reciprocal", cache->k_scale,
+                    cache->v_scale);
     if (p->d_q_out == p->d_q || p->d_q_out == p->d_k || p->d_q_out == p->d_v)
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "d_q_out is one of the inputs");
     if (p->tokens == 0) return ok();
@@ -365,8 +370,6 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
     a.y_dtype = p->q_out_dtype;
     a.cache_dtype = cache->dtype;
     a.slots = p->d_slots;
-    a.k_over = 1.0f / cache->k_scale;
-    a.v_over = 1.0f / cache->v_scale;
     return launched(attn::launch_rope(a, cache->head_dim, static_cast<hipStream_t>(stream)), "rope append launch");
 }
 
