@@ -407,7 +407,9 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     const int out_size = size_of(p->out_dtype);
     TRY(check_stride("q_stride", p->q_stride, row, 2));
     TRY(check_stride("out_stride", p->out_stride, row, out_size));
-    if (!std::isfinite(p->scale)) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "scale %g is not finite", p->scale);
+    a.scale = (float)((double)p->scale * cache->k_scale * 1.44269504088896340736);
+    if (!std::isfinite(a.scale))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "scale %g (times the keys' %g and log2(e)) is not finite", p->scale, cache->k_scale);
     TRY(check_range("window", p->window, 0, INT64_MAX));
     TRY(check_range("max_pages", p->max_pages, 1, kMaxI32));
     TRY(check_range("table_stride", p->table_stride, p->max_pages, (int64_t)1 << 40));
@@ -448,7 +450,6 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     // added to the scalar address)
     a.wide = (double)(c.n_pages - 1) * (double)c.page_stride + (double)(cache->page_size + 8) * (double)c.token_stride + 1024 >=
              4294967296.0;
-    a.scale = (float)((double)p->scale * cache->k_scale * 1.44269504088896340736);
     a.shares = shares;
     a.launch_shares = tiles < (int64_t)shares ? (uint32_t)tiles : shares;
     a.by_units = attn::FastDiv((uint32_t)(cache->kv_heads * head_tiles));

@@ -192,6 +192,12 @@ def test_decode_refusals(cache, args, status, word):
     _refused(_native.lib().openmini_attn_decode(_cache(**cache), _attn(**args), None), status, word)
 
 
+@pytest.mark.parametrize("k_scale,scale", [(1e10, 1e30), (3e38, -2.0), (1.0, 3e38)])
+def test_decode_refuses_scales_past_fp32(k_scale, scale):
+    """Each finite, their product with log2(e) not: a score of 0 would be NaN."""
+    _refused(_native.lib().openmini_attn_decode(_cache(k_scale=k_scale), _attn(scale=scale), None), BAD, "scale")
+
+
 def test_workspace_bytes():
     L = _native.lib()
     assert L.openmini_attn_workspace_bytes(64, 8, 128) > 0
