@@ -465,7 +465,7 @@ int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_a
     // a window's first tile need not begin with it
     const int64_t most = (keys + tile - 1) / tile + (keys < max_len), pairs = p->rows * cache->kv_heads * head_tiles;
     a.whole = attn::decode_whole(most, pairs);
-    a.uncut = attn::decode_uncut(most, pairs);
+    a.uncut = attn::decode_uncut(most, p->rows, (int64_t)cache->kv_heads * head_tiles, shares, cache->head_dim, f8);
     if (a.uncut) a.launch_shares = p->rows < (int64_t)shares ? (uint32_t)p->rows : shares;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = p->q_dtype == OPENMINI_ATTN_BF16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)

@@ -2,6 +2,7 @@
 // (attn_plan.hip, attn_rope.hip, attn_decode.hpp).
 #pragma once
 
+#include "attn_decode_shape.hpp"
 #include "qmm_internal.hpp"
 
 #include "../../include/openmini_attn.h"
@@ -84,41 +85,6 @@ struct RopeArgs {
 hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s);
 
 // ---- attn_decode_*.hip ---------------------------------------------------------------
-constexpr int kDecodeWaves = 4;  // waves of a workgroup
-// Keys that a wave takes at a time, in 32s: about 16 KB of keys and values.
-constexpr int decode_subtiles(int head_dim, bool f8) {
-    return f8 ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1) : head_dim <= 64 ? 2 : 1;
-}
-constexpr int kHeadTile = 16;    // query heads a workgroup serves (the MFMA's columns)
-constexpr int kMaxHeads = 1024;  // query heads
-// Waves of a call, at most (one share each unless the units alone are more): one for each
-// SIMD.  Two or three raise the bytes in flight past what the memory needs, and then equal
-// shares end at different times (131071 keys, 8 heads of 128, bf16: 2048 waves 103 us, 1536
-// 116, 1024 93).
-constexpr int kRound = 1024;
-
-// Whether workgroups take whole rows: `most` tiles in a row at most, by the table's columns
-// and the window, and `pairs` of a row and a unit.  Up to two workgroups for each CU, and rows
-// of up to two tiles a wave, or four where the shares are no more than 16 for each pair
-// either.  Measured, whole rows against shares (us): 8 pairs of 300 keys, heads of 128, bf16
-// 7.0 / 9.4, of 700 9.8 / 10.7, of 1000 12.5 / 10.9; 64 pairs of 1000 13.5 / 16.2, of 2000
-// 22.6 / 18.5; 256 of up to 4000, heads of 64, 46.8 / 36.4; 512 of 400 15.1 / 20.4; 1024 of
-// 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.
-inline bool decode_whole(int64_t most, int64_t pairs) {
-    return most == 1 ? pairs <= 256 : pairs <= 512 && most <= (pairs < 64 ? 16 : 32);
-}
-
-// Whether the shares are rows, as many to a wave as to any other whatever their lengths, so
-// that no row is cut and there is no join: more pairs than workgroups take whole, of so few
-// tiles that lengths do not differ by much.  Measured, uncut against shares of tiles (us):
-// 1024 pairs of half to all of 4 tiles, heads of 128, bf16 11.3 / 16.9, of a twentieth to all
-// 9.6 / 13.0; 2048 the same 20.8 / 27.7 and 15.1 / 17.1; of 8 tiles 39.2 / 43.1 and 23.5 / 23.7,
-// in heads of 256 77.3 / 81.4 and 63.9 / 46.7; 6000 of a twentieth to all of 4 tiles 40.3 / 39.9.
-// 264 of one tile against whole rows 5.3 / 5.8, 128 5.2 / 5.3.
-inline bool decode_uncut(int64_t most, int64_t pairs) {
-    return most == 1 ? pairs > 256 : pairs > 512 && most <= (pairs <= 4096 ? 4 : 2);
-}
-
 // Whether a call reads keys and values past the caches (loads marked as not used again),
 // with `keys` of each key head at most: where these are 128 MiB or more, which the caches (256
 // MB, and a step's weights between two calls) would not hold for the next, and where lines of
