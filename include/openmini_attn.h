@@ -66,8 +66,11 @@ typedef struct {
  * takes from d_free in request order, starting at *d_head (NULL: at 0), into its table:
  * d_tables[r * table_stride + i] is the page of its tokens i * page_size on.  Nothing else
  * of the tables is written.  A request is refused, and takes nothing, if its tokens would
- * not fit max_pages pages, or if it needs pages and the free list has too few left after
- * the requests before it.  Outputs:
+ * not fit max_pages pages, or if it needs pages and the free list has fewer than it and all
+ * requests before it need (those too long for the table apart).  So the first request that is
+ * short of pages refuses all behind it that need any, also where what is left would do for
+ * them: the order of requests is that in which they are served, and a server that wants its
+ * decoding requests to go on puts them before the prompts.  Outputs:
  *   d_starts[requests + 1]  first token of each request in the step, and the token count
  *   d_lens[requests]        cached + new (refused: cached)
  *   for token j < max_tokens, request after request (-1, -1, -1, 0 past the last):
