@@ -177,7 +177,11 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
  *   s_i = scale * q . k_i,  out = sum_i softmax(s)_i v_i,  lse = log sum_i exp(s_i).
  * Query head h reads key head h / (q_heads / kv_heads).  A row that sees no key, or whose
  * request is outside [0, requests), is 0 with lse -inf; keys on pages outside the cache are
- * not seen.  What the cache holds past a row's keys does not matter (NaN included).
+ * not seen.  What the cache holds past a row's keys does not matter (NaN included).  Among
+ * them, a key whose score is -inf has no weight, and a row with no other is empty too; a score
+ * of +inf or NaN makes its head NaN.  A value that is NaN makes its dimension of all heads
+ * that read it NaN, one that is infinite makes it infinite or NaN (a probability is several
+ * factors, some of them 0 or below).  d_out, d_lse and d_work share no memory with the inputs.
  *
  * Types: q F16 or BF16 and the cache the same type, or F8_E4M3, which is converted to q's
  * (exactly); out q's type or F32.  Products are of 16-bit operands with 32-bit sums; the

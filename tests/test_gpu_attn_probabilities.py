@@ -128,3 +128,22 @@ def test_equal_scores_of_any_size(qmm, size, sign):
         out = ref.decode(c.run(qmm, scale=sign * size)[0], F32)
         want = c.values[0][:, 0].mean(0)
         assert np.all(np.abs(out[0] - want) <= (2.0 ** -22 + (n / 32 + 64) * 2.0 ** -24) * want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_t,c_t,bits", [(BF16, BF16, 0x7F80), (BF16, BF16, 0xFF80), (BF16, BF16, 0x7FC0), (F16, F16, 0x7C00), (F16, F16, 0x7E00),
+                                          (F16, F8, 0x7F), (BF16, F8, 0xFF)])
+def test_values_without_a_number(qmm, q_t, c_t, bits):
+    """An infinite value makes its dimension infinite or NaN for the heads that read it, NaN makes it
+    NaN, and nothing else: other dimensions, key heads and rows are as without it."""
+    for lens in ([300, 40], [5000, 300]):
+        c = Case(qmm, lens, 8, 2, 64, q_t, c_t, seed=21)
+        want = c.run(qmm)
+        c.vb[c.tables[0, 2], 5, 1, 37] = bits
+        c.upload(qmm)
+        got = c.run(qmm)
+        same = np.ones(got[0].shape, bool)
+        same[0, 4:, 37] = False
+        assert np.array_equal(got[0][same], want[0][same]) and np.array_equal(got[1], want[1])
+        hit = ref.decode(got[0], F32)[~same]
+        assert not np.isfinite(hit).any() and (np.isinf(ref.decode(np.array([bits], ref.BITS[c_t]), c_t)[0]) or np.isnan(hit).all())
