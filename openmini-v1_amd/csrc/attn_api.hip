@@ -246,7 +246,6 @@ int openmini_kv_plan(const openmini_kv_plan_args_t* p, void* stream) {
     a.table_stride = p->table_stride;
     a.requests = (uint32_t)p->requests;
     a.n_free = (uint32_t)p->n_free;
-    a.max_pages = (uint32_t)p->max_pages;
     a.max_held = (uint32_t)(p->max_pages * p->page_size);
     a.max_tokens = (uint32_t)p->max_tokens;
     a.page = attn::FastDiv((uint32_t)p->page_size);

@@ -43,7 +43,7 @@ struct PlanArgs {
     const int32_t *cached, *fresh, *free, *head;
     int32_t *tables, *starts, *lens, *rows, *positions, *slots, *row_lens, *counts;
     int64_t table_stride;
-    uint32_t requests, n_free, max_pages, max_held, max_tokens;  // max_held = max_pages * page_size
+    uint32_t requests, n_free, max_held, max_tokens;  // max_held = max_pages * page_size
     FastDiv page;
 };
 hipError_t launch_plan(const PlanArgs& a, hipStream_t s);

@@ -9,7 +9,7 @@
 //
 // Bound by latency: a launch, one load, the sums, the bisection, one more load for a
 // token's page.  Measured (MI355X): one request and token 2.3 us, 256 requests with 33000
-// tokens 4.3 us (554 KB; with the call from Python 4.9 us either way).
+// tokens 4.5 us (554 KB; with the call from Python 4.7 us either way).
 #include "attn_internal.hpp"
 
 namespace attn {
