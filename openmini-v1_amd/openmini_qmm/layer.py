@@ -227,6 +227,9 @@ class CachedAttention:
             raise InvalidInput(f"{tokens} tokens, planned for {min(self.max_tokens, plan.max_tokens)}")
         if plan.page_size != self.cache.page_size:
             raise InvalidInput(f"plan for pages of {plan.page_size} tokens, the cache's have {self.cache.page_size}")
+        for name, buf, columns in (("d_x", d_x, self.weights.q_proj.k_cols), ("d_out", d_out, self.weights.o_proj.n_rows)):
+            if buf.nbytes < 4 * tokens * columns:
+                raise InvalidInput(f"{name} holds {buf.nbytes} bytes, {4 * tokens * columns} are needed")
         if d_positions is None and self.rope.n_axes > 1:
             raise InvalidInput(f"the plan's positions are for one axis, the rope has {self.rope.n_axes}")
         w = self.weights

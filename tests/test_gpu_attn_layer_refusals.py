@@ -3,7 +3,7 @@ and whose results would be those of other tokens."""
 import pytest
 
 from attn_ref import F16
-from test_gpu_attn_step import DIM, HEADS, KV, MAX_PAGES, PAGE, Layer
+from test_gpu_attn_step import DIM, HEADS, HIDDEN, KV, MAX_PAGES, PAGE, Layer
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,13 @@ def test_positions_of_several_axes_are_needed(qmm, orc):
     d = qmm.DeviceBuffer(1 << 18)
     with pytest.raises(qmm.InvalidInput, match="the rope has 3"):
         layer.step.forward_device(d, plan, d, 1, 3, d)
+
+
+def test_short_buffers(qmm, layer):
+    """The projections write as many rows as they are told."""
+    plan = qmm.StepPlan(PAGE, 1, 64, MAX_PAGES)
+    d, short = qmm.DeviceBuffer(1 << 18), qmm.DeviceBuffer(3 * HIDDEN * 4 - 4)
+    with pytest.raises(qmm.InvalidInput, match="d_x holds"):
+        layer.step.forward_device(short, plan, d, 1, 3, d)
+    with pytest.raises(qmm.InvalidInput, match="d_out holds"):
+        layer.step.forward_device(d, plan, d, 1, 3, short)
