@@ -33,8 +33,8 @@
 // 90 (83), the kernel alone 84, 6.4 TB/s; 16 rows of 700 - 2100 keys, 32 heads of 128, fp16 54
 // (50); 64 rows of up to 4096 keys in a window, 4 heads of 64, bf16 28 (17); 128 rows of 2000 -
 // 12000 keys, 8 heads of 128, e4m3 245 (230).  One row of 300 keys, in one launch, 6.9 (2.4, a
-// launch).  Heads of 64 in e4m3 are bound by the issue of instructions instead (183 vector
-// instructions for 32 keys): 100 rows of 1000 - 8000 keys, 8 heads, 84 us, 4.4 TB/s.
+// launch).  Heads of 64 in e4m3 are bound by the issue of instructions instead (195 vector
+// instructions for 32 keys): 100 rows of 1000 - 8000 keys, 8 heads, 85 us, 4.3 TB/s.
 #pragma once
 
 #include <type_traits>

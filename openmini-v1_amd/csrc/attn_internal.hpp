@@ -92,7 +92,7 @@ hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s);
 // several rows, or tiles of heads, read the same keys.  Measured, with and without (us): one
 // row of 131071 keys, 8 heads of 128, bf16 90.3 / 98.4; 128 rows of up to 12000, e4m3 245 /
 // 271; 16 of up to 4000 (196 MB) 40.4 / 42.6, of 2000 27.7 / 27.4; of heads of 64 in e4m3,
-// token after token of a head 68.7 / 74.1, head after head (64 bytes each) 96.0 / 85.0;
+// token after token of a head 71.8 / 75.5, head after head (64 bytes each) 95.8 / 84.8;
 // 32 heads of one key head 33.2 / 24.8.
 inline bool decode_streams(const Cache& c, int kv_heads, int head_dim, bool f8, int64_t keys) {
     const int row_bytes = head_dim * (f8 ? 1 : 2);
