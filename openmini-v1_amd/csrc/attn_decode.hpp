@@ -30,9 +30,9 @@
 // registers of the present one are free, one wave to a SIMD, a row's first behind the last
 // products of the row before.  Measured (MI355X, us with the second launch, which is 4 to 6
 // of them; in brackets a read of as many bytes): 131071 keys of one row, 8 heads of 128, bf16
-// 90 (83), the kernel alone 84, 6.4 TB/s; 16 rows of 700 - 2100 keys, 32 heads of 128, fp16 54
+// 90 (83), the kernel alone 84, 6.4 TB/s; 16 rows of 700 - 2100 keys, 32 heads of 128, fp16 53
 // (50); 64 rows of up to 4096 keys in a window, 4 heads of 64, bf16 28 (17); 128 rows of 2000 -
-// 12000 keys, 8 heads of 128, e4m3 245 (230).  One row of 300 keys, in one launch, 6.9 (2.4, a
+// 12000 keys, 8 heads of 128, e4m3 245 (230).  One row of 300 keys, in one launch, 7.1 (2.4, a
 // launch).  Heads of 64 in e4m3 are bound by the issue of instructions instead (195 vector
 // instructions for 32 keys): 100 rows of 1000 - 8000 keys, 8 heads, 85 us, 4.3 TB/s.
 #pragma once
