@@ -1,169 +1,13 @@
-// C ABI of the attention step (include/openmini_attn.h): argument checks and kernel
+// C ABI of the attention step (include/openmini_attn.h, and the decode call of
+// include/openmini_kv_i8.h): argument checks and kernel
 // dispatch.  Host code only; every failure returns a status and leaves a message.
-#include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <new>
 
-#include "attn_internal.hpp"
+#include "attn_check.hpp"
 
-struct openmini_rope {
-    attn::Rope r;
-    int device = 0;
-};
+using namespace attn;
 
 namespace {
-
-int fail(int code, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    return qmm::report_error(code, buf);
-}
-
-int ok() {
-    qmm::set_last_error("");
-    return OPENMINI_QMM_OK;
-}
-
-int launched(hipError_t e, const char* what) {
-    if (e != hipSuccess) return fail(OPENMINI_QMM_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
-    return ok();
-}
-
-#define TRY(expr)                                  \
-    do {                                           \
-        const int rc_ = (expr);                    \
-        if (rc_ != OPENMINI_QMM_OK) return rc_;    \
-    } while (0)
-
-constexpr int64_t kMaxI32 = INT32_MAX;
-
-bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
-
-int invalid(const char* what, int64_t v) {
-    return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "invalid %s: %lld", what, (long long)v);
-}
-
-int check_range(const char* what, int64_t v, int64_t lo, int64_t hi) {
-    if (v < lo || v > hi)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%s = %lld is outside [%lld, %lld]", what, (long long)v, (long long)lo,
-                    (long long)hi);
-    return OPENMINI_QMM_OK;
-}
-
-int check_pointer(const char* what, const void* p, uintptr_t to) {
-    if (!p) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null %s", what);
-    if (!aligned(p, to)) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%s is not %d-byte aligned", what, (int)to);
-    return OPENMINI_QMM_OK;
-}
-
-// A stride in elements of `size` bytes: a multiple of 16 bytes, below 2^40 elements.
-int check_stride(const char* what, int64_t v, int64_t least, int size) {
-    if (v < least || v > ((int64_t)1 << 40) || (v * size) % 16)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%s = %lld elements: at least %lld and a multiple of 16 bytes", what,
-                    (long long)v, (long long)least);
-    return OPENMINI_QMM_OK;
-}
-
-// Whether `count` elements of 4 bytes from p on share memory with an array of rows of `row`
-// elements, `stride` from one to the next, from q on.
-bool shares_memory(const void* p, int64_t count, const void* q, int64_t rows, int64_t row, int64_t stride) {
-    if (!p || count <= 0) return false;
-    const int64_t from = ((int64_t)(uintptr_t)p - (int64_t)(uintptr_t)q) / 4, to = from + count;  // both 4-byte aligned
-    if (to <= 0 || from >= (rows - 1) * stride + row) return false;
-    const int64_t r = from < 0 ? 0 : from / stride;  // the row that begins at `from` or before it
-    return from < r * stride + row || (r + 1 < rows && to > (r + 1) * stride);
-}
-
-bool dense_type(int t) { return t == OPENMINI_ATTN_F32 || t == OPENMINI_ATTN_F16 || t == OPENMINI_ATTN_BF16; }
-bool half_type(int t) { return t == OPENMINI_ATTN_F16 || t == OPENMINI_ATTN_BF16; }
-int size_of(int t) { return t == OPENMINI_ATTN_F32 ? 4 : t == OPENMINI_ATTN_F8_E4M3 ? 1 : 2; }
-
-int unsupported(const char* what, int t) { return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "%s: type %d is not taken", what, t); }
-
-int check_cache(const openmini_kv_cache_t* c, attn::Cache* out) {
-    if (!c) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null cache");
-    if (!half_type(c->dtype) && c->dtype != OPENMINI_ATTN_F8_E4M3) return unsupported("cache", c->dtype);
-    TRY(check_pointer("cache d_k", c->d_k, 16));
-    TRY(check_pointer("cache d_v", c->d_v, 16));
-    TRY(check_range("kv_heads", c->kv_heads, 1, 1024));
-    TRY(check_range("head_dim", c->head_dim, 8, 512));
-    if (c->head_dim % 8) return invalid("head_dim (a multiple of 8)", c->head_dim);
-    TRY(check_range("page_size", c->page_size, 1, (int64_t)1 << 20));
-    TRY(check_range("n_pages", c->n_pages, 1, kMaxI32 / c->page_size));
-    const int size = size_of(c->dtype);
-    TRY(check_stride("page_stride", c->page_stride, 0, size));
-    TRY(check_stride("token_stride", c->token_stride, 0, size));
-    TRY(check_stride("head_stride", c->head_stride, 0, size));
-    if (!std::isfinite(c->k_scale) || !std::isfinite(c->v_scale) || c->k_scale <= 0 || c->v_scale <= 0)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "cache scales %g, %g: positive and finite", c->k_scale, c->v_scale);
-    out->k = static_cast<uint8_t*>(c->d_k);
-    out->v = static_cast<uint8_t*>(c->d_v);
-    out->page_stride = c->page_stride * size;
-    out->token_stride = c->token_stride * size;
-    out->head_stride = c->head_stride * size;
-    out->n_pages = (uint32_t)c->n_pages;
-    out->slots = (uint32_t)(c->n_pages * c->page_size);
-    out->page = attn::FastDiv((uint32_t)c->page_size);
-    out->k_scale = c->k_scale;
-    out->v_scale = c->v_scale;
-    return OPENMINI_QMM_OK;
-}
-
-int check_rope(const openmini_rope* rope) {
-    if (!rope) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null rope handle");
-    int dev = 0;
-    TRY(qmm::current_device(&dev));
-    if (dev != rope->device)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "rope handle lives on device %d, current device is %d", rope->device, dev);
-    return OPENMINI_QMM_OK;
-}
-
-// Checks common to both rotary calls.
-int check_heads(const openmini_rope* rope, int64_t tokens, int64_t heads, int64_t head_dim, const int32_t* d_positions,
-                int64_t position_stride) {
-    TRY(check_range("tokens", tokens, 0, kMaxI32));
-    TRY(check_range("heads", heads, 1, 4096));
-    TRY(check_range("head_dim", head_dim, 8, 512));
-    if (head_dim % 8) return invalid("head_dim (a multiple of 8)", head_dim);
-    if (2 * rope->r.n_pairs > head_dim)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%d rotary pairs do not fit head_dim = %lld", rope->r.n_pairs,
-                    (long long)head_dim);
-    TRY(check_pointer("d_positions", d_positions, 4));
-    if (rope->r.axes > 1 && position_stride < tokens)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "position_stride = %lld below the %lld tokens", (long long)position_stride,
-                    (long long)tokens);
-    return OPENMINI_QMM_OK;
-}
-
-void set_rope(attn::RopeArgs& a, const openmini_rope* rope, int64_t tokens, int heads, int kv_heads, int head_dim,
-              const int32_t* d_positions, int64_t position_stride) {
-    a.positions = d_positions;
-    a.position_stride = position_stride;
-    a.pairs = rope->r.pairs;
-    a.scale = rope->r.scale;
-    a.n_pairs = rope->r.n_pairs;
-    a.adjacent = rope->r.adjacent;
-    a.tokens = (int32_t)tokens;
-    a.heads = heads;
-    a.kv_heads = kv_heads;
-    a.per_head = attn::FastDiv((uint32_t)head_dim / 8);
-    a.per_token = attn::FastDiv((uint32_t)((heads + 2 * kv_heads) * (head_dim / 8)));
-    a.by_pairs = attn::FastDiv((uint32_t)rope->r.n_pairs);
-}
-
-constexpr int kDims[] = {64, 96, 128, 192, 256};
-
-bool decode_dim(int d) {
-    for (int k : kDims)
-        if (k == d) return true;
-    return false;
-}
-
-size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
 // The workspace: the split rows, then the parts' maxima and sums, then their accumulators.
 struct Workspace {
@@ -178,9 +22,6 @@ Workspace workspace(int q_heads, int kv_heads, int head_tiles, int head_dim) {
     return w;
 }
 
-constexpr int64_t kMaxRows = (int64_t)1 << 20;
-constexpr int64_t kMostKeys = kMaxI32 - 255;  // whole tiles of keys stay below 2^31
-
 bool decode_sizes(int q_heads, int kv_heads, int head_dim, int* head_tiles) {
     if (kv_heads < 1 || q_heads < kv_heads || q_heads > 1024 || q_heads % kv_heads ||
         !decode_dim(head_dim))
@@ -188,6 +29,106 @@ bool decode_sizes(int q_heads, int kv_heads, int head_dim, int* head_tiles) {
     const int group = q_heads / kv_heads;
     *head_tiles = (group + attn::kHeadTile - 1) / attn::kHeadTile;
     return true;
+}
+
+// Both decode calls: on 8-bit integers with the blocks' scales (i8), or on the other caches.
+int decode(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales, const openmini_attn_args_t* p, void* stream,
+           bool i8) {
+    if (!p) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null arguments");
+    attn::DecodeI8Args a = {};
+    TRY(i8 ? check_cache_i8(cache, scales, &a.cache, &a.scales) : check_cache(cache, &a.cache));
+    if (!half_type(p->q_dtype)) return unsupported("q", p->q_dtype);
+    const bool f8 = i8 || cache->dtype == OPENMINI_ATTN_F8_E4M3;  // an element is a byte
+    if (!f8 && cache->dtype != p->q_dtype)
+        return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "q of type %d on a cache of type %d", p->q_dtype, cache->dtype);
+    if (p->out_dtype != p->q_dtype && p->out_dtype != OPENMINI_ATTN_F32) return unsupported("out", p->out_dtype);
+    if (!decode_dim(cache->head_dim))
+        return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "head_dim = %d (64, 96, 128, 192 and 256 are taken)", cache->head_dim);
+    if (cache->page_size % 8)
+        return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "page_size = %d is not a multiple of 8", cache->page_size);
+    TRY(check_range("rows", p->rows, 0, kMaxRows));
+    int head_tiles = 0;
+    if (!decode_sizes(p->q_heads, cache->kv_heads, cache->head_dim, &head_tiles))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "q_heads = %d for kv_heads = %d: a multiple, at most 1024", p->q_heads,
+                    cache->kv_heads);
+    TRY(check_pointer("d_q", p->d_q, 16));
+    TRY(check_pointer("d_out", p->d_out, 16));
+    TRY(check_pointer("d_lens", p->d_lens, 4));
+    TRY(check_pointer("d_tables", p->d_tables, 4));
+    if (p->d_rows) TRY(check_pointer("d_rows", p->d_rows, 4));
+    if (p->d_lse) TRY(check_pointer("d_lse", p->d_lse, 4));
+    const int64_t row = (int64_t)p->q_heads * cache->head_dim;
+    const int out_size = size_of(p->out_dtype);
+    TRY(check_stride("q_stride", p->q_stride, row, 2));
+    TRY(check_stride("out_stride", p->out_stride, row, out_size));
+    a.scale = (float)((double)p->scale * cache->k_scale * 1.44269504088896340736);
+    if (!std::isfinite(a.scale))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "scale %g (times the keys' %g and log2(e)) is not finite", p->scale, cache->k_scale);
+    TRY(check_range("window", p->window, 0, INT64_MAX));
+    TRY(check_range("max_pages", p->max_pages, 1, kMaxI32));
+    TRY(check_range("table_stride", p->table_stride, p->max_pages, (int64_t)1 << 40));
+    TRY(check_range("requests", p->requests, 1, kMaxI32));
+    if (p->rows == 0) return ok();
+    const attn::Cache& c = a.cache;
+    const int64_t held = p->max_pages * cache->page_size, max_len = held < kMostKeys ? held : kMostKeys;
+    const uint32_t shares = attn::decode_shares(cache->kv_heads, head_tiles);
+    // tiles of the call at most
+    const int64_t tiles = p->rows * (max_len / (32 * attn::decode_subtiles(cache->head_dim, f8)) + 2);
+    if (tiles > (int64_t)UINT32_MAX / 2)
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%lld rows of up to %lld keys are too many for one call",
+                    (long long)p->rows, (long long)max_len);
+    const auto w = workspace(p->q_heads, cache->kv_heads, head_tiles, cache->head_dim);
+    TRY(check_pointer("d_work", p->d_work, 256));
+    if (p->work_bytes < w.bytes)
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "workspace of %zu bytes, %zu are needed", p->work_bytes, w.bytes);
+    TRY(qmm::current_device(nullptr));
+    a.q = static_cast<const uint8_t*>(p->d_q);
+    a.out = static_cast<uint8_t*>(p->d_out);
+    a.lse = p->d_lse;
+    a.lens = p->d_lens;
+    a.rows = p->d_rows;
+    a.tables = p->d_tables;
+    a.q_stride = p->q_stride * 2;
+    a.out_stride = p->out_stride * out_size;
+    a.table_stride = p->table_stride;
+    a.window = p->window && p->window < max_len ? (uint32_t)p->window : (uint32_t)max_len;
+    a.n_rows = (uint32_t)p->rows;
+    a.requests = (uint32_t)p->requests;
+    a.max_len = (uint32_t)max_len;
+    a.q_heads = p->q_heads;
+    a.kv_heads = cache->kv_heads;
+    a.group = p->q_heads / cache->kv_heads;
+    a.head_tiles = head_tiles;
+    a.out_f32 = p->out_dtype == OPENMINI_ATTN_F32;
+    // the last byte that a lane's own offset reaches (heads and the eight keys of a group are
+    // added to the scalar address)
+    a.wide = (double)(c.n_pages - 1) * (double)c.page_stride + (double)(cache->page_size + 8) * (double)c.token_stride + 1024 >=
+             4294967296.0;
+    a.shares = shares;
+    a.launch_shares = tiles < (int64_t)shares ? (uint32_t)tiles : shares;
+    a.by_units = attn::FastDiv((uint32_t)(cache->kv_heads * head_tiles));
+    a.by_head_tiles = attn::FastDiv((uint32_t)head_tiles);
+    uint8_t* work = static_cast<uint8_t*>(p->d_work);
+    a.split = reinterpret_cast<attn::Split*>(work);
+    a.part_ml = reinterpret_cast<float2*>(work + w.ml_at);
+    a.part_acc = reinterpret_cast<float*>(work + w.acc_at);
+    a.by_row = p->rows <= (int64_t)shares;
+    const int64_t keys = max_len < (int64_t)a.window ? max_len : (int64_t)a.window, tile = 32 * attn::decode_subtiles(cache->head_dim, f8);
+    a.stream = head_tiles == 1 && p->rows <= p->requests &&
+               attn::decode_streams(c, cache->kv_heads, cache->head_dim, f8, p->rows * keys);
+    // a window's first tile need not begin with it
+    const int64_t most = (keys + tile - 1) / tile + (keys < max_len), pairs = p->rows * cache->kv_heads * head_tiles;
+    a.whole = attn::decode_whole(most, pairs);
+    a.uncut = attn::decode_uncut(most, p->rows, (int64_t)cache->kv_heads * head_tiles, shares, cache->head_dim, f8);
+    if (a.uncut) a.launch_shares = p->rows < (int64_t)shares ? (uint32_t)p->rows : shares;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool bf16 = p->q_dtype == OPENMINI_ATTN_BF16;
+    hipError_t e = i8     ? (bf16 ? attn::launch_decode_i8_bf16 : attn::launch_decode_i8_f16)(a, cache->head_dim, s)
+                   : bf16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)
+                          : attn::launch_decode_f16(a, cache->head_dim, f8, s);
+    if (e == hipSuccess && !a.whole && !a.uncut && a.launch_shares > 1)
+        e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
+    return launched(e, "attention launch");
 }
 
 }  // namespace
@@ -334,41 +275,14 @@ int openmini_rope_append(const openmini_rope_t* rope, const openmini_kv_cache_t*
     TRY(check_rope(rope));
     attn::RopeArgs a = {};
     TRY(check_cache(cache, &a.cache));
-    if (!dense_type(p->in_dtype)) return unsupported("q, k, v", p->in_dtype);
-    if (!half_type(p->q_out_dtype)) return unsupported("q_out", p->q_out_dtype);
-    TRY(check_heads(rope, p->tokens, p->q_heads, cache->head_dim, p->d_positions, p->position_stride));
-    TRY(check_pointer("d_q", p->d_q, 16));
-    TRY(check_pointer("d_k", p->d_k, 16));
-    TRY(check_pointer("d_v", p->d_v, 16));
-    TRY(check_pointer("d_q_out", p->d_q_out, 16));
-    TRY(check_pointer("d_slots", p->d_slots, 4));
-    const int in = size_of(p->in_dtype);
-    const int64_t q_row = (int64_t)p->q_heads * cache->head_dim, kv_row = (int64_t)cache->kv_heads * cache->head_dim;
-    TRY(check_stride("q_stride", p->q_stride, q_row, in));
-    TRY(check_stride("k_stride", p->k_stride, kv_row, in));
-    TRY(check_stride("v_stride", p->v_stride, kv_row, in));
-    TRY(check_stride("q_out_stride", p->q_out_stride, q_row, 2));
+    TRY(check_append(rope, cache, p));
     a.k_over = 1.0f / cache->k_scale;
     a.v_over = 1.0f / cache->v_scale;
     if (!std::isfinite(a.k_over) || !std::isfinite(a.v_over))
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "cache scales %g, %g: below 2^-128 they have no reciprocal", cache->k_scale,
                     cache->v_scale);
-    if (p->d_q_out == p->d_q || p->d_q_out == p->d_k || p->d_q_out == p->d_v)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "d_q_out is one of the inputs");
     if (p->tokens == 0) return ok();
-    set_rope(a, rope, p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->d_positions, p->position_stride);
-    a.x = static_cast<const uint8_t*>(p->d_q);
-    a.k = static_cast<const uint8_t*>(p->d_k);
-    a.v = static_cast<const uint8_t*>(p->d_v);
-    a.x_stride = p->q_stride * in;
-    a.k_stride = p->k_stride * in;
-    a.v_stride = p->v_stride * in;
-    a.y = static_cast<uint8_t*>(p->d_q_out);
-    a.y_stride = p->q_out_stride * 2;
-    a.x_dtype = p->in_dtype;
-    a.y_dtype = p->q_out_dtype;
-    a.cache_dtype = cache->dtype;
-    a.slots = p->d_slots;
+    set_append(a, rope, cache, p);
     return launched(attn::launch_rope(a, cache->head_dim, static_cast<hipStream_t>(stream)), "rope append launch");
 }
 
@@ -379,99 +293,12 @@ size_t openmini_attn_workspace_bytes(int q_heads, int kv_heads, int head_dim) {
 }
 
 int openmini_attn_decode(const openmini_kv_cache_t* cache, const openmini_attn_args_t* p, void* stream) {
-    if (!p) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null arguments");
-    attn::DecodeArgs a = {};
-    TRY(check_cache(cache, &a.cache));
-    if (!half_type(p->q_dtype)) return unsupported("q", p->q_dtype);
-    const bool f8 = cache->dtype == OPENMINI_ATTN_F8_E4M3;
-    if (!f8 && cache->dtype != p->q_dtype)
-        return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "q of type %d on a cache of type %d", p->q_dtype, cache->dtype);
-    if (p->out_dtype != p->q_dtype && p->out_dtype != OPENMINI_ATTN_F32) return unsupported("out", p->out_dtype);
-    if (!decode_dim(cache->head_dim))
-        return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "head_dim = %d (64, 96, 128, 192 and 256 are taken)", cache->head_dim);
-    if (cache->page_size % 8)
-        return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "page_size = %d is not a multiple of 8", cache->page_size);
-    TRY(check_range("rows", p->rows, 0, kMaxRows));
-    int head_tiles = 0;
-    if (!decode_sizes(p->q_heads, cache->kv_heads, cache->head_dim, &head_tiles))
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "q_heads = %d for kv_heads = %d: a multiple, at most 1024", p->q_heads,
-                    cache->kv_heads);
-    TRY(check_pointer("d_q", p->d_q, 16));
-    TRY(check_pointer("d_out", p->d_out, 16));
-    TRY(check_pointer("d_lens", p->d_lens, 4));
-    TRY(check_pointer("d_tables", p->d_tables, 4));
-    if (p->d_rows) TRY(check_pointer("d_rows", p->d_rows, 4));
-    if (p->d_lse) TRY(check_pointer("d_lse", p->d_lse, 4));
-    const int64_t row = (int64_t)p->q_heads * cache->head_dim;
-    const int out_size = size_of(p->out_dtype);
-    TRY(check_stride("q_stride", p->q_stride, row, 2));
-    TRY(check_stride("out_stride", p->out_stride, row, out_size));
-    a.scale = (float)((double)p->scale * cache->k_scale * 1.44269504088896340736);
-    if (!std::isfinite(a.scale))
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "scale %g (times the keys' %g and log2(e)) is not finite", p->scale, cache->k_scale);
-    TRY(check_range("window", p->window, 0, INT64_MAX));
-    TRY(check_range("max_pages", p->max_pages, 1, kMaxI32));
-    TRY(check_range("table_stride", p->table_stride, p->max_pages, (int64_t)1 << 40));
-    TRY(check_range("requests", p->requests, 1, kMaxI32));
-    if (p->rows == 0) return ok();
-    const attn::Cache& c = a.cache;
-    const int64_t held = p->max_pages * cache->page_size, max_len = held < kMostKeys ? held : kMostKeys;
-    const uint32_t shares = attn::decode_shares(cache->kv_heads, head_tiles);
-    // tiles of the call at most
-    const int64_t tiles = p->rows * (max_len / (32 * attn::decode_subtiles(cache->head_dim, f8)) + 2);
-    if (tiles > (int64_t)UINT32_MAX / 2)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%lld rows of up to %lld keys are too many for one call",
-                    (long long)p->rows, (long long)max_len);
-    const auto w = workspace(p->q_heads, cache->kv_heads, head_tiles, cache->head_dim);
-    TRY(check_pointer("d_work", p->d_work, 256));
-    if (p->work_bytes < w.bytes)
-        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "workspace of %zu bytes, %zu are needed", p->work_bytes, w.bytes);
-    TRY(qmm::current_device(nullptr));
-    a.q = static_cast<const uint8_t*>(p->d_q);
-    a.out = static_cast<uint8_t*>(p->d_out);
-    a.lse = p->d_lse;
-    a.lens = p->d_lens;
-    a.rows = p->d_rows;
-    a.tables = p->d_tables;
-    a.q_stride = p->q_stride * 2;
-    a.out_stride = p->out_stride * out_size;
-    a.table_stride = p->table_stride;
-    a.window = p->window && p->window < max_len ? (uint32_t)p->window : (uint32_t)max_len;
-    a.n_rows = (uint32_t)p->rows;
-    a.requests = (uint32_t)p->requests;
-    a.max_len = (uint32_t)max_len;
-    a.q_heads = p->q_heads;
-    a.kv_heads = cache->kv_heads;
-    a.group = p->q_heads / cache->kv_heads;
-    a.head_tiles = head_tiles;
-    a.out_f32 = p->out_dtype == OPENMINI_ATTN_F32;
-    // the last byte that a lane's own offset reaches (heads and the eight keys of a group are
-    // added to the scalar address)
-    a.wide = (double)(c.n_pages - 1) * (double)c.page_stride + (double)(cache->page_size + 8) * (double)c.token_stride + 1024 >=
-             4294967296.0;
-    a.shares = shares;
-    a.launch_shares = tiles < (int64_t)shares ? (uint32_t)tiles : shares;
-    a.by_units = attn::FastDiv((uint32_t)(cache->kv_heads * head_tiles));
-    a.by_head_tiles = attn::FastDiv((uint32_t)head_tiles);
-    uint8_t* work = static_cast<uint8_t*>(p->d_work);
-    a.split = reinterpret_cast<attn::Split*>(work);
-    a.part_ml = reinterpret_cast<float2*>(work + w.ml_at);
-    a.part_acc = reinterpret_cast<float*>(work + w.acc_at);
-    a.by_row = p->rows <= (int64_t)shares;
-    const int64_t keys = max_len < (int64_t)a.window ? max_len : (int64_t)a.window, tile = 32 * attn::decode_subtiles(cache->head_dim, f8);
-    a.stream = head_tiles == 1 && p->rows <= p->requests &&
-               attn::decode_streams(c, cache->kv_heads, cache->head_dim, f8, p->rows * keys);
-    // a window's first tile need not begin with it
-    const int64_t most = (keys + tile - 1) / tile + (keys < max_len), pairs = p->rows * cache->kv_heads * head_tiles;
-    a.whole = attn::decode_whole(most, pairs);
-    a.uncut = attn::decode_uncut(most, p->rows, (int64_t)cache->kv_heads * head_tiles, shares, cache->head_dim, f8);
-    if (a.uncut) a.launch_shares = p->rows < (int64_t)shares ? (uint32_t)p->rows : shares;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipError_t e = p->q_dtype == OPENMINI_ATTN_BF16 ? attn::launch_decode_bf16(a, cache->head_dim, f8, s)
-                                                    : attn::launch_decode_f16(a, cache->head_dim, f8, s);
-    if (e == hipSuccess && !a.whole && !a.uncut && a.launch_shares > 1)
-        e = attn::launch_join(a, cache->head_dim, p->out_dtype, s);
-    return launched(e, "attention launch");
+    return decode(cache, nullptr, p, stream, false);
+}
+
+int openmini_attn_decode_i8(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales, const openmini_attn_args_t* p,
+                            void* stream) {
+    return decode(cache, scales, p, stream, true);
 }
 
 }  // extern "C"

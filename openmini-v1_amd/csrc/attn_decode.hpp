@@ -50,6 +50,11 @@ using qmm::f32x4;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
+// What a cache holds: 16 bits, e4m3, or 8-bit integers with a scale for each block.
+enum Elem { kHalf, kF8, kI8 };
+template <Elem E>
+using ArgsOf = std::conditional_t<E == kI8, DecodeI8Args, DecodeArgs>;
+
 struct BF16 {
     static constexpr int kExactParts = 3;  // that hold an fp32 probability, 8 bits each
     static constexpr bool kNarrow = false;  // parts have the range of fp32
@@ -68,6 +73,11 @@ struct BF16 {
     template <bool kHigh>
     static __device__ __forceinline__ uint32_t from_f8(uint32_t u) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 1.0f, kHigh));
+    }
+    // Two of the four 8-bit integers of u: six instructions for all four.
+    template <bool kHigh>
+    static __device__ __forceinline__ uint32_t from_i8(uint32_t u) {
+        return pair((float)(int8_t)(u >> (kHigh ? 16 : 0)), (float)(int8_t)(u >> (kHigh ? 24 : 8)));
     }
 };
 
@@ -90,7 +100,19 @@ struct F16 {
     static __device__ __forceinline__ uint32_t from_f8(uint32_t u) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, 1.0f, kHigh));
     }
+    // c + 128 as the last bits of 1024, less 1152: five instructions for all four.
+    template <bool kHigh>
+    static __device__ __forceinline__ uint32_t from_i8(uint32_t u) {
+        const uint32_t up = __builtin_amdgcn_perm(0x64646464u, u ^ 0x80808080u, kHigh ? 0x04030402u : 0x04010400u);
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(qmm::f16x2, up) - qmm::f16x2{(_Float16)1152.0f, (_Float16)1152.0f});
+    }
 };
+
+template <class T, Elem E, bool kHigh>
+__device__ __forceinline__ uint32_t from_byte(uint32_t u) {
+    if constexpr (E == kI8) return T::template from_i8<kHigh>(u);
+    return T::template from_f8<kHigh>(u);
+}
 
 // kStream: loads that leave the caches to others (decode_streams).
 template <bool kStream, class V>
@@ -270,16 +292,17 @@ __device__ __forceinline__ bool find_share(const First& a, uint32_t p, Share& ou
 // they are joined in LDS: one launch, and no wave that looks for its share, but as many CUs
 // as there are rows and units, and a CU reads about 50 GB/s.  For short rows (decode_whole);
 // the last tile of a wave is most of its work then, so no loads of a next one are behind it.
-template <int D, class T, bool F8, int kSub, int W, bool kWide, bool kWhole, bool kStream>
-__global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel(const int32_t* lens, const int32_t* rows,
+template <int D, class T, Elem E, int kSub, int W, bool kWide, bool kWhole, bool kStream>
+__global__ __launch_bounds__(64 * W, D == 256 && E == kHalf ? 1 : 2) void decode_kernel(const int32_t* lens, const int32_t* rows,
                                                                                  uint32_t n_rows, uint32_t requests,
                                                                                  uint32_t max_len, uint32_t window,
                                                                                  uint32_t shares, uint32_t units,
                                                                                  uint32_t units_m, uint32_t units_shift, uint32_t eighth,
                                                                                  uint32_t uncut,
-                                                                                 DecodeArgs a) {
+                                                                                 ArgsOf<E> a) {
+    constexpr bool F8 = E != kHalf;           // a cache element is a byte
     const First f = {lens, rows, n_rows, requests, max_len, window, shares, uncut};
-    using P = std::conditional_t<F8, BF16, T>;  // of the second product's parts: both hold e4m3
+    using P = std::conditional_t<F8, BF16, T>;  // of the second product's parts: both hold e4m3 and 8-bit integers
     constexpr int kEl = F8 ? 1 : 2;           // bytes of a cache element
     constexpr uint32_t kKeys = 32 * kSub;     // keys of a tile, in kSub tiles of 32
     constexpr int kSteps = D / 32;            // MFMAs over head_dim of the first product
@@ -379,6 +402,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     struct Pages {  // of a tile's K and V groups, and the groups' places in them
         int32_t k[kSub], v[kSub];
         uint32_t k_in[kSub], v_in[kSub];
+        // kI8: the scales of the lane's keys and values (those of a V group)
+        float k_scale[E == kI8 ? kSub : 1], v_scale[E == kI8 ? kSub : 1];
     };
     auto page_of = [&](const Tile& t, int32_t key, int32_t* page, uint32_t* in_page) {
         const uint32_t at = a.cache.page.div_by_many((uint32_t)key);
@@ -400,9 +425,15 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     };
 
     uint32_t kraw[kSub][2][kKWords], vraw[kSub][8][kVWords];
-    auto load_k = [&](const Pages& pages) {
+    auto load_k = [&](Pages& pages) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
+            if constexpr (E == kI8) {
+                const int64_t page = (uint32_t)pages.v[u] < a.cache.n_pages ? pages.v[u] : 0;
+                const int64_t at = page * a.scales.page_stride + (int64_t)(pages.v_in[u] >> a.scales.shift) * a.scales.block_stride;
+                pages.k_scale[u] = a.scales.k[at + kv * a.scales.head_stride];
+                pages.v_scale[u] = a.scales.v[at + kv * a.scales.head_stride];
+            }
             const Place at = place_of(pages.k[u], pages.k_in[u] + k_row) + g * 16;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -446,8 +477,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                     u32x4 kf;
                     if constexpr (F8) {
                         const uint32_t w0 = kraw[u][s][2 * st], w1 = kraw[u][s][2 * st + 1];
-                        kf = u32x4{T::template from_f8<false>(w0), T::template from_f8<true>(w0),
-                                   T::template from_f8<false>(w1), T::template from_f8<true>(w1)};
+                        kf = u32x4{from_byte<T, E, false>(w0), from_byte<T, E, true>(w0), from_byte<T, E, false>(w1),
+                                   from_byte<T, E, true>(w1)};
                     } else {
                         kf = u32x4{kraw[u][s][4 * st], kraw[u][s][4 * st + 1], kraw[u][s][4 * st + 2],
                                    kraw[u][s][4 * st + 3]};
@@ -464,24 +495,33 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
         bool whole = key0 >= cur.lo && key0 + (int32_t)kKeys - 24 <= cur.hi;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
+            const float scale = E == kI8 ? a.scale * now.k_scale[u] : a.scale;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[u][j] = sc[u][j / 4][j % 4] * a.scale;
+                x[u][j] = sc[u][j / 4][j % 4] * scale;
                 if constexpr (P::kNarrow) least = fminf(least, x[u][j]);
             }
             whole = whole && (uint32_t)now.v[u] < a.cache.n_pages;
         }
         if (!__all(whole)) {
 #pragma unroll
-            for (int u = 0; u < kSub; ++u)
+            for (int u = 0; u < kSub; ++u) {
+                const bool paged = (uint32_t)now.v[u] < a.cache.n_pages;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int32_t key = key0 + 32 * u + j;
-                    const bool seen = (uint32_t)now.v[u] < a.cache.n_pages && key >= cur.lo && key < cur.hi;
+                    const bool seen = paged && key >= cur.lo && key < cur.hi;
                     x[u][j] = seen ? x[u][j] : -INFINITY;
+                    if constexpr (E != kI8) {
 #pragma unroll
-                    for (int w = 0; w < kVWords; ++w) vraw[u][j][w] = seen ? vraw[u][j][w] : 0;  // 0 * NaN is NaN
+                        for (int w = 0; w < kVWords; ++w) vraw[u][j][w] = seen ? vraw[u][j][w] : 0;  // 0 * NaN is NaN
+                    }
                 }
+                if constexpr (E == kI8) {  // nor is a scale that no key of the group needs
+                    const int32_t key = key0 + 32 * u;
+                    now.v_scale[u] = paged && key + 8 > cur.lo && key < cur.hi ? now.v_scale[u] : 0;
+                }
+            }
         }
         float top = x[0][0];
 #pragma unroll
@@ -534,7 +574,10 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                     for (int j = 0; j < 8; j += 2) {
                         const float r0 = exp2_of(x[u][j] - base), r1 = exp2_of(x[u][j + 1] - base);
                         l += r0 + r1;
-                        split(r0, r1, j);
+                        if constexpr (E == kI8)
+                            split(r0 * now.v_scale[u], r1 * now.v_scale[u], j);
+                        else
+                            split(r0, r1, j);
                     }
                 }
                 // a zero that is not known to be one: else V's fragments are made before the loop
@@ -555,12 +598,12 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
                             for (int q = 0; q < 4; ++q) {
                                 const uint32_t v0 = vraw[u][2 * q][word0 + w], v1 = vraw[u][2 * q + 1][word0 + w];
                                 const uint32_t lo = __builtin_amdgcn_perm(v1, v0, 0x05010400u);
-                                f[0][q] = P::template from_f8<false>(lo);
-                                f[1][q] = P::template from_f8<true>(lo);
+                                f[0][q] = from_byte<P, E, false>(lo);
+                                f[1][q] = from_byte<P, E, true>(lo);
                                 if constexpr (kWidth >= 4) {
                                     const uint32_t hi = __builtin_amdgcn_perm(v1, v0, 0x07030602u);
-                                    f[2][q] = P::template from_f8<false>(hi);
-                                    f[3][q] = P::template from_f8<true>(hi);
+                                    f[2][q] = from_byte<P, E, false>(hi);
+                                    f[3][q] = from_byte<P, E, true>(hi);
                                 }
                             }
 #pragma unroll
@@ -779,41 +822,41 @@ __global__ __launch_bounds__(64 * W, D == 256 && !F8 ? 1 : 2) void decode_kernel
     }
 }
 
-template <int D, class T, bool F8, bool kWide, bool kWhole, bool kStream>
-hipError_t launch_one(const DecodeArgs& a, hipStream_t s) {
+template <int D, class T, Elem E, bool kWide, bool kWhole, bool kStream>
+hipError_t launch_one(const ArgsOf<E>& a, hipStream_t s) {
+    constexpr bool F8 = E != kHalf;
     constexpr int W = kWhole && !(D == 256 && !F8) ? 2 * kDecodeWaves : kDecodeWaves, kSub = decode_subtiles(D, F8);
     const uint64_t units = (uint64_t)a.kv_heads * a.head_tiles;
     const uint64_t all = kWhole ? a.n_rows * units : (a.launch_shares * units + W - 1) / W, wgs = (all + 7) / 8 * 8;
-    hipLaunchKernelGGL((decode_kernel<D, T, F8, kSub, W, kWide, kWhole, kStream>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
+    hipLaunchKernelGGL((decode_kernel<D, T, E, kSub, W, kWide, kWhole, kStream>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,
                        a.n_rows, a.requests, a.max_len, a.window, a.shares, a.by_units.d, a.by_units.m, a.by_units.shift,
                        (uint32_t)(wgs / 8), (uint32_t)a.uncut, a);
     return hipGetLastError();
 }
 
-template <int D, class T, bool F8>
-hipError_t launch_f8(const DecodeArgs& a, hipStream_t s) {
-    if (a.whole) return launch_one<D, T, F8, true, true, false>(a, s);
+template <int D, class T, Elem E>
+hipError_t launch_dim(const ArgsOf<E>& a, hipStream_t s) {
+    if (a.whole) return launch_one<D, T, E, true, true, false>(a, s);
     if constexpr (D % 64 == 0)  // decode_streams takes no others
-        if (a.stream)
-            return a.wide ? launch_one<D, T, F8, true, false, true>(a, s) : launch_one<D, T, F8, false, false, true>(a, s);
-    return a.wide ? launch_one<D, T, F8, true, false, false>(a, s) : launch_one<D, T, F8, false, false, false>(a, s);
+        if (a.stream) return a.wide ? launch_one<D, T, E, true, false, true>(a, s) : launch_one<D, T, E, false, false, true>(a, s);
+    return a.wide ? launch_one<D, T, E, true, false, false>(a, s) : launch_one<D, T, E, false, false, false>(a, s);
 }
 
-template <int D, class T>
-hipError_t launch_dim(const DecodeArgs& a, bool f8, hipStream_t s) {
-    return f8 ? launch_f8<D, T, true>(a, s) : launch_f8<D, T, false>(a, s);
+template <class T, Elem E>
+hipError_t launch_elem(const ArgsOf<E>& a, int head_dim, hipStream_t s) {
+    switch (head_dim) {
+    case 64: return launch_dim<64, T, E>(a, s);
+    case 96: return launch_dim<96, T, E>(a, s);
+    case 128: return launch_dim<128, T, E>(a, s);
+    case 192: return launch_dim<192, T, E>(a, s);
+    case 256: return launch_dim<256, T, E>(a, s);
+    default: return hipErrorInvalidValue;
+    }
 }
 
 template <class T>
 hipError_t launch_type(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s) {
-    switch (head_dim) {
-    case 64: return launch_dim<64, T>(a, f8, s);
-    case 96: return launch_dim<96, T>(a, f8, s);
-    case 128: return launch_dim<128, T>(a, f8, s);
-    case 192: return launch_dim<192, T>(a, f8, s);
-    case 256: return launch_dim<256, T>(a, f8, s);
-    default: return hipErrorInvalidValue;
-    }
+    return f8 ? launch_elem<T, kF8>(a, head_dim, s) : launch_elem<T, kHalf>(a, head_dim, s);
 }
 
 }  // namespace attn

@@ -3,9 +3,10 @@
 #pragma once
 
 #include "attn_decode_shape.hpp"
+#include "attn_prompt_shape.hpp"
 #include "qmm_internal.hpp"
 
-#include "../../include/openmini_attn.h"
+#include "../../include/openmini_kv_i8.h"
 
 namespace attn {
 
@@ -34,6 +35,13 @@ struct Cache {
     uint32_t n_pages, slots;  // slots = n_pages * page_size
     FastDiv page;
     float k_scale, v_scale;
+};
+
+// The scales of a cache of 8-bit integers: strides in elements, tokens to a block 2^shift.
+struct Scales {
+    float *k, *v;
+    int64_t page_stride, block_stride, head_stride;
+    uint32_t shift;
 };
 
 // ---- attn_plan.hip -------------------------------------------------------------------
@@ -83,6 +91,34 @@ struct RopeArgs {
     FastDiv per_token, per_head, by_pairs;  // items of a token and of a head; n_pairs
 };
 hipError_t launch_rope(const RopeArgs& a, int head_dim, hipStream_t s);
+
+// ---- attn_append_i8.hip --------------------------------------------------------------
+constexpr int kMaxI8Dim = 256;  // head_dim
+
+struct AppendI8Args {
+    RopeArgs r;  // per_token: items of q alone
+    Scales scales;
+    FastDiv by_slices;             // of a q token's items
+    uint32_t kv_wgs, q_groups;     // workgroups for k and v, in front; groups of q tokens
+    uint32_t chunk, wg_heads;      // tokens whose runs a workgroup takes, of wg_heads heads
+    FastDiv by_head_groups;
+};
+hipError_t launch_append_i8(AppendI8Args& a, int head_dim, hipStream_t s);
+
+// ---- attn_read.hip -------------------------------------------------------------------
+struct ReadArgs {
+    Cache cache;
+    Scales scales;
+    const int32_t *tables, *starts, *first;
+    int64_t table_stride;
+    uint32_t requests, max_len;
+    int64_t tokens;
+    uint8_t *k_out, *v_out;
+    int64_t k_stride, v_stride;  // bytes
+    int32_t kv_heads, out_dtype, cache_dtype;
+    FastDiv per_head, per_token;  // items of a head, and of a token
+};
+hipError_t launch_read(const ReadArgs& a, hipStream_t s);
 
 // ---- attn_decode_*.hip ---------------------------------------------------------------
 // Whether a call reads keys and values past the caches (loads marked as not used again),
@@ -136,6 +172,10 @@ struct DecodeArgs {
     int32_t stream;  // keys and values are read past the caches
 };
 
+struct DecodeI8Args : DecodeArgs {
+    Scales scales;
+};
+
 // log(sum of exponentials) from a base in powers of two and the sum above it, whose exponent
 // joins the base first (fp16's sums are 2^15 up: the two nearly cancel).
 __device__ __forceinline__ float log_sum(float m, float l) {
@@ -151,5 +191,32 @@ hipError_t launch_join(const DecodeArgs& a, int head_dim, int out_dtype, hipStre
 
 hipError_t launch_decode_bf16(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s);
 hipError_t launch_decode_f16(const DecodeArgs& a, int head_dim, bool f8, hipStream_t s);
+hipError_t launch_decode_i8_bf16(const DecodeI8Args& a, int head_dim, hipStream_t s);
+hipError_t launch_decode_i8_f16(const DecodeI8Args& a, int head_dim, hipStream_t s);
+
+// ---- attn_prompt_*.hip ---------------------------------------------------------------
+struct PromptArgs {
+    Cache cache;
+    Scales scales;
+    const uint8_t* q;
+    uint8_t* out;
+    float* lse;
+    const int32_t *lens, *starts, *tables;
+    int64_t q_stride, out_stride;  // bytes
+    int64_t table_stride;
+    uint32_t rows, requests, max_len, window;
+    int32_t q_heads, group;
+    FastDiv by_tokens, by_heads;      // query tokens and heads of a tile
+    FastDiv by_units, by_head_tiles;  // units: key heads times tiles of their query heads
+    int32_t negative;  // the scale's sign
+    float scale;       // its magnitude, times k_scale and log2(e)
+    uint32_t tiles;    // of query tokens, at most
+    uint32_t splits;   // workgroups that share a tile's keys
+    float* part_acc;   // [tiles * units][splits][tile rows][head_dim]
+    float2* part_ml;   // [tiles * units][splits][tile rows]
+};
+hipError_t launch_prompt_bf16(const PromptArgs& a, int head_dim, int cache_dtype, bool out_f32, hipStream_t s);
+hipError_t launch_prompt_f16(const PromptArgs& a, int head_dim, int cache_dtype, bool out_f32, hipStream_t s);
+hipError_t launch_prompt_join(const PromptArgs& a, int head_dim, int out_dtype, hipStream_t s);
 
 }  // namespace attn

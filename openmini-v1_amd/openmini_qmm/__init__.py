@@ -2,11 +2,11 @@
 attention step between its projections.
 
 The compute path is libopenmini_qmm.so (hand-written HIP, C-ABI in
-include/openmini_qmm.h and include/openmini_attn.h); this package is its host-side mirror of the reference's
+include/openmini_qmm.h, include/openmini_attn.h and include/openmini_kv_i8.h); this package is its host-side mirror of the reference's
 operator interface (see ops.py) plus synthetic-input helpers (synth.py).
 """
 from ._native import LIB_PATH, Q4_0, Q8_0, QmmError, lib  # noqa: F401
-from .attention import (DType, KVCache, PagedAttention, Rope, StepPlan, rope_axes,  # noqa: F401
+from .attention import (DType, KVCache, PagedAttention, PromptAttention, Rope, StepPlan, rope_axes,  # noqa: F401
                         rope_frequencies)
 from .layer import (AttentionWeights, CachedAttention, FFNWeights, ffn_gate_up, ffn_gate_up_bf16,  # noqa: F401
                     ffn_gate_up_f32, gemv_multi)

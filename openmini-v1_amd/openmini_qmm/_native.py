@@ -1,5 +1,5 @@
-"""ctypes binding of libopenmini_qmm.so (C-ABI in include/openmini_qmm.h and
-include/openmini_attn.h).
+"""ctypes binding of libopenmini_qmm.so (C-ABI in include/openmini_qmm.h,
+include/openmini_attn.h and include/openmini_kv_i8.h).
 
 The library is the only compute path: if it is missing this module raises, there
 is no CPU fallback.  Build it with `python openmini-v1_amd/build.py`.
@@ -191,6 +191,38 @@ ATTN_SIGNATURES = {
     "openmini_attn_decode": (_i, [ctypes.POINTER(KvCache), ctypes.POINTER(AttnArgs), _p]),
 }
 
+
+class KvScales(ctypes.Structure):  # openmini_kv_scales_t
+    _fields_ = [
+        ("d_k", _p), ("d_v", _p), ("block", ctypes.c_int32), ("page_stride", _i64), ("block_stride", _i64), ("head_stride", _i64),
+    ]
+
+
+class KvReadArgs(ctypes.Structure):  # openmini_kv_read_args_t
+    _fields_ = [
+        ("d_tables", _p), ("table_stride", _i64), ("max_pages", _i64), ("requests", _i64), ("d_starts", _p), ("d_first", _p),
+        ("tokens", _i64), ("d_k_out", _p), ("d_v_out", _p), ("k_stride", _i64), ("v_stride", _i64), ("out_dtype", ctypes.c_int32),
+    ]
+
+
+class PromptArgs(ctypes.Structure):  # openmini_attn_prompt_args_t
+    _fields_ = [
+        ("d_q", _p), ("q_stride", _i64), ("d_out", _p), ("out_stride", _i64), ("d_lse", _p), ("q_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("scale", ctypes.c_float), ("window", _i64),
+        ("rows", _i64), ("d_lens", _p), ("d_starts", _p), ("d_tables", _p), ("table_stride", _i64), ("max_pages", _i64),
+        ("requests", _i64), ("d_work", _p), ("work_bytes", _sz),
+    ]
+
+
+# name -> (restype, argtypes); mirrors include/openmini_kv_i8.h one to one.
+KV_I8_SIGNATURES = {
+    "openmini_rope_append_i8": (_i, [_p, ctypes.POINTER(KvCache), ctypes.POINTER(KvScales), ctypes.POINTER(RopeAppendArgs), _p]),
+    "openmini_attn_decode_i8": (_i, [ctypes.POINTER(KvCache), ctypes.POINTER(KvScales), ctypes.POINTER(AttnArgs), _p]),
+    "openmini_kv_read": (_i, [ctypes.POINTER(KvCache), ctypes.POINTER(KvScales), ctypes.POINTER(KvReadArgs), _p]),
+    "openmini_attn_prompt_workspace_bytes": (_sz, [_i, _i, _i]),
+    "openmini_attn_prompt": (_i, [ctypes.POINTER(KvCache), ctypes.POINTER(KvScales), ctypes.POINTER(PromptArgs), _p]),
+}
+
 _lib = None
 
 
@@ -203,7 +235,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python openmini-v1_amd/build.py` "
                 "(the HIP library is the only compute path)")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in (*SIGNATURES.items(), *ATTN_SIGNATURES.items()):
+        for name, (res, args) in (*SIGNATURES.items(), *ATTN_SIGNATURES.items(), *KV_I8_SIGNATURES.items()):
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

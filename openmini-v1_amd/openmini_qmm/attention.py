@@ -1,11 +1,13 @@
 """The attention step between a layer's q / k / v projections and its output projection,
-over include/openmini_attn.h:
+over include/openmini_attn.h and include/openmini_kv_i8.h:
 
   StepPlan         pages and slots for a step's tokens, on the GPU (openmini_kv_plan)
-  KVCache          one layer's paged keys and values
+  KVCache          one layer's paged keys and values, in 16 bits, e4m3, or 8-bit integers with a
+                   scale for each block of tokens and head; read() brings tokens back out
   Rope             rotary positions with one or more axes: apply() on a dense tensor,
                    append() on a step's q and k with the cache write
   PagedAttention   attention of single query tokens over the cache (openmini_attn_decode)
+  PromptAttention  attention of runs of query tokens over the cache (openmini_attn_prompt)
 
 Buffers are DeviceBuffer or anything with `ptr` (c_void_p) and `nbytes`; calls only enqueue
 work on `stream` (None: the null stream).  Sizes that do not fit their buffers raise
@@ -27,11 +29,12 @@ class DType(enum.IntEnum):
     F16 = 1
     BF16 = 2
     F8_E4M3 = 3
+    I8 = 4  # OPENMINI_ATTN_I8: caches only
 
     @classmethod
     def of(cls, name: str) -> "DType":
-        """From "f32", "f16", "bf16" or "f8"."""
-        return {"f32": cls.F32, "f16": cls.F16, "bf16": cls.BF16, "f8": cls.F8_E4M3}[name]
+        """From "f32", "f16", "bf16", "f8" or "i8"."""
+        return {"f32": cls.F32, "f16": cls.F16, "bf16": cls.BF16, "f8": cls.F8_E4M3, "i8": cls.I8}[name]
 
     @property
     def nbytes(self) -> int:
@@ -40,7 +43,7 @@ class DType(enum.IntEnum):
 
 # Calls build their argument structure and compare sizes in line: a step's smallest launches
 # take 3 - 4 us, which a helper call for each buffer would add half of.
-_NBYTES = (4, 2, 2, 1)  # of a DType
+_NBYTES = (4, 2, 2, 1, 1)  # of a DType
 
 
 def _short(what: str, buf, nbytes: int):
@@ -57,10 +60,15 @@ class KVCache:
     """Keys and values of one layer in pages of page_size tokens, in buffers of the caller
     (one type; layout "token": [n_pages][page_size][kv_heads][head_dim], "head":
     [n_pages][kv_heads][page_size][head_dim]).  A stored element stands for itself times
-    k_scale (v_scale)."""
+    k_scale (v_scale).
+
+    DType.I8: codes of -127 to 127, each times its block's scale: `block` tokens (8, 16 or 32) of
+    one head have one, fp32 in d_k_scales and d_v_scales ("token": [n_pages][page_size /
+    block][kv_heads], "head": [n_pages][kv_heads][page_size / block])."""
 
     def __init__(self, d_k, d_v, dtype: DType, n_pages: int, page_size: int, kv_heads: int, head_dim: int,
-                 layout: str = "token", k_scale: float = 1.0, v_scale: float = 1.0):
+                 layout: str = "token", k_scale: float = 1.0, v_scale: float = 1.0, block: int = 0, d_k_scales=None,
+                 d_v_scales=None):
         if layout not in ("token", "head"):
             raise InvalidInput(f"layout {layout!r} is neither 'token' nor 'head'")
         dtype = DType(dtype)
@@ -74,11 +82,55 @@ class KVCache:
         token, head = (kv_heads * head_dim, head_dim) if layout == "token" else (head_dim, page_size * head_dim)
         self.desc = _native.KvCache(d_k.ptr, d_v.ptr, dtype, kv_heads, head_dim, page_size, n_pages,
                                     page_size * kv_heads * head_dim, token, head, k_scale, v_scale)
+        self.block, self.d_k_scales, self.d_v_scales, self.scales = int(block), d_k_scales, d_v_scales, None
+        if dtype != DType.I8:
+            if block or d_k_scales is not None or d_v_scales is not None:
+                raise InvalidInput(f"blocks with scales in a cache of {dtype.name}")
+        else:
+            each = _blocks(page_size, block)
+            if d_k_scales is None or d_v_scales is None:
+                raise InvalidInput("a cache of I8 needs d_k_scales and d_v_scales")
+            for name, buf in (("d_k_scales", d_k_scales), ("d_v_scales", d_v_scales)):
+                if buf.nbytes < 4 * n_pages * each * kv_heads:
+                    _short(name, buf, 4 * n_pages * each * kv_heads)
+            of_block, of_head = (kv_heads, 1) if layout == "token" else (1, each)
+            self.scales = _native.KvScales(d_k_scales.ptr, d_v_scales.ptr, block, each * kv_heads, of_block, of_head)
 
     @classmethod
-    def allocate(cls, dtype: DType, n_pages: int, page_size: int, kv_heads: int, head_dim: int, **kw) -> "KVCache":
+    def allocate(cls, dtype: DType, n_pages: int, page_size: int, kv_heads: int, head_dim: int, block: int = 16, **kw) -> "KVCache":
+        """With buffers of its own (`block`: of DType.I8)."""
         nbytes = n_pages * page_size * kv_heads * head_dim * DType(dtype).nbytes
+        if dtype == DType.I8:
+            scales = 4 * n_pages * _blocks(page_size, block) * kv_heads
+            kw.update(block=block, d_k_scales=DeviceBuffer(scales), d_v_scales=DeviceBuffer(scales))
         return cls(DeviceBuffer(nbytes), DeviceBuffer(nbytes), dtype, n_pages, page_size, kv_heads, head_dim, **kw)
+
+    def read(self, d_tables, max_pages: int, d_starts, requests: int, tokens: int, d_k_out, d_v_out, out_dtype: DType,
+             d_first=None, stream=None, table_stride: int | None = None, k_stride: int | None = None,
+             v_stride: int | None = None) -> None:
+        """Rows d_starts[r] to d_starts[r + 1] - 1 of d_k_out and d_v_out [tokens][kv_heads][head_dim]
+        (either may be None) are request r's tokens from d_first[r] on (None: from the first)."""
+        row = self.kv_heads * self.head_dim
+        ts = max_pages if table_stride is None else table_stride
+        ks, vs = row if k_stride is None else k_stride, row if v_stride is None else v_stride
+        if d_tables.nbytes < 4 * _rows_bytes(requests, ts, max_pages, 1):
+            _short("d_tables", d_tables, 4 * _rows_bytes(requests, ts, max_pages, 1))
+        if d_starts.nbytes < 4 * (requests + 1):
+            _short("d_starts", d_starts, 4 * (requests + 1))
+        if d_first is not None and d_first.nbytes < 4 * requests:
+            _short("d_first", d_first, 4 * requests)
+        for name, buf, stride in (("d_k_out", d_k_out, ks), ("d_v_out", d_v_out, vs)):
+            if buf is not None and buf.nbytes < _rows_bytes(tokens, stride, row, _NBYTES[out_dtype]):
+                _short(name, buf, _rows_bytes(tokens, stride, row, _NBYTES[out_dtype]))
+        check(lib().openmini_kv_read(self.desc, self.scales, _native.KvReadArgs(
+            d_tables.ptr, ts, max_pages, requests, d_starts.ptr, d_first.ptr if d_first is not None else None, tokens,
+            d_k_out.ptr if d_k_out is not None else None, d_v_out.ptr if d_v_out is not None else None, ks, vs, out_dtype), stream))
+
+
+def _blocks(page_size: int, block: int) -> int:
+    if block <= 0 or page_size % block:
+        raise InvalidInput(f"pages of {page_size} tokens do not hold whole blocks of {block}")
+    return page_size // block
 
 
 # ---- pages and slots -------------------------------------------------------------------
@@ -174,6 +226,7 @@ class Rope:
         check(lib().openmini_rope_create(freq, axis, self.pairs, self.n_axes, int(pairing == "adjacent"), scale,
                                          ctypes.byref(self.handle)))
         self._apply, self._append = lib().openmini_rope_apply, lib().openmini_rope_append
+        self._append_i8 = lib().openmini_rope_append_i8
 
     def apply(self, d_x, x_dtype: DType, d_y, y_dtype: DType, d_positions, tokens: int, heads: int, head_dim: int,
               inverse: bool = False, stream=None, x_stride: int | None = None, y_stride: int | None = None,
@@ -201,7 +254,8 @@ class Rope:
                q_heads: int, stream=None, q_stride: int | None = None, k_stride: int | None = None,
                v_stride: int | None = None, position_stride: int | None = None) -> None:
         """A step of a layer: d_q_out [tokens][q_heads][head_dim] = q turned; k turned and v
-        as it is go to the tokens' slots of the cache (negative: nowhere)."""
+        as it is go to the tokens' slots of the cache (negative: nowhere), into a cache of I8
+        with its blocks' scales (openmini_rope_append_i8)."""
         q_row, kv_row = q_heads * cache.head_dim, cache.kv_heads * cache.head_dim
         qs = q_row if q_stride is None else q_stride
         ks, vs = kv_row if k_stride is None else k_stride, kv_row if v_stride is None else v_stride
@@ -224,9 +278,12 @@ class Rope:
             _short("d_positions", d_positions, n)
         if d_slots.nbytes < 4 * tokens:
             _short("d_slots", d_slots, 4 * tokens)
-        rc = self._append(self.handle, cache.desc, _native.RopeAppendArgs(
-            d_q.ptr, d_k.ptr, d_v.ptr, qs, ks, vs, d_q_out.ptr, q_row, in_dtype, q_dtype, tokens, q_heads, d_positions.ptr, ps,
-            d_slots.ptr), stream)
+        args = _native.RopeAppendArgs(d_q.ptr, d_k.ptr, d_v.ptr, qs, ks, vs, d_q_out.ptr, q_row, in_dtype, q_dtype, tokens, q_heads,
+                                      d_positions.ptr, ps, d_slots.ptr)
+        if cache.scales is None:
+            rc = self._append(self.handle, cache.desc, args, stream)
+        else:
+            rc = self._append_i8(self.handle, cache.desc, cache.scales, args, stream)
         if rc:
             check(rc)
 
@@ -259,7 +316,7 @@ class PagedAttention:
         if not nbytes:
             raise InvalidInput(f"no attention of {q_heads} query heads on {kv_heads} key heads of {head_dim}")
         self.work = DeviceBuffer(nbytes)
-        self._call = lib().openmini_attn_decode
+        self._call, self._call_i8 = lib().openmini_attn_decode, lib().openmini_attn_decode_i8
 
     def run(self, cache: KVCache, d_q, d_out, d_tables, max_pages: int, d_lens, rows: int, d_rows=None,
             requests: int | None = None, d_lse=None, stream=None, table_stride: int | None = None,
@@ -294,12 +351,59 @@ class PagedAttention:
         n = 4 * _rows_bytes(requests, ts, max_pages, 1)
         if d_tables.nbytes < n:
             _short("d_tables", d_tables, n)
-        rc = self._call(cache.desc, _native.AttnArgs(
+        args = _native.AttnArgs(
             d_q.ptr, qs, d_out.ptr, os_, d_lse.ptr if d_lse is not None else None, self.q_dtype, self.out_dtype, self.q_heads,
             self.scale, self.window, rows, d_lens.ptr, d_rows.ptr if d_rows is not None else None, d_tables.ptr, ts, max_pages,
-            max(requests, 1), self.work.ptr, self.work.nbytes), stream)
+            max(requests, 1), self.work.ptr, self.work.nbytes)
+        rc = self._call(cache.desc, args, stream) if cache.scales is None else self._call_i8(cache.desc, cache.scales, args, stream)
         if rc:
             check(rc)
 
 
-__all__ = ["DType", "KVCache", "PagedAttention", "Rope", "StepPlan", "rope_axes", "rope_frequencies"]
+class PromptAttention:
+    """Attention of runs of query tokens, a prompt's or a piece of one, over a paged cache of any
+    type (openmini_attn_prompt), with the workspace that its calls take turns with: one object
+    for calls that follow each other.  out_dtype None: q_dtype (F32 costs two more products of
+    probabilities and values, on F16 caches one or three).  scale None: 1 / sqrt(head_dim).
+    window > 0: each row sees its last `window` keys."""
+
+    def __init__(self, q_heads: int, kv_heads: int, head_dim: int, q_dtype: DType = DType.BF16, out_dtype: DType | None = None,
+                 scale: float | None = None, window: int = 0):
+        self.q_heads, self.kv_heads, self.head_dim = int(q_heads), int(kv_heads), int(head_dim)
+        self.q_dtype = DType(q_dtype)
+        self.out_dtype = self.q_dtype if out_dtype is None else DType(out_dtype)
+        self.scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        self.window = int(window)
+        nbytes = lib().openmini_attn_prompt_workspace_bytes(self.q_heads, self.kv_heads, self.head_dim)
+        if not nbytes:
+            raise InvalidInput(f"no attention of {q_heads} query heads on {kv_heads} key heads of {head_dim}")
+        self.work = DeviceBuffer(nbytes)
+        self._call = lib().openmini_attn_prompt
+
+    def run(self, cache: KVCache, d_q, d_out, d_tables, max_pages: int, d_starts, d_lens, rows: int, requests: int, d_lse=None,
+            stream=None, table_stride: int | None = None, q_stride: int | None = None, out_stride: int | None = None) -> None:
+        """d_out [rows][q_heads][head_dim]: rows d_starts[r] to d_starts[r + 1] - 1 belong to request r
+        (the others are left as they were) and row j attends to its first d_lens[j] keys, whose pages
+        are d_tables[r][:max_pages] (StepPlan's starts and row_lens); d_lse [rows][q_heads] fp32, the
+        log of the sum of exponentials."""
+        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
+            raise InvalidInput(f"cache of {cache.kv_heads} heads of {cache.head_dim}, expected {self.kv_heads} of {self.head_dim}")
+        row = self.q_heads * self.head_dim
+        qs, os_ = row if q_stride is None else q_stride, row if out_stride is None else out_stride
+        ts = max_pages if table_stride is None else table_stride
+        for name, buf, n in (("d_q", d_q, _rows_bytes(rows, qs, row, 2)), ("d_out", d_out, _rows_bytes(rows, os_, row, _NBYTES[self.out_dtype])),
+                             ("d_lens", d_lens, 4 * rows), ("d_starts", d_starts, 4 * (requests + 1)),
+                             ("d_tables", d_tables, 4 * _rows_bytes(requests, ts, max_pages, 1))):
+            if buf.nbytes < n:
+                _short(name, buf, n)
+        if d_lse is not None and d_lse.nbytes < 4 * rows * self.q_heads:
+            _short("d_lse", d_lse, 4 * rows * self.q_heads)
+        rc = self._call(cache.desc, cache.scales, _native.PromptArgs(
+            d_q.ptr, qs, d_out.ptr, os_, d_lse.ptr if d_lse is not None else None, self.q_dtype, self.out_dtype, self.q_heads,
+            self.scale, self.window, rows, d_lens.ptr, d_starts.ptr, d_tables.ptr, ts, max_pages, requests, self.work.ptr,
+            self.work.nbytes), stream)
+        if rc:
+            check(rc)
+
+
+__all__ = ["DType", "KVCache", "PagedAttention", "PromptAttention", "Rope", "StepPlan", "rope_axes", "rope_frequencies"]

@@ -5,6 +5,7 @@ pub mod attn_ffi;
 pub mod engine;
 pub mod ffi;
 pub mod gpu_quant_ops;
+pub mod kv_i8_ffi;
 pub mod layer;
 pub mod loader;
 
