@@ -23,7 +23,7 @@ import ctypes
 import numpy as np
 
 from ._native import check, lib
-from .attention import DType, KVCache, PagedAttention, Rope, StepPlan
+from .attention import DType, KVCache, PagedAttention, PromptAttention, Rope, StepPlan
 from .ops import DeviceBuffer, InvalidInput, QuantizedWeight, gemm_f32_workspace
 
 MAX_GROUP = 4  # weights per gemv_multi launch
@@ -175,17 +175,25 @@ class AttentionWeights:
         return d_o.download(np.float32, (m, self.o_proj.n_rows))
 
 
+class _From:
+    """A buffer from some byte on."""
+
+    def __init__(self, buf, offset: int):
+        self.ptr, self.nbytes = ctypes.c_void_p(buf.ptr.value + offset), buf.nbytes - offset
+
+
 class CachedAttention:
     """One layer's attention over its paged cache: the q / k / v projections, rotary
     positions and the cache write, attention, and the output projection,
-    for any mix of decoding requests and short prompts (a prompt's tokens are rows of their
-    own, each seeing the keys up to its position).
+    for any mix of decoding requests and prompts.  A prompt's tokens see the keys up to their
+    position each; as rows of their own, or with a `prompt` attention as a run that reads the
+    keys once (forward_device's `decoding`).
 
-    `attention` may be shared by layers that run one after the other; buffers for up to
-    max_tokens rows are allocated here."""
+    `attention` and `prompt` may be shared by layers that run one after the other; buffers for
+    up to max_tokens rows are allocated here."""
 
     def __init__(self, weights: AttentionWeights, rope: Rope, cache: KVCache, q_heads: int, max_tokens: int,
-                 q_dtype: DType = DType.BF16, attention: PagedAttention | None = None):
+                 q_dtype: DType = DType.BF16, attention: PagedAttention | None = None, prompt: PromptAttention | None = None):
         head_dim = cache.head_dim
         if weights.o_proj is None:
             raise InvalidInput("no o_proj")
@@ -195,6 +203,7 @@ class CachedAttention:
         self.weights, self.rope, self.cache = weights, rope, cache
         self.q_heads, self.max_tokens, self.q_dtype = int(q_heads), int(max_tokens), DType(q_dtype)
         self.attention = attention or PagedAttention(q_heads, cache.kv_heads, head_dim, q_dtype, DType.F32)
+        self.prompt = prompt
         q, kv = q_heads * head_dim, cache.kv_heads * head_dim
         self.d_q, self.d_k, self.d_v = (DeviceBuffer(max_tokens * n * 4) for n in (q, kv, kv))
         self.d_q16, self.d_attn = DeviceBuffer(max_tokens * q * 2), DeviceBuffer(max_tokens * q * 4)
@@ -205,21 +214,36 @@ class CachedAttention:
 
     @attention.setter
     def attention(self, shared: PagedAttention) -> None:
+        self._check(shared)
+        self._attention = shared
+
+    @property
+    def prompt(self) -> PromptAttention | None:
+        return self._prompt
+
+    @prompt.setter
+    def prompt(self, shared: PromptAttention | None) -> None:
+        if shared is not None:
+            self._check(shared)
+        self._prompt = shared
+
+    def _check(self, shared) -> None:
         if shared.q_dtype != self.q_dtype or shared.out_dtype != DType.F32:
             raise InvalidInput("the shared attention has other types")
         theirs, ours = (shared.q_heads, shared.kv_heads, shared.head_dim), (self.q_heads, self.cache.kv_heads, self.cache.head_dim)
         if theirs != ours:
             raise InvalidInput(f"the shared attention has heads {theirs}, the layer {ours}")
-        self._attention = shared
 
     def forward_device(self, d_x: DeviceBuffer, plan: StepPlan, d_tables, requests: int, tokens: int, d_out: DeviceBuffer,
-                       d_positions=None, stream=None, max_pages: int | None = None) -> None:
+                       d_positions=None, stream=None, max_pages: int | None = None, decoding: int | None = None) -> None:
         """d_out [tokens, hidden] for the step that `plan` laid out (plan.run on the same
         stream before the first layer): d_x [tokens, hidden] fp32, d_tables the tables that
         the plan filled.  d_positions [axes][tokens]: None takes the plan's, for a rope of one
         axis (of several, text too has its position on each).
         max_pages: columns that the step's longest request needs, where that is known (None:
-        the tables' width); attention of short rows is faster for it."""
+        the tables' width); attention of short rows is faster for it.
+        decoding: the first `decoding` requests of the step add one token each, the others runs,
+        which `prompt` attends to (None: every token is a row of decode attention)."""
         most = plan.max_pages if max_pages is None else int(max_pages)
         if not 0 < most <= plan.max_pages:
             raise InvalidInput(f"max_pages {most}, tables of {plan.max_pages}")
@@ -232,12 +256,26 @@ class CachedAttention:
                 raise InvalidInput(f"{name} holds {buf.nbytes} bytes, {4 * tokens * columns} are needed")
         if d_positions is None and self.rope.n_axes > 1:
             raise InvalidInput(f"the plan's positions are for one axis, the rope has {self.rope.n_axes}")
+        rows = tokens
+        if decoding is not None:
+            if self.prompt is None:
+                raise InvalidInput("runs need a prompt attention")
+            if not 0 <= decoding <= min(requests, tokens) or (decoding == requests and decoding < tokens):
+                raise InvalidInput(f"{decoding} decoding requests of {requests}, {tokens} tokens")
+            if (self.prompt.window, self.prompt.scale) != (self.attention.window, self.attention.scale):
+                raise InvalidInput("the attentions of rows and of runs differ in window or scale")
+            rows = decoding
         w = self.weights
         w.project_qkv_device(d_x, self.d_q, self.d_k, self.d_v, tokens, stream)
         self.rope.append(self.cache, self.d_q, self.d_k, self.d_v, DType.F32, self.d_q16, self.q_dtype,
                          plan.positions if d_positions is None else d_positions, plan.slots, tokens, self.q_heads, stream)
-        self.attention.run(self.cache, self.d_q16, self.d_attn, d_tables, most, plan.row_lens, tokens,
-                           d_rows=plan.rows, requests=requests, table_stride=plan.max_pages, stream=stream)
+        if rows:
+            self.attention.run(self.cache, self.d_q16, self.d_attn, d_tables, most, plan.row_lens, rows,
+                               d_rows=plan.rows, requests=requests, table_stride=plan.max_pages, stream=stream)
+        if rows < tokens:
+            self.prompt.run(self.cache, self.d_q16, self.d_attn, _From(d_tables, 4 * rows * plan.max_pages), most,
+                            _From(plan.starts, 4 * rows), plan.row_lens, tokens, requests - rows, table_stride=plan.max_pages,
+                            stream=stream)
         w.o_proj.gemv(self.d_attn, d_out, tokens, stream)
 
 
