@@ -103,8 +103,8 @@ int openmini_kv_read(const openmini_kv_cache_t* cache, const openmini_kv_scales_
  * Types: q F16 or BF16; the cache of q's type (`scales` NULL), F8_E4M3 (NULL) or I8; out q's
  * type or F32.  Products are of 16-bit operands with 32-bit sums.  With 16-bit outputs a
  * probability is rounded once to 16 bits: bf16 on BF16 caches; else fp16, which holds 11 bits of
- * it down to 2^-29 of a row's largest (values' scales included) and less below, nothing from
- * 2^-40 on.  With F32 outputs it enters as the sum of three bf16 parts, or on F16 caches as in
+ * it down to 2^-25 of a row's largest (values' scales included) and less below, nothing from
+ * 2^-36 on.  With F32 outputs it enters as the sum of three bf16 parts, or on F16 caches as in
  * openmini_attn_decode.  Sums, maxima and lse are fp32.  head_dim: 64, 96, 128, 192 or 256;
  * page_size: a multiple of 8; q_heads: a multiple of kv_heads, at most 1024; requests: at most
  * 2^20.  A scale of 8-bit values below 2^-60 counts as 2^-60.

@@ -9,20 +9,6 @@ namespace {
 constexpr int64_t kMaxRuns = (int64_t)1 << 20;
 constexpr int64_t kMaxThreads = (int64_t)UINT32_MAX;  // of a launch
 
-// A tile of openmini_attn_prompt for these heads: its query heads and tokens, and how many
-// tiles of heads a key head has.
-struct Tile {
-    int heads, tokens, head_tiles;
-};
-Tile tile_of(int group, int head_dim) {
-    const int rows = prompt_rows(head_dim);
-    Tile t;
-    t.head_tiles = (group + rows - 1) / rows;
-    t.heads = (group + t.head_tiles - 1) / t.head_tiles;
-    t.tokens = rows / t.heads;
-    return t;
-}
-
 bool prompt_sizes(int q_heads, int kv_heads, int head_dim) {
     return kv_heads >= 1 && q_heads >= kv_heads && q_heads <= 1024 && q_heads % kv_heads == 0 && decode_dim(head_dim);
 }
@@ -145,9 +131,10 @@ int openmini_attn_prompt(const openmini_kv_cache_t* cache, const openmini_kv_sca
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "workspace of %zu bytes, %zu are needed", p->work_bytes, need);
     const int64_t held = p->max_pages * cache->page_size, max_len = held < kMostKeys ? held : kMostKeys;
     a.group = p->q_heads / cache->kv_heads;
-    const Tile tile = tile_of(a.group, cache->head_dim);
-    const int64_t tiles = p->rows / tile.tokens + p->requests, units = (int64_t)cache->kv_heads * tile.head_tiles;
-    if (tiles * units * 64 * prompt_waves(cache->head_dim) > kMaxThreads)
+    // keys that a tile sees at most: all, or its rows' windows (a run's lengths rise by one)
+    const int64_t seen = p->window && p->window < max_len - 256 ? p->window + 256 : max_len;
+    const PromptShape shape = prompt_shape(cache->head_dim, p->rows, p->requests, cache->kv_heads, a.group, seen);
+    if (shape.wgs() * 64 * shape.waves > kMaxThreads)
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%lld rows of %lld requests are too many for one call", (long long)p->rows,
                     (long long)p->requests);
     TRY(qmm::current_device(nullptr));
@@ -165,15 +152,16 @@ int openmini_attn_prompt(const openmini_kv_cache_t* cache, const openmini_kv_sca
     a.max_len = (uint32_t)max_len;
     a.window = p->window && p->window < max_len ? (uint32_t)p->window : (uint32_t)max_len;
     a.q_heads = p->q_heads;
-    a.by_tokens = FastDiv((uint32_t)tile.tokens);
-    a.by_heads = FastDiv((uint32_t)tile.heads);
-    a.by_units = FastDiv((uint32_t)units);
-    a.by_head_tiles = FastDiv((uint32_t)tile.head_tiles);
+    a.by_tokens = FastDiv((uint32_t)shape.tokens);
+    a.by_heads = FastDiv((uint32_t)shape.heads);
+    a.by_units = FastDiv((uint32_t)shape.units);
+    a.by_head_tiles = FastDiv((uint32_t)shape.head_tiles);
     a.negative = scale < 0;
     // a score of -inf (a key that is not seen) stays one under a scale of zero
     a.scale = std::fmax(std::fabs(scale), 1e-37f);
-    a.tiles = (uint32_t)tiles;
-    a.splits = (uint32_t)prompt_splits(tiles * units, max_len < a.window + tile.tokens ? max_len : a.window + tile.tokens);
+    a.waves = shape.waves;
+    a.tiles = (uint32_t)shape.tiles;
+    a.splits = (uint32_t)shape.splits;
     a.part_ml = static_cast<float2*>(p->d_work);
     a.part_acc = reinterpret_cast<float*>(static_cast<uint8_t*>(p->d_work) + ml);
     const hipStream_t s = static_cast<hipStream_t>(stream);

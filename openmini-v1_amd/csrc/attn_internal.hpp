@@ -210,6 +210,7 @@ struct PromptArgs {
     FastDiv by_units, by_head_tiles;  // units: key heads times tiles of their query heads
     int32_t negative;  // the scale's sign
     float scale;       // its magnitude, times k_scale and log2(e)
+    int32_t waves;     // of a workgroup, 32 rows each
     uint32_t tiles;    // of query tokens, at most
     uint32_t splits;   // workgroups that share a tile's keys
     float* part_acc;   // [tiles * units][splits][tile rows][head_dim]

@@ -12,15 +12,25 @@
 // neighbours to each operand, which share a block and its scale.
 //
 // V lies in LDS transposed, [dimension][key]: a thread brings four keys of four dimensions and
-// transposes them by byte permutations on the way.  Both arrays are swizzled so that the eight
-// lanes of an LDS access fall on different banks.
+// transposes them by byte permutations on the way.
 //
 // 8-bit integers are exact in 16 bits; their blocks' scales act on 32-bit numbers: a key's on
 // the score, a value's as its logarithm in the exponent, so that p v_scale is what is rounded
 // to 16 bits (at most 1, whatever the scales) and l adds p v_scale / v_scale.
 //
-// The loads of a step are issued a step ahead of their use and its pages two; two buffers,
-// one barrier a step.  Bound by the matrix rate for long prompts.
+// The loads of a step are issued more than a step ahead of their use and its page three; two buffers,
+// one barrier a step.  What comes goes to LDS beside the matrix instructions of the first product.
+// Accumulators are scaled only where a maximum has grown by 2^4: with 32 rows to a wave one of them
+// grows in most steps.
+//
+// Bound by the issue of instructions: a step of 64 keys takes a wave 2 us, alone on its SIMD or with
+// another, of which the matrix unit is busy for .4 (heads of 128); matrix and vector instructions of
+// the two waves run at the same time for two fifths of that only.  Measured (MI355X): 8191 tokens of
+// 64 / 8 heads of 128 1130 to 1180 us, 930 to 976 TFLOP/s (a large product of the library 1350); 4096
+// tokens of 32 / 8 heads of 64, 96, 128, 192, 256 150, 165, 165, 535, 525 us, on a bf16 cache of 128 174.
+// Of 192 and 256 a SIMD holds one wave.  What gave nothing or less: a second product a step later, for
+// half of the waves or among the exponentials (1.24, 1.47 ms of 1.26), wave priorities, 128 keys
+// a step, three waves a SIMD of 32 keys a step (1.31 of 1.18), rows out through LDS.
 #pragma once
 
 #include "attn_decode.hpp"
@@ -54,8 +64,8 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t u) {
     return ((u & kAll) == kAll ? 0xFFFFu : 0u) | ((u >> 16 & kAll) == kAll ? 0xFFFF0000u : 0u);
 }
 
-// A tile's place: slot t of the call's tiles; run r has those from starts[r] / tokens + r on, at
-// least as many as it needs.
+// A tile's place: slot t of the call's tiles; of n tokens each, run r has those from
+// (starts[r] + r (n - 1)) / n on, at least as many as it needs.
 struct PromptTile {
     uint32_t run, token0, tokens;  // tokens: 0 for a slot that no run needs
     uint32_t kv, head0, heads;     // its key head, its first query head, its heads
@@ -65,7 +75,7 @@ __device__ __forceinline__ PromptTile prompt_tile(const int32_t* starts, uint32_
     auto start = [&](uint32_t r) { return min((uint32_t)max(starts[r], 0), rows); };
     PromptTile t;
     t.tokens = 0;
-    t.run = find_run(requests, slot, [&](uint32_t r) { return by_tokens.div(start(r)) + r; });
+    t.run = find_run(requests, slot, [&](uint32_t r) { return by_tokens.div(start(r) + r * (by_tokens.d - 1)); });
     t.kv = by_head_tiles.div(unit);
     const uint32_t part = (unit - t.kv * by_head_tiles.d) * by_heads.d;
     t.head0 = t.kv * (uint32_t)group + part;
@@ -73,29 +83,33 @@ __device__ __forceinline__ PromptTile prompt_tile(const int32_t* starts, uint32_
     t.token0 = 0;
     if (t.run >= requests) return t;
     const uint32_t first = start(t.run), end = start(t.run + 1);
-    const uint64_t at = first + (uint64_t)(slot - by_tokens.div(first) - t.run) * by_tokens.d;
+    const uint64_t at = first + (uint64_t)(slot - by_tokens.div(first + t.run * (by_tokens.d - 1))) * by_tokens.d;
     if (at >= end) return t;
     t.token0 = (uint32_t)at;
     t.tokens = min(by_tokens.d, end - t.token0);
     return t;
 }
 
-template <int D, class T, Elem E, bool kF32>
-__global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt_kernel(PromptArgs a) {
+template <int D, class T, Elem E, bool kF32, int W>
+__global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(PromptArgs a) {
     // of the second product: byte caches fit both types, fp16 has the finer step and bf16 the
     // range that exact parts need
     using P = std::conditional_t<E == kHalf, T, std::conditional_t<kF32, BF16, F16>>;
     constexpr int kParts = kF32 ? P::kExactParts : 1;
     constexpr bool kLow = kF32 && P::kNarrow;  // as in decode attention: what two fp16 parts leave
-    constexpr int W = prompt_waves(D), kThreads = 64 * W, kKeys = prompt_keys(D), kSub = kKeys / 32;
+    constexpr int kThreads = 64 * W, kKeys = prompt_keys(D), kSub = kKeys / 32;
     constexpr int kEl = E == kHalf ? 2 : 1;
     constexpr int kSteps = D / 16, kTiles = D / 32;
-    constexpr int kKRow = (D / 8 + 7) / 8 * 128, kVRow = kKeys * 2;  // bytes of a row in LDS
-    constexpr int kKPieces = kKeys * D * kEl / 16, kKLoads = (kKPieces + kThreads - 1) / kThreads;
-    constexpr int kVUnits = kKeys / 4 * (D / 4), kVLoads = (kVUnits + kThreads - 1) / kThreads;
+    // bytes of a row in LDS: 16 more than its elements, so that the eight lanes of an access, each at
+    // its row, fall on different banks, and all of a lane's reads are at fixed distances
+    constexpr int kKRow = D * 2 + 16, kVRow = kKeys * 2 + 16;
+    constexpr int kKLoads = (8 * D * kEl / 16 + 63) / 64, kVLoads = (D / 2 + 63) / 64;
     constexpr int kGroups = kKeys / 8;
+    constexpr int kOwn = kGroups / W;  // groups that a wave brings
+    static_assert(kGroups % W == 0);
 
-    __shared__ __attribute__((aligned(16))) uint8_t k_lds[2][kKeys * kKRow], v_lds[2][D * kVRow];
+    constexpr int kKBytes = kKeys * kKRow, kVBytes = D * kVRow;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kKBytes + 2 * kVBytes];  // both arrays, of two steps
     // of eight keys: their score's factor, the logarithm and the reciprocal of their values' scale,
     // and whether their page is in the cache
     __shared__ __attribute__((aligned(16))) f32x4 group_lds[2][kGroups];
@@ -111,7 +125,8 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
     const uint32_t at_row = (uint32_t)(wave * kWaveRows + col), at_token = a.by_heads.div(at_row), at_head = at_row - at_token * a.by_heads.d;
     const bool real = at_token < tile.tokens && at_head < tile.heads;
     const uint32_t row = tile.token0 + min(at_token, tile.tokens - 1), head = tile.head0 + min(at_head, tile.heads - 1);
-    const int32_t hi = min(max(a.lens[row], 0), (int32_t)a.max_len), lo = (int32_t)max((uint32_t)hi, a.window) - (int32_t)a.window;
+    const bool any_real = __any(real);  // a wave without a row of its own sees nothing
+    const int32_t hi = any_real ? min(max(a.lens[row], 0), (int32_t)a.max_len) : 0, lo = (int32_t)max((uint32_t)hi, a.window) - (int32_t)a.window;
 
     u32x4 qf[kSteps];
     {
@@ -136,13 +151,13 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
     lo_least = __builtin_amdgcn_readfirstlane(lo_least);
     if (lane == 0) {
         bounds[0][wave] = hi_most;
-        bounds[1][wave] = hi_least;
+        bounds[1][wave] = any_real ? hi_least : INT32_MAX;
         bounds[2][wave] = lo_most;
         bounds[3][wave] = lo_least;
     }
     if (tid < 3) flags[tid] = 0;
     __syncthreads();
-    int32_t all_hi = bounds[0][0], each_hi = bounds[1][0], each_lo = bounds[2][0], all_lo = bounds[3][0];
+    int32_t all_hi = bounds[0][0], each_hi = bounds[1][0], each_lo = bounds[2][0], all_lo = bounds[3][0];  // wave 0 has rows
 #pragma unroll
     for (int w = 1; w < W; ++w) {
         all_hi = max(all_hi, bounds[0][w]);
@@ -162,91 +177,104 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
         to = min(from + each, to);
     }
 
+    auto k_lds = [&](int buf) { return lds + buf * kKBytes; };
+    auto v_lds = [&](int buf) { return lds + 2 * kKBytes + buf * kVBytes; };
     const int32_t* table = a.tables + tile.run * a.table_stride;
     const uint8_t* k_base = a.cache.k + tile.kv * a.cache.head_stride;
     const uint8_t* v_base = a.cache.v + tile.kv * a.cache.head_stride;
     const int32_t last = all_hi - 1;
 
-    // What a thread brings of a step: pieces of 16 bytes of a key, units of 4 keys and 4
-    // dimensions, and (the first threads) a group's scales.
-    auto piece_key = [&](int i) { return (tid + i * kThreads) / (D * kEl / 16); };
-    auto piece_at = [&](int i) { return (tid + i * kThreads) % (D * kEl / 16); };
-    auto unit_keys = [&](int i) { return (tid + i * kThreads) / (D / 4); };
-    auto unit_dims = [&](int i) { return (tid + i * kThreads) % (D / 4); };
+    // What a wave brings of a step: groups of eight keys, which share a page and a block, so that their
+    // place is worked out once, in scalar registers; a lane pieces of 16 bytes of a key, and units of 4 keys
+    // and 4 dimensions of the values.
+    constexpr int kRowPieces = D * kEl / 16;
+    auto piece_of = [&](int i) __attribute__((always_inline)) { return lane + 64 * i; };
+    // Bytes: a piece is two accesses of LDS, of which eight lanes take four pieces of two keys, whose
+    // rows lie an odd number of accesses apart.
+    constexpr bool kPairs = kEl == 1 && kRowPieces % 4 == 0;
+    auto key_of = [&](int i) __attribute__((always_inline)) { return kPairs ? piece_of(i) / (2 * kRowPieces) * 2 + (piece_of(i) >> 2 & 1) : piece_of(i) / kRowPieces; };
+    auto part_of = [&](int i) __attribute__((always_inline)) {
+        return kPairs ? (piece_of(i) >> 3) % (kRowPieces / 4) * 4 + (piece_of(i) & 3) : piece_of(i) % kRowPieces;
+    };
+    auto has_piece = [&](int i) __attribute__((always_inline)) { return (8 * kRowPieces) % 64 == 0 || piece_of(i) < 8 * kRowPieces; };
+    auto has_unit = [&](int i) __attribute__((always_inline)) { return (D / 2) % 64 == 0 || piece_of(i) < D / 2; };
+    int64_t k_off[kKLoads], v_off[kVLoads];
+#pragma unroll
+    for (int i = 0; i < kKLoads; ++i)
+        k_off[i] = key_of(i) * a.cache.token_stride + part_of(i) * 16;
+#pragma unroll
+    for (int i = 0; i < kVLoads; ++i)
+        v_off[i] = piece_of(i) / (D / 4) * 4 * a.cache.token_stride + piece_of(i) % (D / 4) * 4 * kEl;
     struct Pages {
-        int32_t k[kKLoads], v[kVLoads], group;
-        uint32_t k_in[kKLoads], v_in[kVLoads], group_in;
+        int32_t page[kOwn];  // the same in all lanes, not yet in a scalar register
+        uint32_t in_page[kOwn];
     };
-    auto page_of = [&](int32_t key, int32_t* page, uint32_t* in_page) {
-        const uint32_t at = a.cache.page.div((uint32_t)min(key, last));
-        *page = table[at];
-        *in_page = (uint32_t)min(key, last) - at * a.cache.page.d;
-    };
-    auto pages_of = [&](uint32_t step) {
+    auto pages_of = [&](uint32_t step) __attribute__((always_inline)) {
         Pages p;
-        const int32_t key0 = (int32_t)(step * kKeys);
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i) page_of(key0 + piece_key(i), &p.k[i], &p.k_in[i]);
-#pragma unroll
-        for (int i = 0; i < kVLoads; ++i) page_of(key0 + 4 * unit_keys(i), &p.v[i], &p.v_in[i]);
-        page_of(key0 + 8 * (tid < kGroups ? tid : 0), &p.group, &p.group_in);
+        for (int g = 0; g < kOwn; ++g) {
+            const uint32_t key = min(step * kKeys + 8 * (uint32_t)(kOwn * wave + g), (uint32_t)last & ~7u);
+            const uint32_t at = a.cache.page.div(key);
+            uint32_t v_at = at;
+            asm("" : "+v"(v_at));  // a vector load: a scalar one would be waited for with the reads of LDS
+            p.page[g] = table[v_at];
+            p.in_page[g] = key - at * a.cache.page.d;
+        }
         return p;
     };
-    auto in_cache = [&](int32_t page) { return (uint32_t)page < a.cache.n_pages; };
-    auto place_of = [&](int32_t page, uint32_t in_page) {
-        return (in_cache(page) ? (int64_t)page * a.cache.page_stride : 0) + (int64_t)in_page * a.cache.token_stride;
-    };
+    auto in_cache = [&](int32_t page) __attribute__((always_inline)) { return (uint32_t)page < a.cache.n_pages; };
     struct Raw {
         u32x4 k[kKLoads];
         uint32_t v[kVLoads][4][kEl];
         float k_scale, v_scale;
+        bool paged;
     };
-    auto load = [&](const Pages& p, Raw& r) {
+    auto load_group = [&](int32_t page, uint32_t in_page, Raw& r) __attribute__((always_inline)) {
+        page = __builtin_amdgcn_readfirstlane(page);
+        r.paged = in_cache(page);
+        const int64_t place = (r.paged ? page * a.cache.page_stride : 0) + (int64_t)in_page * a.cache.token_stride;
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i)
-            if (kKPieces % kThreads == 0 || tid + i * kThreads < kKPieces)
-                r.k[i] = *reinterpret_cast<const u32x4*>(k_base + place_of(p.k[i], p.k_in[i]) + piece_at(i) * 16);
+            if (has_piece(i)) r.k[i] = *reinterpret_cast<const u32x4*>(k_base + place + k_off[i]);
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i)
-            if (kVUnits % kThreads == 0 || tid + i * kThreads < kVUnits) {
-                // a unit past the row's keys begins inside them: its page has all four
-                const uint8_t* v = v_base + place_of(p.v[i], p.v_in[i] & ~3u) + unit_dims(i) * 4 * kEl;
+            if (has_unit(i)) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) attn::load<4 * kEl, false>(v + j * a.cache.token_stride, r.v[i][j]);
+                for (int j = 0; j < 4; ++j) attn::load<4 * kEl, false>(v_base + (place + j * a.cache.token_stride) + v_off[i], r.v[i][j]);
             }
-        if constexpr (E == kI8)
-            if (tid < kGroups) {
-                const int64_t at = (in_cache(p.group) ? p.group : 0) * a.scales.page_stride +
-                                   (int64_t)(p.group_in >> a.scales.shift) * a.scales.block_stride + tile.kv * a.scales.head_stride;
-                r.k_scale = a.scales.k[at];
-                r.v_scale = a.scales.v[at];
-            }
+        if constexpr (E == kI8) {
+            int64_t at = (r.paged ? page : 0) * a.scales.page_stride + (int64_t)(in_page >> a.scales.shift) * a.scales.block_stride +
+                         tile.kv * a.scales.head_stride;
+            asm("" : "+v"(at));
+            r.k_scale = a.scales.k[at];
+            r.v_scale = a.scales.v[at];
+        }
     };
-    auto v_swizzle = [](int dim) { return kKeys == 64 ? (dim ^ (dim >> 3)) & 7 : ((dim >> 1) ^ (dim >> 3)) & 3; };
-    auto store = [&](const Pages& p, Raw& r, uint32_t step, int buf, int flag) {
+    auto load = [&](const Pages& p, Raw* r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < kOwn; ++g) load_group(p.page[g], p.in_page[g], r[g]);
+    };
+    auto store_group = [&](Raw& r, int group, uint32_t step, int buf, int flag) __attribute__((always_inline)) {
         const int32_t key0 = (int32_t)(step * kKeys);
         const bool partial = key0 < each_lo || key0 + kKeys > each_hi;
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i)
-            if (kKPieces % kThreads == 0 || tid + i * kThreads < kKPieces) {
-                const int key = piece_key(i), at = piece_at(i);
+            if (has_piece(i)) {
+                const int key = 8 * group + key_of(i);
                 const int r_lds = (key & ~12) | (key & 4) << 1 | (key & 8) >> 1;
-                uint8_t* to_row = k_lds[buf] + r_lds * kKRow;
-                const int by = r_lds & 7;
+                u32x4* to = reinterpret_cast<u32x4*>(k_lds(buf) + r_lds * kKRow + part_of(i) * (32 / kEl));
                 if constexpr (E == kHalf) {
-                    *reinterpret_cast<u32x4*>(to_row + ((at ^ by) * 16)) = r.k[i];
+                    *to = r.k[i];
                 } else {
                     const u32x4 w = r.k[i];
-                    *reinterpret_cast<u32x4*>(to_row + (((2 * at) ^ by) * 16)) =
-                        u32x4{from_byte<T, E, false>(w[0]), from_byte<T, E, true>(w[0]), from_byte<T, E, false>(w[1]), from_byte<T, E, true>(w[1])};
-                    *reinterpret_cast<u32x4*>(to_row + (((2 * at + 1) ^ by) * 16)) =
-                        u32x4{from_byte<T, E, false>(w[2]), from_byte<T, E, true>(w[2]), from_byte<T, E, false>(w[3]), from_byte<T, E, true>(w[3])};
+                    to[0] = u32x4{from_byte<T, E, false>(w[0]), from_byte<T, E, true>(w[0]), from_byte<T, E, false>(w[1]), from_byte<T, E, true>(w[1])};
+                    to[1] = u32x4{from_byte<T, E, false>(w[2]), from_byte<T, E, true>(w[2]), from_byte<T, E, false>(w[3]), from_byte<T, E, true>(w[3])};
                 }
             }
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i)
-            if (kVUnits % kThreads == 0 || tid + i * kThreads < kVUnits) {
-                const int kg = unit_keys(i), quad = unit_dims(i);
+            if (has_unit(i)) {
+                const int kg = 2 * group + piece_of(i) / (D / 4), quad = piece_of(i) % (D / 4);
                 u32x2 v[4];  // of each dimension, four keys
                 if constexpr (E == kHalf) {
 #pragma unroll
@@ -266,11 +294,10 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
                     v[3] = u32x2{from_byte<P, E, true>(h01), from_byte<P, E, true>(h23)};
                 }
                 if constexpr (E != kI8)  // 0 * NaN is NaN: nothing past the rows' keys, and who sees what is left is told
-                    if (partial || !in_cache(p.v[i])) {
-                        const int32_t key = key0 + 4 * kg;
-                        const bool paged = in_cache(p.v[i]);
-                        const u32x2 keep = {(paged && key <= last ? 0xFFFFu : 0) | (paged && key + 1 <= last ? 0xFFFF0000u : 0),
-                                            (paged && key + 2 <= last ? 0xFFFFu : 0) | (paged && key + 3 <= last ? 0xFFFF0000u : 0)};
+                    if (partial || !r.paged) {
+                        const int32_t key = r.paged ? key0 + 4 * kg : INT32_MAX - 3;
+                        const u32x2 keep = {(key <= last ? 0xFFFFu : 0) | (key + 1 <= last ? 0xFFFF0000u : 0),
+                                            (key + 2 <= last ? 0xFFFFu : 0) | (key + 3 <= last ? 0xFFFF0000u : 0)};
                         uint32_t bad = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -280,24 +307,25 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
                         if (bad) atomicOr(&flags[flag], 2u);
                     }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int dim = 4 * quad + e;
-                    *reinterpret_cast<u32x2*>(v_lds[buf] + dim * kVRow + (((kg >> 1) ^ v_swizzle(dim)) * 16) + (kg & 1) * 8) = v[e];
-                }
+                for (int e = 0; e < 4; ++e) *reinterpret_cast<u32x2*>(v_lds(buf) + (quad + D / 4 * e) * kVRow + kg * 8) = v[e];
             }
-        if (tid < kGroups) {
-            const bool paged = in_cache(p.group);
-            f32x4 g = {a.scale, 0, 1, paged ? 1.0f : 0.0f};
+        if (lane == 0) {
+            f32x4 g = {a.scale, 0, 1, r.paged ? 1.0f : 0.0f};
             if constexpr (E == kI8) {
                 const float k = a.scale * r.k_scale, v = r.v_scale;
                 g[0] = k < 1e-37f ? 1e-37f : k;  // -inf times 0 is NaN
                 const float up = v < 8.673617379884035e-19f ? 8.673617379884035e-19f : v;  // 2^-60
                 g[1] = __builtin_amdgcn_logf(up);
-                g[2] = 1.0f / up;
+                g[2] = __builtin_amdgcn_rcpf(up);  // within 2^-23
             }
-            group_lds[buf][tid] = g;
-            if (!paged && key0 + 8 * tid <= last) atomicOr(&flags[flag], 1u);
+            group_lds[buf][group] = g;
+            if (!r.paged && key0 + 8 * group <= last) atomicOr(&flags[flag], 1u);
         }
+    };
+
+    auto store = [&](Raw* r, uint32_t step, int buf, int flag) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < kOwn; ++g) store_group(r[g], kOwn * wave + g, step, buf, flag);
     };
 
     f32x16 acc[kTiles];
@@ -307,10 +335,13 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
         for (int i = 0; i < 16; ++i) acc[t][i] = 0;
     float m = -INFINITY, l = 0;
 
-    auto v_at = [&](int buf, int dim, int slot) { return v_lds[buf] + dim * kVRow + ((slot ^ v_swizzle(dim)) * 16); };
+    // Dimension 4 q + e is row q + D / 4 e of V: the lanes that write side by side are at neighbouring
+    // rows, and a lane's accumulators hold 16 neighbouring dimensions: row 32 t + 8 a + 4 half + b
+    // of tile t is accumulator 4 a + b.
+    auto v_at = [&](int buf, int row, int slot) __attribute__((always_inline)) { return v_lds(buf) + row * kVRow + slot * 16; };
     // Values without a number in a step that not every row sees whole: their dimension is NaN for
     // the rows that see them, and they are taken out for the others.  Rare, and slow.
-    auto part_ways = [&](uint32_t step, int buf) {
+    auto part_ways = [&](uint32_t step, int buf) __attribute__((always_inline)) {
         const int32_t key0 = (int32_t)(step * kKeys);
         for (int key = 0; key < kKeys; ++key) {
             const bool seen = key0 + key >= lo && key0 + key < hi && group_lds[buf][key / 8][3] != 0;
@@ -318,32 +349,46 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int dim = 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
-                    const uint32_t v = *reinterpret_cast<const uint16_t*>(v_at(buf, dim, key / 8) + key % 8 * 2);
+                    const int row = 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
+                    const uint32_t v = *reinterpret_cast<const uint16_t*>(v_at(buf, row, key / 8) + key % 8 * 2);
                     if (seen && not_finite<P>(v)) acc[t][i] = __uint_as_float(0x7FC00000u);
                 }
         }
         __syncthreads();
         for (int i = tid; i < D * kVRow / 4; i += kThreads) {
-            uint32_t* v = reinterpret_cast<uint32_t*>(v_lds[buf]) + i;
+            uint32_t* v = reinterpret_cast<uint32_t*>(v_lds(buf)) + i;
             *v &= ~not_finite<P>(*v);
         }
         __syncthreads();
     };
 
-    auto compute = [&](uint32_t step, int buf, uint32_t said) {
+    // The accumulators are scaled only where a maximum passes its base by more than 2^kLag: p
+    // reaches as much then.  fp16's is 2^(15 - kLag) at the base, so 2^15 at most, below the largest
+    // number; parts that leave out what lies low have no room for it.
+    constexpr float kLag = !P::kNarrow ? 8 : kLow ? 0 : 4;
+    auto base_of = [](float top) { return P::kNarrow && fabsf(top) < 8388608.0f ? top - (15 - kLag) : top; };
+    f32x16 sc[kSub];  // scores of a step, then its probabilities
+    bool low = false;
+    // Whether the wave's rows see any of the step.
+    auto sees = [&](uint32_t step) __attribute__((always_inline)) {
         const int32_t key0 = (int32_t)(step * kKeys);
-        if (key0 >= hi_most || key0 + kKeys <= lo_least) return;
-        f32x16 sc[kSub];
+        return key0 < hi_most && key0 + kKeys > lo_least;
+    };
+    auto scores = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
+        for (int u = 0; u < kSub; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[u][i] = 0;
-            const uint8_t* k_row = k_lds[buf] + (32 * u + col) * kKRow;
+        const uint8_t* k_row = k_lds(buf) + col * kKRow + half * 16;
 #pragma unroll
-            for (int st = 0; st < kSteps; ++st)
-                sc[u] = mfma32(T{}, *reinterpret_cast<const u32x4*>(k_row + (((2 * st + half) ^ (col & 7)) * 16)), qf[st], sc[u]);
-        }
+        for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+                sc[u] = mfma32(T{}, *reinterpret_cast<const u32x4*>(k_row + 32 * u * kKRow + st * 32), qf[st], sc[u]);
+    };
+    // The scores become probabilities; m and l.
+    auto probabilities = [&](uint32_t step, int buf, uint32_t said) __attribute__((always_inline)) {
+        const int32_t key0 = (int32_t)(step * kKeys);
         f32x4 group[2 * kSub];
 #pragma unroll
         for (int j = 0; j < 2 * kSub; ++j) group[j] = E == kI8 ? group_lds[buf][2 * j + half] : f32x4{a.scale, 0, 1, 1};
@@ -370,8 +415,8 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
             top = fmaxf(top, E == kI8 ? __builtin_fmaf(t, group[j][0], group[j][1]) : t);
         }
         if constexpr (E != kI8) top *= a.scale;
-        const float lift = P::base_of(halves_max(top));
-        if (__any(lift > m)) {
+        const float lift = base_of(halves_max(top));
+        if (__any(lift > m + kLag)) {
             const float up = fmaxf(m, lift), by = exp2_of(m - above(up));
             m = up;
             l *= by;
@@ -379,8 +424,7 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
             for (int t = 0; t < kTiles; ++t) acc[t] *= by;
         }
         const float base = above(m);
-        constexpr float kUp = 549755813888.0f;  // 2^39
-        bool low = false;
+        low = false;
 #pragma unroll
         for (int j = 0; j < 2 * kSub; ++j) {
             const float off = E == kI8 ? group[j][1] - base : -base, by = E == kI8 ? group[j][0] : a.scale;
@@ -394,7 +438,10 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
             }
             l = E == kI8 ? __builtin_fmaf(sum, group[j][2], l) : l + sum;
         }
-        auto add = [&](int j, u32x4 pf) {
+    };
+    constexpr float kUp = 549755813888.0f;  // 2^39
+    auto product = [&](int buf) __attribute__((always_inline)) {
+        auto add = [&](int j, u32x4 pf) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
                 acc[t] = mfma32(P{}, *reinterpret_cast<const u32x4*>(v_at(buf, 32 * t + col, 2 * j + half)), pf, acc[t]);
@@ -442,79 +489,99 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D <= 128 ? 2 : 1) void prompt
     };
 
     if (from < to) {
-        Raw raw;
-        Pages now = pages_of(from);
-        load(now, raw);
-        Pages then = pages_of(min(from + 1, to - 1));
-        store(now, raw, from, 0, 0);
+        Raw raw[2][kOwn];  // of steps from + 0, 2, ... and from + 1, 3, ...
+        const uint32_t end = to - 1;
+        Pages then;
+        {
+            const Pages first = pages_of(from), second = pages_of(min(from + 1, end));
+            then = pages_of(min(from + 2, end));
+            load(first, raw[0]);
+            load(second, raw[1]);
+        }
+        store(raw[0], from, 0, 0);
         __syncthreads();
         int flag = 0;
-        for (uint32_t step = from; step < to; ++step) {
-            const int buf = (int)(step - from) & 1, next_flag = flag == 2 ? 0 : flag + 1;
-            const bool more = step + 1 < to;
-            if (more) {
-                now = then;
-                load(now, raw);
-                then = pages_of(min(step + 2, to - 1));
-            }
+        // Past the last step it is loaded and stored again: no branches around loads, whose waits would
+        // be for all.
+        auto one_step = [&](uint32_t step, auto buf_tag) __attribute__((always_inline)) {
+            constexpr int buf = decltype(buf_tag)::value;
+            const int next_flag = flag == 2 ? 0 : flag + 1;
+            // the page before the loads: a wait for it is none for them
+            const Pages later = pages_of(min(step + 3, end));
+            load(then, raw[buf]);
+            then = later;
             const uint32_t said = flags[flag];
             if constexpr (E != kI8)
                 if (said & 2) part_ways(step, buf);
-            compute(step, buf, said);
-            if (more) store(now, raw, step + 1, buf ^ 1, next_flag);
+            if (sees(step)) {
+                scores(buf);
+                store(raw[buf ^ 1], min(step + 1, end), buf ^ 1, next_flag);  // beside the matrix instructions
+                probabilities(step, buf, said);
+                product(buf);
+            } else {
+                store(raw[buf ^ 1], min(step + 1, end), buf ^ 1, next_flag);
+            }
             // the flags of the step after the next: read last a step ago, before a barrier
             if (tid == 0) flags[next_flag == 2 ? 0 : next_flag + 1] = 0;
             flag = next_flag;
             __syncthreads();
+        };
+        for (uint32_t step = from;; step += 2) {
+            one_step(step, std::integral_constant<int, 0>{});
+            if (step == end) break;
+            one_step(step + 1, std::integral_constant<int, 1>{});
+            if (step + 1 == end) break;
         }
     }
 
     l = halves_sum(l);
     if (!real) return;
+    // the lane's accumulators, four neighbouring dimensions at a time
+    auto each_four = [&](auto&& f) {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[(2 * k + D / 16 * e) / 8][(2 * k + D / 16 * e) % 8 / 2 * 4 + b];
+                f(32 * k + 16 * half + 4 * b, v);
+            }
+    };
     if (a.splits > 1) {
         const int64_t entry = (((int64_t)slot * a.by_units.d + unit) * a.splits + blockIdx.y) * (W * kWaveRows) + at_row;
-        float* o = a.part_acc + entry * D + 4 * half;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(o + 32 * t + 2 * i) = f32x4{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
+        float* o = a.part_acc + entry * D;
+        each_four([&](int dim, f32x4 v) { *reinterpret_cast<f32x4*>(o + dim) = v; });
         if (half == 0) a.part_ml[entry] = make_float2(m, l);
         return;
     }
     const float over = l > 0 || l != l ? a.cache.v_scale / l : 0.0f;
     uint8_t* out = a.out + row * a.out_stride + (int64_t)head * D * (kF32 ? 4 : 2);
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        if constexpr (kF32) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(out + (32 * t + 2 * i + 4 * half) * 4) =
-                    f32x4{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]} * over;
-        } else {
-            // the two lanes of a column exchange fours: dimensions 0 - 7 to one, 8 - 15 to the other
-#pragma unroll
-            for (int i = 0; i < 16; i += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) w[e / 2] = T::pair(acc[t][i + e] * over, acc[t][i + e + 1] * over);
-                const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-                const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-                *reinterpret_cast<u32x4*>(out + (32 * t + 2 * i + 8 * half) * 2) = u32x4{x[0], y[0], x[1], y[1]};
-            }
-        }
-    }
+    each_four([&](int dim, f32x4 v) {
+        v *= over;
+        if constexpr (kF32)
+            *reinterpret_cast<f32x4*>(out + dim * 4) = v;
+        else
+            *reinterpret_cast<u32x2*>(out + dim * 2) = u32x2{T::pair(v[0], v[1]), T::pair(v[2], v[3])};
+    });
     if (a.lse && half == 0) a.lse[(int64_t)row * a.q_heads + head] = log_sum(m, l);
+}
+
+template <int D, class T, Elem E, int W>
+hipError_t launch_prompt_waves(const PromptArgs& a, bool out_f32, hipStream_t s) {
+    const dim3 grid(a.tiles * a.by_units.d, a.splits), block(64 * W);
+    if (out_f32)
+        hipLaunchKernelGGL((prompt_kernel<D, T, E, true, W>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((prompt_kernel<D, T, E, false, W>), grid, block, 0, s, a);
+    return hipGetLastError();
 }
 
 template <int D, class T, Elem E>
 hipError_t launch_prompt_elem(const PromptArgs& a, bool out_f32, hipStream_t s) {
-    const dim3 grid(a.tiles * a.by_units.d, a.splits), block(64 * prompt_waves(D));
-    if (out_f32)
-        hipLaunchKernelGGL((prompt_kernel<D, T, E, true>), grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL((prompt_kernel<D, T, E, false>), grid, block, 0, s, a);
-    return hipGetLastError();
+    if constexpr (D <= 128)
+        if (a.waves == 8) return launch_prompt_waves<D, T, E, 8>(a, out_f32, s);
+    return launch_prompt_waves<D, T, E, 4>(a, out_f32, s);
 }
 
 template <int D, class T>

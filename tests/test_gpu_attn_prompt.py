@@ -16,12 +16,12 @@ def bounds(o, size, dots, v_most, dim, q_t, c_t, out_t, n):
     the logarithm of a scale of up to 2^60 added (60 2^-24 and the sum's rounding), the maximum's
     difference and the exponential: dim + 16 roundings of 2^-24 of the sum of magnitudes, and 2^-17;
     an error e of the scores moves the output by at most 2 e sum p |v|.  A probability is rounded
-    once, by 2^-8 of it in bf16 (bf16 caches) or 2^-11 in fp16, where those below 2^-29 of the
-    largest lose 2^-40 of it; as parts, for fp32 outputs, 2^-21 stays.  Sums in 32 bits of n terms,
+    once, by 2^-8 of it in bf16 (bf16 caches) or 2^-11 in fp16: 2^11 at a row's base, at most 2^4 above
+    which its largest lies, so that half of the least unit, 2^-25, is 2^-36 of the largest; as parts, for fp32 outputs, 2^-21 stays.  Sums in 32 bits of n terms,
     32 at a time, of the steps and of the splits."""
     e = (dim + 16) * 2.0 ** -24 * dots + (2.0 ** -17 if c_t == I8 else 2.0 ** -22)
     part = 2.0 ** -21 if out_t == F32 else 2.0 ** -8 if c_t == BF16 else 2.0 ** -11
-    d = (2 * e[:, None] + part + (n / 32 + 64) * 2.0 ** -24) * size + n * 2.0 ** -40 * v_most
+    d = (2 * e[:, None] + part + (n / 32 + 64) * 2.0 ** -24) * size + n * 2.0 ** -36 * v_most
     d = d + ref.ROUND[out_t] * (np.abs(o) + d) + ref.TINY[out_t]
     return d, e + (n / 32 + 64) * 2.0 ** -24 + 2.0 ** -22
 
@@ -255,7 +255,7 @@ def test_keys_without_a_number(qmm):
 
 @pytest.mark.parametrize("q_t,c_t", TYPES)
 def test_sinks(qmm, q_t, c_t):
-    """A first key far above the others whose value is zero: up to 2^-28 of it for 16-bit outputs, and
+    """A first key far above the others whose value is zero: up to 2^-25 of it for 16-bit outputs, and
     any that fp32 holds for fp32 ones."""
     c = Case(qmm, [700], [6], 4, 1, 64, q_t, c_t, seed=13)
     p = c.c
