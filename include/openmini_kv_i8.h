@@ -69,7 +69,7 @@ int openmini_attn_decode_i8(const openmini_kv_cache_t* cache, const openmini_kv_
  * past the table, before 0 or on a page outside the cache reads as zeros.  Rows of no request are
  * left as they were, and so are those from `tokens` on.  d_starts does not decrease.  Either
  * output may be NULL.  Caches of every type; `scales` is NULL but for 8-bit integers.
- * head_dim: a multiple of 8, at most 512; tokens: at most 2^27; requests: at most 2^20. */
+ * head_dim: a multiple of 8, at most 512; tokens: at most 2^26; requests: at most 2^20. */
 typedef struct {
     const int32_t* d_tables;
     int64_t table_stride;

@@ -45,7 +45,7 @@ int openmini_kv_read(const openmini_kv_cache_t* cache, const openmini_kv_scales_
     TRY(check_any_cache(cache, scales, &a.cache, &a.scales));
     if (!dense_type(p->out_dtype)) return unsupported("k_out, v_out", p->out_dtype);
     TRY(check_range("requests", p->requests, 1, kMaxRuns));
-    TRY(check_range("tokens", p->tokens, 0, (int64_t)1 << 27));
+    TRY(check_range("tokens", p->tokens, 0, (int64_t)1 << 26));
     TRY(check_range("max_pages", p->max_pages, 1, kMaxI32));
     TRY(check_range("table_stride", p->table_stride, p->max_pages, (int64_t)1 << 40));
     TRY(check_pointer("d_tables", p->d_tables, 4));

@@ -169,10 +169,10 @@ def test_prompt_refusals(cache, args, status, word):
 
 def test_calls_past_a_launch():
     """Workgroups of more than 2^32 threads together."""
-    c = _cache(dtype=DType.BF16, kv_heads=16, head_dim=128)
-    args = _prompt(q_heads=16, q_stride=2048, out_stride=2048, rows=1, requests=1 << 20)
+    c = _cache(dtype=DType.BF16, kv_heads=64, head_dim=128)
+    args = _prompt(q_heads=64, q_stride=8192, out_stride=8192, rows=1, requests=1 << 20)
     _refused(_native.lib().openmini_attn_prompt(c, None, args, None), BAD, "too many")
-    _refused(_native.lib().openmini_kv_read(_cache(), _scales(), _read(tokens=(1 << 27) + 1), None), BAD, "tokens")
+    _refused(_native.lib().openmini_kv_read(_cache(), _scales(), _read(tokens=(1 << 26) + 1), None), BAD, "tokens")
 
 
 def test_prompt_workspace_bytes():
