@@ -20,6 +20,11 @@
 // maximum, however little above the last.
 //
 // q goes as in openmini_rope_apply, in the same launch, behind the workgroups of k and v.
+//
+// Bound by memory once the loads of the next head are on their way before a head's barrier and the
+// registers of k's and v's own instances are few enough for five workgroups a CU (both in one: three).
+// Measured (MI355X, one launch): 8191 tokens of 32 heads of 128, float in and out, 106 us (538 MB, 5.1
+// TB/s; 167 before); 200 requests' tokens of 64 and 8 heads 6.4 us; one token 4.3 us.
 #include "attn_rope.hpp"
 
 namespace attn {
@@ -28,11 +33,13 @@ namespace {
 constexpr float kLeastScale = 9.094947017729282e-13f;  // 2^-40
 constexpr uint32_t kMostRuns = 32;                     // tokens of a chunk
 constexpr uint32_t kMostHeads = 8;                     // of a workgroup
-static_assert((2 * kMostRuns - 1) * (kMaxI8Dim / 8) <= 8 * kRopeThreads, "eight items a thread hold the longest runs");
+static_assert(kMostRuns * (kMaxI8Dim / 8) <= 4 * kRopeThreads, "four items a thread hold a chunk");
 
 struct Runs {
-    int32_t of[64];            // a token's run (the lane of its first token), or -1
-    int64_t place[64];         // byte offset of its slot
+    int32_t of[64];     // a token's run (the lane of its first token), or -1
+    int32_t token[64];  // those that have a run of the workgroup's, in order
+    uint32_t tokens;    // how many
+    int64_t place[64];  // byte offset of a token's slot
     int64_t scale_at[kMostRuns];
     int64_t block_at[kMostRuns];  // byte offset of the block's first token
     int32_t held[kMostRuns];      // tokens before the run's in its block
@@ -66,20 +73,22 @@ __device__ __forceinline__ uint32_t scaled_codes(uint32_t c, float by) {
     return codes(make_float4((float)(int8_t)c, (float)(int8_t)(c >> 8), (float)(int8_t)(c >> 16), (float)(int8_t)(c >> 24)), by);
 }
 
-// k or v of the runs of a chunk.  kItems: items of a thread, at most.
-template <int kIn, bool kStream, int kItems>
-__device__ __forceinline__ void kv_workgroup(AppendI8Args a, int head_dim, uint32_t chunk, uint32_t head_group, bool values) {
+// k or v of the runs of a chunk.  Its tokens are as many as the chunk's where these follow each other
+// or are all by themselves, and kItems items a thread hold them; the next head's loads are behind this
+// one's barrier then.  Up to chunk + block - 1 they can be: then each head is read twice.
+template <int kIn, bool kStream, int kItems, bool kValues>
+__device__ __forceinline__ void kv_workgroup(AppendI8Args a, int head_dim, uint32_t chunk, uint32_t head_group) {
     extern __shared__ __attribute__((aligned(16))) float sines[];  // [tokens][pairs], and as many cosines
     __shared__ Runs runs;
     constexpr int kSize = kIn == OPENMINI_ATTN_F32 ? 4 : 2;
     RopeArgs r = a.r;
-    const uint32_t tid = threadIdx.x, block = 1u << a.scales.shift, tokens = a.chunk + block - 1, per_head = r.per_head.d;
+    const uint32_t tid = threadIdx.x, block = 1u << a.scales.shift, window = a.chunk + block - 1, per_head = r.per_head.d;
     const int64_t token0 = (int64_t)chunk * a.chunk;
     const int32_t head0 = (int32_t)(head_group * a.wg_heads), heads = min((int32_t)a.wg_heads, r.kv_heads - head0);
-    float* scale_of = values ? a.scales.v : a.scales.k;
+    float* scale_of = kValues ? a.scales.v : a.scales.k;
     if (tid < 64) {
         const int64_t token = token0 + tid;
-        const bool mine = tid < tokens && token < r.tokens;
+        const bool mine = tid < window && token < r.tokens;
         const int32_t slot = mine ? r.slots[token] : -1;
         int32_t before = __shfl_up(slot, 1);
         if (tid == 0) before = token0 > 0 ? r.slots[token0 - 1] : -1;
@@ -90,6 +99,7 @@ __device__ __forceinline__ void kv_workgroup(AppendI8Args a, int head_dim, uint3
         const uint64_t upto = lead_mask & (~0ull >> (63 - tid));
         const int32_t first = real && upto ? 63 - __clzll((long long)upto) : -1;
         const bool owned = first >= 0 && (uint32_t)first < a.chunk;
+        const uint64_t owned_mask = __ballot(owned);
         int64_t place = 0;
         if (real) {
             const uint32_t page = r.cache.page.div((uint32_t)slot), in_page = (uint32_t)slot - page * r.cache.page.d;
@@ -97,7 +107,7 @@ __device__ __forceinline__ void kv_workgroup(AppendI8Args a, int head_dim, uint3
             if (leads && tid < a.chunk) {
                 // tokens up to the next run, the next that has no slot, or the window's end
                 const uint64_t behind = tid < 63 ? (lead_mask | ~real_mask) >> (tid + 1) : 0;
-                runs.count[tid] = min((int32_t)(behind ? __ffsll((unsigned long long)behind) : 64), (int32_t)(tokens - tid));
+                runs.count[tid] = min((int32_t)(behind ? __ffsll((unsigned long long)behind) : 64), (int32_t)(window - tid));
                 runs.held[tid] = (int32_t)at;
                 runs.block_at[tid] = place - (int64_t)at * r.cache.token_stride;
                 const int64_t scale_at = (int64_t)page * a.scales.page_stride +
@@ -108,91 +118,133 @@ __device__ __forceinline__ void kv_workgroup(AppendI8Args a, int head_dim, uint3
         }
         runs.of[tid] = owned ? first : -1;
         runs.place[tid] = place;
+        if (owned) runs.token[__popcll(owned_mask & (((uint64_t)1 << tid) - 1))] = (int32_t)tid;
+        if (tid == 0) runs.tokens = (uint32_t)__popcll(owned_mask);
     } else {
         for (uint32_t i = tid - 64; i < kMostHeads * kMostRuns; i += kRopeThreads - 64) (&runs.most[0][0])[i] = 0;
     }
     __syncthreads();
-    float* cosines = sines + tokens * r.n_pairs;
-    if (!values)
+    const uint32_t tokens = runs.tokens, items = tokens * per_head;
+    if (!tokens) return;
+
+    // An item: eight elements of a token's head.
+    struct Place {
+        int32_t token, run, first, second, pair, u;
+    };
+    auto place_of = [&](uint32_t at) {
+        Place p;
+        const uint32_t t = r.per_head.div(at);
+        p.u = (int32_t)(at - t * per_head);
+        p.token = runs.token[min(t, 63u)];
+        p.run = runs.of[p.token & 63];
+        const bool turns = !kValues && p.u * 4 < r.n_pairs, halves = turns && !r.adjacent;
+        p.pair = turns ? p.u * 4 : -1;
+        p.first = halves ? p.u * 4 : p.u * 8;
+        p.second = halves ? p.u * 4 + r.n_pairs : p.u * 8 + 4;
+        return p;
+    };
+    const int64_t stride = kValues ? r.v_stride : r.k_stride;
+    const uint8_t* src = (kValues ? r.v : r.k) + token0 * stride + (int64_t)head0 * head_dim * kSize;
+    uint8_t* cache = (kValues ? r.cache.v : r.cache.k) + (int64_t)head0 * r.cache.head_stride;
+    auto load_item = [&](const Place& p, int32_t h, float4* x, float4* y) {
+        const uint8_t* from = src + p.token * stride + (int64_t)h * head_dim * kSize;
+        *x = load4<kIn, kStream>(from + p.first * kSize);
+        *y = load4<kIn, kStream>(from + p.second * kSize);
+    };
+    const float* cosines = sines + window * r.n_pairs;
+    auto turned = [&](const Place& p, float4& x, float4& y) {
+        if constexpr (!kValues)
+            if (p.pair >= 0) {
+                const uint32_t at = (uint32_t)p.token * (uint32_t)r.n_pairs + (uint32_t)p.pair;
+                turn(x, y, *reinterpret_cast<const float4*>(sines + at), *reinterpret_cast<const float4*>(cosines + at), r.adjacent);
+            }
+    };
+    auto tell = [&](const Place& p, int32_t h, bool real, float4 x, float4 y) {  // its run's maximum
+        uint32_t most = real ? max(magnitude(x), magnitude(y)) : 0;
+        if (per_head % 4 == 0) most = quad_max(most);
+        if (real && (per_head % 4 || (tid & 3) == 0)) atomicMax(&runs.most[h][p.run], most);
+    };
+    auto write = [&](const Place& p, int32_t h, float4 x, float4 y) {
+        const int32_t held = runs.held[p.run];
+        const float old = runs.old[h][p.run], scale = new_scale(runs.most[h][p.run], held, old);
+        const float by = scale == scale ? 1.0f / scale : 0.0f;
+        uint8_t* to = cache + h * r.cache.head_stride;
+        uint8_t* c = to + runs.place[p.token];
+        const u32x2 w = {codes(x, by), codes(y, by)};
+        if (p.second == p.first + 4) {
+            *reinterpret_cast<u32x2*>(c + p.first) = w;
+        } else {
+            *reinterpret_cast<uint32_t*>(c + p.first) = w[0];
+            *reinterpret_cast<uint32_t*>(c + p.second) = w[1];
+        }
+        const int32_t nth = p.token - p.run;
+        if (p.u == 0 && nth == 0) scale_of[runs.scale_at[p.run] + h * a.scales.head_stride] = scale;
+        if (held && scale > old) {  // not where either is NaN
+            const float again = old / scale;
+            for (int32_t t = nth; t < held; t += runs.count[p.run]) {
+                u32x2* was = reinterpret_cast<u32x2*>(to + runs.block_at[p.run] + t * r.cache.token_stride + p.u * 8);
+                const u32x2 v = *was;
+                *was = u32x2{scaled_codes(v[0], again), scaled_codes(v[1], again)};
+            }
+        }
+    };
+    const bool once = items <= kItems * kRopeThreads;
+    Place at[kItems];
+    float4 lo[kItems], hi[kItems];
+    if (once)
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            at[i] = place_of(tid + i * kRopeThreads);
+            if (tid + i * kRopeThreads < items) load_item(at[i], 0, &lo[i], &hi[i]);
+        }
+    if constexpr (!kValues) {
         for (uint32_t j = tid; j < tokens * (uint32_t)r.n_pairs; j += kRopeThreads) {
-            const uint32_t token = r.by_pairs.div(j), i = j - token * r.by_pairs.d;
-            if (runs.of[token] < 0) continue;
+            const uint32_t t = r.by_pairs.div(j), i = j - t * r.by_pairs.d, token = (uint32_t)runs.token[t];
             const RopePair pair = r.pairs[i];
             const int32_t p = r.positions[pair.axis * r.position_stride + token0 + token];
             float s, c;
             sin_cos((uint64_t)(int64_t)p * pair.step, &s, &c);
-            sines[j] = s * r.scale;
-            cosines[j] = c * r.scale;
-        }
-    if (!values) __syncthreads();
-
-    // the thread's items: a token and eight elements of each head
-    int32_t run[kItems], token[kItems], first[kItems], second[kItems], pair[kItems];
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-        const uint32_t at = tid + i * kRopeThreads, t = r.per_head.div(at);
-        const int32_t u = (int32_t)(at - t * per_head);
-        token[i] = (int32_t)min(t, 63u);
-        run[i] = t < tokens ? runs.of[t] : -1;
-        const bool turns = !values && u * 4 < r.n_pairs, halves = turns && !r.adjacent;
-        pair[i] = turns ? u * 4 : -1;
-        first[i] = halves ? u * 4 : u * 8;
-        second[i] = halves ? u * 4 + r.n_pairs : u * 8 + 4;
-    }
-    const uint8_t* src = values ? r.v : r.k;
-    const int64_t stride = values ? r.v_stride : r.k_stride;
-    uint8_t* cache = values ? r.cache.v : r.cache.k;
-    for (int32_t h = 0; h < heads; ++h) {
-        float4 lo[kItems], hi[kItems];
-        const uint8_t* from = src + (int64_t)(head0 + h) * head_dim * kSize;
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            if (run[i] < 0) continue;
-            const uint8_t* p = from + (token0 + token[i]) * stride;
-            lo[i] = load4<kIn, kStream>(p + first[i] * kSize);
-            hi[i] = load4<kIn, kStream>(p + second[i] * kSize);
-        }
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            uint32_t most = 0;
-            if (run[i] >= 0) {
-                if (pair[i] >= 0) {
-                    const uint32_t at = (uint32_t)token[i] * (uint32_t)r.n_pairs + (uint32_t)pair[i];
-                    turn(lo[i], hi[i], *reinterpret_cast<const float4*>(sines + at), *reinterpret_cast<const float4*>(cosines + at),
-                         r.adjacent);
-                }
-                most = max(magnitude(lo[i]), magnitude(hi[i]));
-            }
-            if (per_head % 4 == 0) {
-                most = quad_max(most);
-                if (run[i] >= 0 && (tid & 3) == 0) atomicMax(&runs.most[h][run[i]], most);
-            } else if (run[i] >= 0) {
-                atomicMax(&runs.most[h][run[i]], most);
-            }
+            sines[token * r.n_pairs + i] = s * r.scale;
+            sines[(window + token) * r.n_pairs + i] = c * r.scale;
         }
         __syncthreads();
-        uint8_t* to = cache + (int64_t)(head0 + h) * r.cache.head_stride;
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            if (run[i] < 0) continue;
-            const int32_t held = runs.held[run[i]];
-            const float old = runs.old[h][run[i]], scale = new_scale(runs.most[h][run[i]], held, old);
-            const float by = scale == scale ? 1.0f / scale : 0.0f;
-            uint8_t* p = to + runs.place[token[i]];
-            *reinterpret_cast<uint32_t*>(p + first[i]) = codes(lo[i], by);
-            *reinterpret_cast<uint32_t*>(p + second[i]) = codes(hi[i], by);
-            const int32_t u = (int32_t)(tid + i * kRopeThreads - r.per_head.div(tid + i * kRopeThreads) * per_head);
-            const int32_t nth = token[i] - run[i];
-            if (u == 0 && nth == 0) scale_of[runs.scale_at[run[i]] + h * a.scales.head_stride] = scale;
-            if (held && scale > old) {  // not where either is NaN
-                const float again = old / scale;
-                for (int32_t t = nth; t < held; t += runs.count[run[i]]) {
-                    u32x2* c = reinterpret_cast<u32x2*>(to + runs.block_at[run[i]] + t * r.cache.token_stride + u * 8);
-                    const u32x2 v = *c;
-                    *c = u32x2{scaled_codes(v[0], again), scaled_codes(v[1], again)};
+    }
+    if (!once) {
+        for (int32_t h = 0; h < heads; ++h) {
+            for (int pass = 0; pass < 2; ++pass) {
+                for (uint32_t n = tid; n < (items + 63) / 64 * 64; n += kRopeThreads) {
+                    const Place p = place_of(min(n, items - 1));
+                    float4 x, y;
+                    load_item(p, h, &x, &y);
+                    turned(p, x, y);
+                    if (pass == 0)
+                        tell(p, h, n < items, x, y);
+                    else if (n < items)
+                        write(p, h, x, y);
                 }
+                __syncthreads();
             }
         }
+        return;
+    }
+    for (int32_t h = 0; h < heads; ++h) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const bool real = tid + i * kRopeThreads < items;
+            if (real) turned(at[i], lo[i], hi[i]);
+            tell(at[i], h, real, lo[i], hi[i]);
+        }
+        float4 x[kItems], y[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            x[i] = lo[i];
+            y[i] = hi[i];
+            if (h + 1 < heads && tid + i * kRopeThreads < items) load_item(at[i], h + 1, &lo[i], &hi[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kItems; ++i)
+            if (tid + i * kRopeThreads < items) write(at[i], h, x[i], y[i]);
     }
 }
 
@@ -200,7 +252,10 @@ template <int kIn, bool kStream, int kTokens, int kItems>
 __global__ __launch_bounds__(kRopeThreads) void append_i8_kernel(AppendI8Args a, int head_dim, uint32_t beside) {
     if (blockIdx.x < a.kv_wgs) {
         const uint32_t part = blockIdx.x >> 1, chunk = a.by_head_groups.div(part);
-        kv_workgroup<kIn, kStream, kItems>(a, head_dim, chunk, part - chunk * a.by_head_groups.d, blockIdx.x & 1);
+        if (blockIdx.x & 1)
+            kv_workgroup<kIn, kStream, kItems, true>(a, head_dim, chunk, part - chunk * a.by_head_groups.d);
+        else
+            kv_workgroup<kIn, kStream, kItems, false>(a, head_dim, chunk, part - chunk * a.by_head_groups.d);
     } else {
         const uint32_t at = blockIdx.x - a.kv_wgs, group = a.by_slices.div(at);
         rope_workgroup<kIn, kStream, kTokens>(a.r, head_dim, beside, group, at - group * a.by_slices.d);
@@ -218,10 +273,10 @@ hipError_t launch_items(const AppendI8Args& a, int head_dim, uint32_t beside, bo
 
 template <int kIn>
 hipError_t launch_type(const AppendI8Args& a, int head_dim, uint32_t beside, bool stream, uint32_t wgs, size_t lds, hipStream_t s) {
-    const uint32_t items = (a.chunk + (1u << a.scales.shift) - 1) * a.r.per_head.d;
+    const uint32_t items = a.chunk * a.r.per_head.d;
+    if (items <= kRopeThreads) return launch_items<kIn, 1>(a, head_dim, beside, stream, wgs, lds, s);
     if (items <= 2 * kRopeThreads) return launch_items<kIn, 2>(a, head_dim, beside, stream, wgs, lds, s);
-    if (items <= 4 * kRopeThreads) return launch_items<kIn, 4>(a, head_dim, beside, stream, wgs, lds, s);
-    return launch_items<kIn, 8>(a, head_dim, beside, stream, wgs, lds, s);
+    return launch_items<kIn, 4>(a, head_dim, beside, stream, wgs, lds, s);
 }
 
 }  // namespace
