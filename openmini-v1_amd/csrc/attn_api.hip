@@ -72,8 +72,8 @@ int decode(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales,
     const attn::Cache& c = a.cache;
     const int64_t held = p->max_pages * cache->page_size, max_len = held < kMostKeys ? held : kMostKeys;
     const uint32_t shares = attn::decode_shares(cache->kv_heads, head_tiles);
-    // tiles of the call at most
-    const int64_t tiles = p->rows * (max_len / (32 * attn::decode_subtiles(cache->head_dim, f8)) + 2);
+    const int sub = i8 ? attn::decode_subtiles_i8(cache->head_dim) : attn::decode_subtiles(cache->head_dim, f8), tile = 32 * sub;
+    const int64_t tiles = p->rows * (max_len / tile + 2);  // of the call at most
     if (tiles > (int64_t)UINT32_MAX / 2)
         return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%lld rows of up to %lld keys are too many for one call",
                     (long long)p->rows, (long long)max_len);
@@ -113,13 +113,13 @@ int decode(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales,
     a.part_ml = reinterpret_cast<float2*>(work + w.ml_at);
     a.part_acc = reinterpret_cast<float*>(work + w.acc_at);
     a.by_row = p->rows <= (int64_t)shares;
-    const int64_t keys = max_len < (int64_t)a.window ? max_len : (int64_t)a.window, tile = 32 * attn::decode_subtiles(cache->head_dim, f8);
+    const int64_t keys = max_len < (int64_t)a.window ? max_len : (int64_t)a.window;
     a.stream = head_tiles == 1 && p->rows <= p->requests &&
                attn::decode_streams(c, cache->kv_heads, cache->head_dim, f8, p->rows * keys);
     // a window's first tile need not begin with it
     const int64_t most = (keys + tile - 1) / tile + (keys < max_len), pairs = p->rows * cache->kv_heads * head_tiles;
     a.whole = attn::decode_whole(most, pairs);
-    a.uncut = attn::decode_uncut(most, p->rows, (int64_t)cache->kv_heads * head_tiles, shares, cache->head_dim, f8);
+    a.uncut = attn::decode_uncut_of(most, p->rows, (int64_t)cache->kv_heads * head_tiles, shares, sub, cache->head_dim * (f8 ? 1 : 2));
     if (a.uncut) a.launch_shares = p->rows < (int64_t)shares ? (uint32_t)p->rows : shares;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool bf16 = p->q_dtype == OPENMINI_ATTN_BF16;

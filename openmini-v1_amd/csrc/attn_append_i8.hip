@@ -23,7 +23,7 @@
 //
 // Bound by memory once the loads of the next head are on their way before a head's barrier and the
 // registers of k's and v's own instances are few enough for five workgroups a CU (both in one: three).
-// Measured (MI355X, one launch): 8191 tokens of 32 heads of 128, float in and out, 106 us (538 MB, 5.1
+// Measured (MI355X, one launch): 8191 tokens of 32 heads of 128, float in, q in fp16, 106 us (538 MB, 5.1
 // TB/s; 167 before); 200 requests' tokens of 64 and 8 heads 6.4 us; one token 4.3 us.
 #include "attn_rope.hpp"
 

@@ -825,7 +825,8 @@ __global__ __launch_bounds__(64 * W, D == 256 && E == kHalf ? 1 : 2) void decode
 template <int D, class T, Elem E, bool kWide, bool kWhole, bool kStream>
 hipError_t launch_one(const ArgsOf<E>& a, hipStream_t s) {
     constexpr bool F8 = E != kHalf;
-    constexpr int W = kWhole && !(D == 256 && !F8) ? 2 * kDecodeWaves : kDecodeWaves, kSub = decode_subtiles(D, F8);
+    constexpr int W = kWhole && !(D == 256 && !F8) ? 2 * kDecodeWaves : kDecodeWaves;
+    constexpr int kSub = E == kI8 ? decode_subtiles_i8(D) : decode_subtiles(D, F8);
     const uint64_t units = (uint64_t)a.kv_heads * a.head_tiles;
     const uint64_t all = kWhole ? a.n_rows * units : (a.launch_shares * units + W - 1) / W, wgs = (all + 7) / 8 * 8;
     hipLaunchKernelGGL((decode_kernel<D, T, E, kSub, W, kWide, kWhole, kStream>), dim3((unsigned)wgs), dim3(64 * W), 0, s, a.lens, a.rows,

@@ -11,6 +11,10 @@ constexpr int kDecodeWaves = 4;  // waves of a workgroup
 constexpr int decode_subtiles(int head_dim, bool f8) {
     return f8 ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1) : head_dim <= 64 ? 2 : 1;
 }
+// Of a cache of 8-bit integers about 8 KB, whose conversion takes more registers (heads of 64 spilled at
+// four 32s).  Measured, this against the above (us): one row of 300 / 131071 keys, 8 heads of 128, 7.3 / 53.2
+// against 7.6 / 54.8, 128 rows of 2000 to 12000 246 against 252; 64 rows, heads of 64, 23.5 against 26.2.
+constexpr int decode_subtiles_i8(int head_dim) { return head_dim <= 64 ? 2 : 1; }
 constexpr int kHeadTile = 16;    // query heads a workgroup serves (the MFMA's columns)
 // Waves of a call, at most (one share each unless the units alone are more): one for each
 // SIMD.  Two or three raise the bytes in flight past what the memory needs, and then equal
@@ -26,7 +30,8 @@ constexpr int kRound = 1024;
 // .77 / .77).  Measured, whole rows against shares (us): 8 pairs of 300 keys, heads of 128, bf16
 // 7.0 / 9.4, of 700 9.8 / 10.7, of 1000 12.5 / 10.9; 64 pairs of 1000 13.5 / 16.2, of 2000
 // 22.6 / 18.5; 256 of up to 4000, heads of 64, 46.8 / 36.4; 512 of 400 15.1 / 20.4; 1024 of
-// 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.
+// 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.  8-bit integers, heads of 128: 8 pairs of 500 keys 8.1 / 10.5, of
+// 700 9.8 / 10.5, 64 of 1000 12.1 / 14.1, of 2000 19.4 / 17.5, 512 of 1000 28.4 / 28.4.
 inline bool decode_whole(int64_t most, int64_t pairs) {
     return most == 1 ? pairs <= 256 : pairs <= 512 && most <= (pairs < 64 ? 16 : 32);
 }
@@ -46,15 +51,19 @@ inline bool decode_whole(int64_t most, int64_t pairs) {
 // bf16 1.22 1.23 1.09 1.10 1.05 1.01 (of 3 tiles 1.14 1.15 .97 1.00 .99 1.03, but in heads of 128
 // .97 .96 .83 .91 .92 .95).  One key head, whose join has a row for each share: heads of 128 .93
 // .94 .85 .92 .85 .82, of 256 1.14 1.13 1.01 1.01 .94 .95, of 64 in e4m3 1.06 1.07 .95 1.06 .98 .98.
+// 8-bit integers in heads of 128, half to all of 4 tiles, 320 / 560 / 1032 / 1600 / 2056 pairs: .71 .68 .96 .80
+// .99; of 64 .83 .78 1.07 .87 1.09; of 256 .72 .68 1.00 .83 1.00.
 // So the rows are cut where 48 KB of tiles or more would be waited for, or 96 KB where there are one or
 // two units; a tile of 128 keys, which the issue of instructions bounds, counts twice.
-inline bool decode_uncut(int64_t most, int64_t rows, int64_t units, int64_t shares, int head_dim, bool f8) {
+inline bool decode_uncut_of(int64_t most, int64_t rows, int64_t units, int64_t shares, int sub, int key_bytes) {
     const int64_t pairs = rows * units;
     if (most == 1) return pairs > 256;
     if (pairs <= 512 || most > (pairs <= 4096 ? 4 : 2)) return false;
     const int64_t tiles = (rows + shares - 1) / shares * most - (rows * most + shares - 1) / shares;
-    const int sub = decode_subtiles(head_dim, f8), tile = 2 * 32 * sub * head_dim * (f8 ? 1 : 2) * (sub == 4 ? 2 : 1);
-    return tiles * tile < (units > 2 ? 48 << 10 : 96 << 10);
+    return tiles * 2 * 32 * sub * key_bytes * (sub == 4 ? 2 : 1) < (units > 2 ? 48 << 10 : 96 << 10);
+}
+inline bool decode_uncut(int64_t most, int64_t rows, int64_t units, int64_t shares, int head_dim, bool f8) {
+    return decode_uncut_of(most, rows, units, shares, decode_subtiles(head_dim, f8), head_dim * (f8 ? 1 : 2));
 }
 
 }  // namespace attn
