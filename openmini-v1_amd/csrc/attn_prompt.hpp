@@ -392,18 +392,25 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
         f32x4 group[2 * kSub];
 #pragma unroll
         for (int j = 0; j < 2 * kSub; ++j) group[j] = E == kI8 ? group_lds[buf][2 * j + half] : f32x4{a.scale, 0, 1, 1};
+        float least = INFINITY;  // before the mask: an edge is not low
+        if constexpr (kLow)
+#pragma unroll
+            for (int j = 0; j < 2 * kSub; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) least = fminf(least, sc[j / 2][8 * (j & 1) + i]);
         if (key0 < lo_most || key0 + kKeys > hi_least || (said & 1)) {
 #pragma unroll
             for (int j = 0; j < 2 * kSub; ++j) {
-                const bool paged = group_lds[buf][2 * j + half][3] != 0;
-                const int32_t key = key0 + 16 * j + 8 * half;
+                const uint32_t from_lo = (uint32_t)(key0 + 16 * j + 8 * half - lo);
+                const uint32_t span = group_lds[buf][2 * j + half][3] != 0 ? (uint32_t)(hi - lo) : 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool seen = paged && key + i >= lo && key + i < hi;
-                    sc[j / 2][8 * (j & 1) + i] = seen ? sc[j / 2][8 * (j & 1) + i] : -INFINITY;
-                }
+                for (int i = 0; i < 8; ++i)
+                    sc[j / 2][8 * (j & 1) + i] = from_lo + i < span ? sc[j / 2][8 * (j & 1) + i] : -INFINITY;
                 // nor are the scales of a group that the row does not see
-                if (E == kI8 && !(paged && key + 8 > lo && key < hi)) group[j] = f32x4{1, 0, 0, 0};
+                if constexpr (E == kI8) {
+                    const bool some = from_lo + 7 < span + 7 && span != 0;
+                    group[j] = f32x4{some ? group[j][0] : 1, some ? group[j][1] : 0, some ? group[j][2] : 0, 0};
+                }
             }
         }
         float top = -INFINITY;
@@ -424,7 +431,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
             for (int t = 0; t < kTiles; ++t) acc[t] *= by;
         }
         const float base = above(m);
-        low = false;
+        if constexpr (kLow) low = __any(least * a.scale < base - 2.0f);
 #pragma unroll
         for (int j = 0; j < 2 * kSub; ++j) {
             const float off = E == kI8 ? group[j][1] - base : -base, by = E == kI8 ? group[j][0] : a.scale;
@@ -434,57 +441,60 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
                 const float s = exp2_of(__builtin_fmaf(sc[j / 2][8 * (j & 1) + i], by, off));
                 sc[j / 2][8 * (j & 1) + i] = s;
                 sum += s;
-                if constexpr (kLow) low = low || (s < 0.25f && s > 0);
             }
             l = E == kI8 ? __builtin_fmaf(sum, group[j][2], l) : l + sum;
         }
     };
     constexpr float kUp = 549755813888.0f;  // 2^39
     auto product = [&](int buf) __attribute__((always_inline)) {
-        auto add = [&](int j, u32x4 pf) __attribute__((always_inline)) {
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-                acc[t] = mfma32(P{}, *reinterpret_cast<const u32x4*>(v_at(buf, 32 * t + col, 2 * j + half)), pf, acc[t]);
-        };
-#pragma unroll
-        for (int j = 0; j < 2 * kSub; ++j) {
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = sc[j / 2][8 * (j & 1) + i];
+        // p of groups 2 j and 2 j + 1 in parts, which leave their rest in it
+        auto parts = [&](int j, float* p, auto add_tag) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < kParts; ++k) {
                 u32x4 pf;
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     pf[i / 2] = P::pair(p[i], p[i + 1]);
-                    if (kParts > 1) {
-                        p[i] -= P::low(pf[i / 2]);
-                        p[i + 1] -= P::high(pf[i / 2]);
-                    }
+                    p[i] -= P::low(pf[i / 2]);
+                    p[i + 1] -= P::high(pf[i / 2]);
                 }
-                add(j, pf);
+                if constexpr (decltype(add_tag)::value)
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+                        acc[t] = mfma32(P{}, *reinterpret_cast<const u32x4*>(v_at(buf, 32 * t + col, 2 * j + half)), pf, acc[t]);
             }
-            if constexpr (kLow) {
-                if (!__any(low)) continue;
-                // what two parts leave of p < 2^-2, 2^39 up
+        };
+        auto p_of = [&](int j, float* p) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = sc[j / 2][8 * (j & 1) + i];
+        };
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 2 * kSub; ++j) {
+            p_of(j, p);
+            parts(j, p, std::true_type{});
+        }
+        if constexpr (kLow) {
+            if (!low) return;
+            // not the reads and parts above, kept in more registers than there are
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(sc[u][i]));
+            // what two parts leave of p < 2^-2, 2^39 up
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) acc[t] *= kUp;
+#pragma unroll
+            for (int j = 0; j < 2 * kSub; ++j) {
+                p_of(j, p);
+                parts(j, p, std::false_type{});
 #pragma unroll
                 for (int i = 0; i < 8; ++i) p[i] = sc[j / 2][8 * (j & 1) + i] < 0.25f ? p[i] * kUp : 0.0f;
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t) acc[t] *= kUp;
-#pragma unroll
-                for (int k = 0; k < kParts; ++k) {
-                    u32x4 pf;
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        pf[i / 2] = P::pair(p[i], p[i + 1]);
-                        p[i] -= P::low(pf[i / 2]);
-                        p[i + 1] -= P::high(pf[i / 2]);
-                    }
-                    add(j, pf);
-                }
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t) acc[t] *= 1.0f / kUp;
+                parts(j, p, std::true_type{});
             }
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) acc[t] *= 1.0f / kUp;
         }
     };
 
