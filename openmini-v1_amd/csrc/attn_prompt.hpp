@@ -90,8 +90,9 @@ __device__ __forceinline__ PromptTile prompt_tile(const int32_t* starts, uint32_
     return t;
 }
 
-template <int D, class T, Elem E, bool kF32, int W>
-__global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(PromptArgs a) {
+// kPer: waves a SIMD.
+template <int D, class T, Elem E, bool kF32, int W, int kPer>
+__global__ __launch_bounds__(64 * W, kPer) void prompt_kernel(PromptArgs a) {
     // of the second product: byte caches fit both types, fp16 has the finer step and bf16 the
     // range that exact parts need
     using P = std::conditional_t<E == kHalf, T, std::conditional_t<kF32, BF16, F16>>;
@@ -106,6 +107,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
     constexpr int kKLoads = (8 * D * kEl / 16 + 63) / 64, kVLoads = (D / 2 + 63) / 64;
     constexpr int kGroups = kKeys / 8;
     constexpr int kOwn = kGroups / W;  // groups that a wave brings
+    constexpr int kSets = D <= 128 || kPer == 1 ? 2 : 1;  // steps whose data are on their way
     static_assert(kGroups % W == 0);
 
     constexpr int kKBytes = kKeys * kKRow, kVBytes = D * kVRow;
@@ -499,14 +501,14 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
     };
 
     if (from < to) {
-        Raw raw[2][kOwn];  // of steps from + 0, 2, ... and from + 1, 3, ...
+        Raw raw[kSets][kOwn];  // of steps from + 0, 2, ... and from + 1, 3, ...
         const uint32_t end = to - 1;
         Pages then;
         {
             const Pages first = pages_of(from), second = pages_of(min(from + 1, end));
-            then = pages_of(min(from + 2, end));
+            then = kSets == 2 ? pages_of(min(from + 2, end)) : second;
             load(first, raw[0]);
-            load(second, raw[1]);
+            if constexpr (kSets == 2) load(second, raw[1]);
         }
         store(raw[0], from, 0, 0);
         __syncthreads();
@@ -517,19 +519,28 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
             constexpr int buf = decltype(buf_tag)::value;
             const int next_flag = flag == 2 ? 0 : flag + 1;
             // the page before the loads: a wait for it is none for them
-            const Pages later = pages_of(min(step + 3, end));
-            load(then, raw[buf]);
+            const Pages later = pages_of(min(step + 1 + kSets, end));
+            load(then, raw[kSets == 2 ? buf : 0]);
             then = later;
             const uint32_t said = flags[flag];
             if constexpr (E != kI8)
                 if (said & 2) part_ways(step, buf);
-            if (sees(step)) {
-                scores(buf);
-                store(raw[buf ^ 1], min(step + 1, end), buf ^ 1, next_flag);  // beside the matrix instructions
-                probabilities(step, buf, said);
-                product(buf);
+            if constexpr (kSets == 2) {
+                if (sees(step)) {
+                    scores(buf);
+                    store(raw[buf ^ 1], min(step + 1, end), buf ^ 1, next_flag);  // beside the matrix instructions
+                    probabilities(step, buf, said);
+                    product(buf);
+                } else {
+                    store(raw[buf ^ 1], min(step + 1, end), buf ^ 1, next_flag);
+                }
             } else {
-                store(raw[buf ^ 1], min(step + 1, end), buf ^ 1, next_flag);
+                if (sees(step)) {
+                    scores(buf);
+                    probabilities(step, buf, said);
+                    product(buf);
+                }
+                store(raw[0], min(step + 1, end), buf ^ 1, next_flag);
             }
             // the flags of the step after the next: read last a step ago, before a barrier
             if (tid == 0) flags[next_flag == 2 ? 0 : next_flag + 1] = 0;
@@ -577,14 +588,27 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void prompt_kernel(Prompt
     if (a.lse && half == 0) a.lse[(int64_t)row * a.q_heads + head] = log_sum(m, l);
 }
 
+template <int D, class T, Elem E, bool kF32, int W>
+hipError_t launch_prompt_out(const PromptArgs& a, hipStream_t s) {
+    const dim3 grid(a.tiles * a.by_units.d, a.splits), block(64 * W);
+    // Two workgroups a CU hide each other's waits, though heads of 192 and 256 have registers for one step's
+    // data then, not two, and those of 256 keep 80 to 240 bytes in scratch.  4096 tokens of 32 heads against one
+    // workgroup (MI355X, us): of 192 304 / 533 (16-bit caches 313 / 511), of 256 357 / 520 (557 / 572, fp32
+    // out 612 / 641).  Heads of 256: 600 tokens (150 workgroups) 49 / 43, 1200 (300) 90 / 80, 2000 (500) 146 / 140, 512 behind 8000 keys
+    // (512) 210 / 267, and with what two fp16 parts leave 1100 / 711.
+    if constexpr (D == 256)
+        if ((E == kHalf && kF32 && T::kNarrow) || (int64_t)grid.x * grid.y <= prompt_alone(D)) {
+            hipLaunchKernelGGL((prompt_kernel<D, T, E, kF32, W, 1>), grid, block, 0, s, a);
+            return hipGetLastError();
+        }
+    if constexpr (!(D == 256 && E == kHalf && kF32 && T::kNarrow))
+        hipLaunchKernelGGL((prompt_kernel<D, T, E, kF32, W, 2>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
 template <int D, class T, Elem E, int W>
 hipError_t launch_prompt_waves(const PromptArgs& a, bool out_f32, hipStream_t s) {
-    const dim3 grid(a.tiles * a.by_units.d, a.splits), block(64 * W);
-    if (out_f32)
-        hipLaunchKernelGGL((prompt_kernel<D, T, E, true, W>), grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL((prompt_kernel<D, T, E, false, W>), grid, block, 0, s, a);
-    return hipGetLastError();
+    return out_f32 ? launch_prompt_out<D, T, E, true, W>(a, s) : launch_prompt_out<D, T, E, false, W>(a, s);
 }
 
 template <int D, class T, Elem E>

@@ -20,6 +20,8 @@ struct PromptShape {
 
 // Pairs of a tile and a split, at most, where tiles are split, and rows of a tile at most.
 constexpr int kPromptParts = 512;
+// Workgroups of four waves, at most, that have a CU each.
+constexpr int prompt_alone(int head_dim) { return head_dim == 256 ? 384 : 256; }
 constexpr int prompt_rows(int head_dim) { return head_dim <= 128 ? 256 : 128; }
 
 inline PromptShape prompt_tiles(int waves, int64_t rows, int64_t requests, int kv_heads, int group) {
@@ -38,7 +40,8 @@ inline PromptShape prompt_tiles(int waves, int64_t rows, int64_t requests, int k
 // Time of a call, in steps of a workgroup of eight waves, of which a CU holds one (2 us): rounds of
 // workgroups (the longest begin first, so a round need not be full to the last) times their steps,
 // and 1.5 to begin and end; and a second launch that joins splits, whose parts are written and read at
-// 4 TB/s.  Of four waves a CU holds one in .95 of the time, or two in 1.45 of it (heads of up to 128).
+// 4 TB/s.  Of four waves a CU holds one in .95 of the time, or two in 1.45 of it (1.2 in heads of 192 and
+// 256, whose steps are half the keys).
 // Measured (MI355X, us, four waves and eight): 200 tokens of 64 heads of 128 13.6 / 14.9, 3200 keys 97 /
 // 104; a round of pairs of 66 steps 184, of eight waves 121.  64 tokens behind 8000 keys in 1, 4, 8, 16
 // splits 251, 78, 51, 59; 512 behind 30000 in 2 and 3 530 and 690.
@@ -48,9 +51,10 @@ inline double prompt_cost(const PromptShape& p, int head_dim, int64_t rows, int6
     const int64_t spare = requests == 1 ? 2 * (p.tokens - 1) : requests * (p.tokens - 1);  // twice the rows that tiles lack
     const int64_t wgs = (2 * rows + spare + (requests > 1 ? 2 * p.tokens - 1 : 0)) / (2 * p.tokens) * p.units * splits;
     double each = 1, cus = 256;
-    if (head_dim <= 128 && p.waves == 4) {
-        each = wgs <= 256 ? .95 : 1.45;
-        if (wgs > 256) cus = 512;
+    if (p.waves == 4) {
+        const bool alone = wgs <= prompt_alone(head_dim);
+        each = alone ? .95 : head_dim <= 128 ? 1.45 : 1.2;
+        if (!alone) cus = 512;
     }
     const double full = wgs / cus, edge = requests == 1 ? 0 : .06;
     const double rounds = full <= 1 - edge ? 1 : full > 1 + edge || edge == 0 ? full + .3 : 1 + (full - 1 + edge) * (.3 + edge) / (2 * edge);
