@@ -454,11 +454,19 @@ __global__ __launch_bounds__(64 * W, kPer) void prompt_kernel(PromptArgs a) {
 #pragma unroll
             for (int k = 0; k < kParts; ++k) {
                 u32x4 pf;
+                float minus = -1;
+                if constexpr (P::kNarrow) asm("" : "+s"(minus));  // else a conversion and a subtraction
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     pf[i / 2] = P::pair(p[i], p[i + 1]);
-                    p[i] -= P::low(pf[i / 2]);
-                    p[i + 1] -= P::high(pf[i / 2]);
+                    if constexpr (P::kNarrow) {  // from the pair, one instruction each: not rounded a second time
+                        asm("" : "+v"(pf[i / 2]));
+                        p[i] = __builtin_fmaf(P::low(pf[i / 2]), minus, p[i]);
+                        p[i + 1] = __builtin_fmaf(P::high(pf[i / 2]), minus, p[i + 1]);
+                    } else {
+                        p[i] -= P::low(pf[i / 2]);
+                        p[i + 1] -= P::high(pf[i / 2]);
+                    }
                 }
                 if constexpr (decltype(add_tag)::value)
 #pragma unroll
