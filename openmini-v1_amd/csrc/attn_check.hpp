@@ -135,12 +135,12 @@ inline int check_cache_i8(const openmini_kv_cache_t* c, const openmini_kv_scales
     for (int i = 0; i < 2; ++i)
         for (int j = 0; j < 2; ++j)
             if (d[j].stride > d[j + 1].stride) std::swap(d[j], d[j + 1]);
-    int64_t reach = 1;
+    double reach = 1;  // exact where a stride can be as much; their sum may pass 63 bits
     for (const auto& x : d) {
-        if (x.stride < 0 || x.stride > ((int64_t)1 << 40) || (x.count > 1 && x.stride < reach))
+        if (x.stride < 0 || x.stride > ((int64_t)1 << 40) || (x.count > 1 && (double)x.stride < reach))
             return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "scales' strides %lld, %lld, %lld: two scales share an element",
                         (long long)s->page_stride, (long long)s->block_stride, (long long)s->head_stride);
-        reach += x.stride * (x.count - 1);
+        reach += (double)x.stride * (double)(x.count - 1);
     }
     to->k = s->d_k;
     to->v = s->d_v;

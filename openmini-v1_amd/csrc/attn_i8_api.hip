@@ -63,6 +63,10 @@ int openmini_kv_read(const openmini_kv_cache_t* cache, const openmini_kv_scales_
         TRY(check_stride("v_stride", p->v_stride, row, size));
     }
     if (p->tokens == 0) return ok();
+    if (p->d_k_out == p->d_v_out) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "d_k_out is d_v_out");
+    for (const void* out : {p->d_k_out, p->d_v_out})
+        if (out && (out == cache->d_k || out == cache->d_v))
+            return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "an output is the cache");
     TRY(qmm::current_device(nullptr));
     const int64_t held = p->max_pages * cache->page_size;
     a.tables = p->d_tables;
@@ -114,6 +118,8 @@ int openmini_attn_prompt(const openmini_kv_cache_t* cache, const openmini_kv_sca
     TRY(check_pointer("d_tables", p->d_tables, 4));
     if (p->d_lse) TRY(check_pointer("d_lse", p->d_lse, 4));
     if (p->d_out == p->d_q) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "d_out is d_q");
+    if (p->d_lse && ((const void*)p->d_lse == p->d_out || (const void*)p->d_lse == p->d_q))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "d_lse is d_out or d_q");
     const int64_t row = (int64_t)p->q_heads * cache->head_dim;
     const int out_size = size_of(p->out_dtype);
     TRY(check_stride("q_stride", p->q_stride, row, 2));

@@ -243,7 +243,8 @@ class CachedAttention:
         max_pages: columns that the step's longest request needs, where that is known (None:
         the tables' width); attention of short rows is faster for it.
         decoding: the first `decoding` requests of the step add one token each, the others runs,
-        which `prompt` attends to (None: every token is a row of decode attention)."""
+        which `prompt` attends to (None: every token is a row of decode attention); rows of d_out
+        behind the step's tokens are unspecified then."""
         most = plan.max_pages if max_pages is None else int(max_pages)
         if not 0 < most <= plan.max_pages:
             raise InvalidInput(f"max_pages {most}, tables of {plan.max_pages}")

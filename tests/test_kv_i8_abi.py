@@ -182,6 +182,25 @@ def test_prompt_workspace_bytes():
         assert L.openmini_attn_prompt_workspace_bytes(*bad) == 0, bad
 
 
+@pytest.mark.parametrize("kw,word", [
+    (dict(d_k_out=16 * P, d_v_out=16 * P), "d_k_out is d_v_out"), (dict(d_k_out=P, d_v_out=None), "output is the cache"),
+    (dict(d_k_out=None, d_v_out=2 * P), "output is the cache"), (dict(d_k_out=16 * P, d_v_out=P), "output is the cache")])
+def test_read_over_itself(kw, word):
+    _refused(_native.lib().openmini_kv_read(_cache(), _scales(), _read(**kw), None), BAD, word)
+
+
+def test_prompt_lse_over_others():
+    for args in (dict(d_lse=2 * P), dict(d_lse=P)):
+        _refused(_native.lib().openmini_attn_prompt(_cache(), _scales(), _prompt(**args), None), BAD, "d_lse is")
+
+
+def test_strides_whose_sum_passes_63_bits():
+    """Scales that share an element behind a stride too far for 64 bits: refused, not wrapped around."""
+    c = _cache(n_pages=(1 << 27) - 1)
+    far = _scales(page_stride=1 << 37, block_stride=1 << 40, head_stride=1)
+    _refused(_native.lib().openmini_kv_read(c, far, _read(), None), BAD, "share an element")
+
+
 class Buf:
     ptr, nbytes = ctypes.c_void_p(P), 1 << 20
 
