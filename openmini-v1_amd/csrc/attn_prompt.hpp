@@ -18,17 +18,18 @@
 // the score, a value's as its logarithm in the exponent, so that p v_scale is what is rounded
 // to 16 bits (at most 1, whatever the scales) and l adds p v_scale / v_scale.
 //
-// The loads of a step are issued more than a step ahead of their use and its page three; two buffers,
-// one barrier a step.  What comes goes to LDS beside the matrix instructions of the first product.
+// The loads of a step are issued more than a step ahead of their use and its page three (heads of 192 and 256: a
+// step and two, with another workgroup on the CU); two buffers, one barrier a step.  What comes goes to LDS beside the matrix instructions of the first product.
 // Accumulators are scaled only where a maximum has grown by 2^4: with 32 rows to a wave one of them
 // grows in most steps.
 //
 // Bound by the issue of instructions: a step of 64 keys takes a wave 2 us, alone on its SIMD or with
 // another, of which the matrix unit is busy for .4 (heads of 128); matrix and vector instructions of
 // the two waves run at the same time for two fifths of that only.  Measured (MI355X): 8191 tokens of
-// 64 / 8 heads of 128 1130 to 1180 us, 930 to 976 TFLOP/s (a large product of the library 1350); 4096
-// tokens of 32 / 8 heads of 64, 96, 128, 192, 256 150, 165, 165, 535, 525 us, on a bf16 cache of 128 174.
-// Of 192 and 256 a SIMD holds one wave.  What gave nothing or less: a second product a step later, for
+// 64 / 8 heads of 128 1150 to 1215 us, 905 to 956 TFLOP/s (a large product of the library 1350); 4096
+// tokens of 32 / 8 heads of 64, 96, 128, 192, 256 150, 163, 169, 304, 357 us, on a bf16 cache of 128 172; 211 tokens of
+// 64 / 8 heads of 128 13.4; 815 tokens in six pieces behind up to 1659 keys, 32 / 8 heads of 64 in fp16, fp32 out, 38.
+// What gave nothing or less: a second product a step later, for
 // half of the waves or among the exponentials (1.24, 1.47 ms of 1.26), wave priorities, 128 keys
 // a step, three waves a SIMD of 32 keys a step (1.31 of 1.18), rows out through LDS.
 #pragma once

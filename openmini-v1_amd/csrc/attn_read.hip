@@ -5,7 +5,8 @@
 // the first is used.  A wave finds the tokens' places, a lane each, and leaves them in LDS.
 //
 // Bound by memory for long calls and by its three dependent loads (starts, page, elements) for short
-// ones.
+// ones.  Measured (MI355X): 64 requests of 500 to 4000 tokens, 8 heads of 128, to fp16 115 us (656 MB, 5.7 TB/s); 300
+// tokens to bf16 4.7 (in a trace 3.5).  One token a thread with its place worked out by itself took 177 and 8.2.
 #include "attn_rope.hpp"
 #include "attn_runs.hpp"
 
