@@ -6,7 +6,8 @@
 //
 // Bound by memory for long calls and by its three dependent loads (starts, page, elements) for short
 // ones.  Measured (MI355X): 64 requests of 500 to 4000 tokens, 8 heads of 128, to fp16 115 us (656 MB, 5.7 TB/s); 300
-// tokens to bf16 4.7 (in a trace 3.5).  One token a thread with its place worked out by itself took 177 and 8.2.
+// tokens to bf16 4.7 (in a trace 3.5); the last blocks of 200 requests in a trace 5.4, where a search of its own for each
+// lane's run took 6.2.  One token a thread with its place worked out by itself took 177 and 8.2.
 #include "attn_rope.hpp"
 #include "attn_runs.hpp"
 
@@ -74,7 +75,24 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a, uint32_t bes
         uint32_t run = find_run(a.requests, (uint32_t)token0, start);
         if (run == a.requests) run = 0;  // the first run begins behind the first token
         const bool mine = tid < tokens && token < a.tokens;
-        if (mine && a.starts[run + 1] <= token)  // the lane's own is behind it
+        // where the run and the 63 behind it end, a lane each: the lane's token is in the first that ends past
+        // it; and the first tokens of the run and of those behind it, loaded beside
+        int32_t from = a.starts[run], first = a.first ? a.first[run] : 0;
+        const int32_t ends = a.starts[min(run + 1 + tid, a.requests)];
+        const int32_t firsts = a.first ? a.first[min(run + 1 + tid, a.requests - 1)] : 0;
+        uint32_t past = 0;  // runs that end before it
+#pragma unroll
+        for (uint32_t half = 32; half; half /= 2)
+            if (__shfl(ends, (int)(past + half - 1)) <= token) past += half;
+        const int behind = (int)max(past, 1u) - 1;
+        const int32_t other_from = __shfl(ends, behind), other_first = __shfl(firsts, behind);
+        int32_t to = __shfl(ends, (int)past);
+        if (past) {
+            from = other_from;
+            first = other_first;
+        }
+        run = min(run + past, a.requests - 1);
+        if (mine && to <= token && past == 63) {  // more runs than that
             for (uint32_t end = a.requests; end - run > 1;) {
                 const uint32_t mid = run + (end - run) / 2;
                 if (a.starts[mid] <= token)
@@ -82,10 +100,14 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a, uint32_t bes
                 else
                     end = mid;
             }
+            from = a.starts[run];
+            to = a.starts[run + 1];
+            first = a.first ? a.first[run] : 0;
+        }
         int64_t at = -2, scale = 0;
-        if (mine && token >= a.starts[run] && token < a.starts[run + 1]) {
+        if (mine && token >= from && token < to) {
             at = -1;
-            const int64_t pos = token - a.starts[run] + (a.first ? a.first[run] : 0);
+            const int64_t pos = token - from + first;
             if (pos >= 0 && pos < a.max_len) {
                 const uint32_t column = a.cache.page.div((uint32_t)pos), in_page = (uint32_t)pos - column * a.cache.page.d;
                 const int32_t page = a.tables[run * a.table_stride + column];
