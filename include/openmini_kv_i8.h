@@ -27,7 +27,8 @@ extern "C" {
  * (8, 16 or 32; page_size is a multiple of it) of one head.  The scale of block b of page p
  * and head h is element p * page_stride + b * block_stride + h * head_stride of d_k, and of
  * d_v alike.  No two scales share an element.  A scale is positive (0 stands for a block of
- * zeros); one that is NaN or infinite makes its whole block NaN. */
+ * zeros).  To attention a block whose scale is NaN or infinite is NaN as a whole;
+ * openmini_kv_read gives the products (under an infinite scale infinities, NaN for codes of 0). */
 #define OPENMINI_ATTN_I8 4
 
 typedef struct {
@@ -56,8 +57,8 @@ int openmini_rope_append_i8(const openmini_rope_t* rope, const openmini_kv_cache
 
 /* openmini_attn_decode on a cache of 8-bit integers, with the same workspace: products of
  * the codes, which are exact in 16 bits; the scales multiply fp32 scores and probabilities.  q is
- * F16 or BF16, out q's type or F32.  A block of keys whose scale is NaN makes the heads that
- * see it NaN, a block of values their outputs. */
+ * F16 or BF16, out q's type or F32.  A block of keys whose scale is NaN or infinite makes the
+ * heads that see it NaN, a block of values their outputs. */
 int openmini_attn_decode_i8(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales,
                             const openmini_attn_args_t* args, void* stream);
 
@@ -95,8 +96,8 @@ int openmini_kv_read(const openmini_kv_cache_t* cache, const openmini_kv_scales_
  *   s_i = scale * q . k_i,  out = sum_i softmax(s)_i v_i,  lse = log sum_i exp(s_i).
  * What openmini_attn_decode says of heads, of rows without keys, of pages outside the cache,
  * of infinite and NaN scores and values, and of what lies past a row's keys holds here too, but
- * an infinite value may make its dimension NaN, and a block of values whose scale is NaN
- * makes lse NaN too.  Rows of no request are left as they were.  d_starts does not decrease.
+ * an infinite value may make its dimension NaN, and a block of values whose scale is NaN or
+ * infinite makes lse NaN too.  Rows of no request are left as they were.  d_starts does not decrease.
  * Keys and values are read once for a tile of query tokens and heads, so a call of many rows
  * to a request takes the time of its products.
  *

@@ -501,7 +501,11 @@ __global__ __launch_bounds__(64 * W, D == 256 && E == kHalf ? 1 : 2) void decode
         bool whole = key0 >= cur.lo && key0 + (int32_t)kKeys - 24 <= cur.hi;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-            const float scale = E == kI8 ? a.scale * now.k_scale[u] : a.scale;
+            float scale = a.scale;
+            if constexpr (E == kI8) {  // of a scale that is not finite NaN: an infinite one would leave scores below zero no weight
+                const float k = now.k_scale[u];
+                scale = __builtin_fmaf(a.scale, k, k - k);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 x[u][j] = sc[u][j / 4][j % 4] * scale;

@@ -315,7 +315,7 @@ __global__ __launch_bounds__(64 * W, kPer) void prompt_kernel(PromptArgs a) {
         if (lane == 0) {
             f32x4 g = {a.scale, 0, 1, r.paged ? 1.0f : 0.0f};
             if constexpr (E == kI8) {
-                const float k = a.scale * r.k_scale, v = r.v_scale;
+                const float v = r.v_scale, k = __builtin_fmaf(a.scale, r.k_scale, r.k_scale - r.k_scale);  // of infinity NaN, as in decode attention
                 g[0] = k < 1e-37f ? 1e-37f : k;  // -inf times 0 is NaN
                 const float up = v < 8.673617379884035e-19f ? 8.673617379884035e-19f : v;  // 2^-60
                 g[1] = __builtin_amdgcn_logf(up);
