@@ -108,7 +108,8 @@ int openmini_kv_read(const openmini_kv_cache_t* cache, const openmini_kv_scales_
  * 2^-36 on.  With F32 outputs it enters as the sum of three bf16 parts, or on F16 caches as in
  * openmini_attn_decode.  Sums, maxima and lse are fp32.  head_dim: 64, 96, 128, 192 or 256;
  * page_size: a multiple of 8; q_heads: a multiple of kv_heads, at most 1024; requests: at most
- * 2^20.  A scale of 8-bit values below 2^-60 counts as 2^-60.
+ * 2^20.  A scale of 8-bit values below 2^-60 counts as 2^-60, one above 2^126 as infinite; those
+ * of a row's blocks are within 2^100 of each other (past that the keys of the least lose weight).
  *
  * Where the tiles are few for the chip, and the table long, several workgroups take parts
  * of a tile's keys and a second launch joins them in order: by the sizes of the call, so equal

@@ -1,4 +1,4 @@
-"""Scales of 8-bit caches at the ends of what they can be."""
+"""Scales of 8-bit caches at the ends of what they can be, and at ordinary sizes to a close bound."""
 import numpy as np
 import pytest
 
@@ -70,3 +70,39 @@ def test_prompts_over_an_infinite_scale_of_keys(qmm, codes, dim, q_t, held, new,
                 assert np.isnan(out[j, :2]).all() and np.isnan(got[1][j, :2]).all(), (j, np.isnan(out[j, :2]).sum(), got[1][j, :2])
                 assert np.isfinite(out[j, 2:]).all() and np.isfinite(got[1][j, 2:]).all(), j
             c.check(got, out_t, scale=scale, skip=set(seeing))
+
+
+@pytest.mark.parametrize("q_t", [BF16, F16])
+@pytest.mark.parametrize("power", [100, 120, 124, 126, 127])
+def test_prompts_over_large_scales_of_values(qmm, q_t, power):
+    """Values of -1 to 1 times 2^power, all of them finite in fp32: correct up to 2^126, NaN past that (the
+    scale's reciprocal is no normal number), never a number that is not the result."""
+    c = prompt.Case(qmm, [0, 50], [40, 20], 4, 2, 64, q_t, I8, seed=power)
+    p = c.c
+    p.bits[1][:] = p.rng.integers(-1, 2, p.bits[1].shape)
+    p.scales[1][np.isfinite(p.scales[1])] = 2.0 ** power
+    p.upload(qmm)
+    got = c.run(qmm, F32)
+    out, lse = ref.decode(got[0], F32), got[1].astype(np.float64)
+    for r, (first, n) in enumerate(c.runs):
+        keys, values = p.tokens(r, range(max(c.lens[first:first + n])))
+        for j in range(first, first + n):
+            o, l, size, dots = ref.attention(c.q[j], keys[:c.lens[j]], values[:c.lens[j]], 0.125)
+            d, e = prompt.bounds(o, size, dots, 2.0 ** power, 64, q_t, I8, F32, c.lens[j])
+            if power <= 126:
+                assert np.all(np.abs(out[j] - o) <= d) and np.all(np.abs(lse[j] - l) <= e + 2.0 ** -22 * np.abs(l)), j
+            else:
+                assert np.isnan(out[j]).all() and np.isnan(lse[j]).all(), j
+
+
+@pytest.mark.parametrize("low,high", [(-60, 40), (-40, 30), (-40, 60)])
+def test_prompts_over_scales_of_values_far_apart(qmm, low, high):
+    """Up to 2^100: the keys of the least scales keep their weight among the others'."""
+    for q_t, out_t in ((BF16, F32), (F16, F16), (BF16, BF16)):
+        c = prompt.Case(qmm, [0, 90], [64, 30], 4, 2, 64, q_t, I8, seed=high, q_size=0.05)
+        p = c.c
+        for r in range(2):  # fp16 outputs: no more than they hold
+            p.scales[1][p.tables[r, 0], 0] = 2.0 ** low
+            p.scales[1][p.tables[r, 1:3], 0] = 2.0 ** (high if out_t != F16 else 5)
+        p.upload(qmm)
+        c.check(c.run(qmm, out_t), out_t)
