@@ -51,7 +51,8 @@ typedef struct {
  * So all roundings of an element add up to at most 2.5 s', whatever the order in which a
  * block fills.  An element that is NaN or infinite makes s' NaN, until a call starts the block
  * with first = 0.  head_dim is at most 256.  One call at a time writes a block: two requests that share a block which
- * is not full each need a copy of it before they go on. */
+ * is not full each need a copy of it before they go on.  Keys and values share no element, nor do their scales, nor
+ * two slots; interleaved in one array they may be. */
 int openmini_rope_append_i8(const openmini_rope_t* rope, const openmini_kv_cache_t* cache,
                             const openmini_kv_scales_t* scales, const openmini_rope_append_args_t* args, void* stream);
 

@@ -8,6 +8,7 @@
 #include <utility>
 
 #include "attn_internal.hpp"
+#include "attn_overlap.hpp"
 
 struct openmini_rope {
     attn::Rope r;
@@ -79,6 +80,18 @@ inline bool shares_memory(const void* p, int64_t count, const void* q, int64_t r
     const int64_t r = from < 0 ? 0 : from / stride;  // the row that begins at `from` or before it
     return from < r * stride + row || (r + 1 < rows && to > (r + 1) * stride);
 }
+
+// Bytes of a cache's keys (values), and of the scales of its keys (values).
+inline Box<4> cache_bytes(const openmini_kv_cache_t* c, int size) {
+    const Axis axes[] = {{1, (int64_t)c->head_dim * size}, {c->head_stride * size, c->kv_heads}, {c->token_stride * size, c->page_size},
+                         {c->page_stride * size, c->n_pages}};
+    return Box<4>(axes);
+}
+inline Box<4> scale_bytes(const openmini_kv_cache_t* c, const openmini_kv_scales_t* s) {
+    const Axis axes[] = {{1, 4}, {s->head_stride * 4, c->kv_heads}, {s->block_stride * 4, c->page_size / s->block}, {s->page_stride * 4, c->n_pages}};
+    return Box<4>(axes);
+}
+inline int64_t bytes_apart(const void* p, const void* q) { return (int64_t)((uintptr_t)p - (uintptr_t)q); }
 
 inline bool dense_type(int t) { return t == OPENMINI_ATTN_F32 || t == OPENMINI_ATTN_F16 || t == OPENMINI_ATTN_BF16; }
 inline bool half_type(int t) { return t == OPENMINI_ATTN_F16 || t == OPENMINI_ATTN_BF16; }

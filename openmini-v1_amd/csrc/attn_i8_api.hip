@@ -23,9 +23,19 @@ extern "C" {
 int openmini_rope_append_i8(const openmini_rope_t* rope, const openmini_kv_cache_t* cache,
                             const openmini_kv_scales_t* scales, const openmini_rope_append_args_t* p, void* stream) {
     if (!p) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null arguments");
-    TRY(check_rope(rope));
+    if (!rope) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "null rope handle");
     AppendI8Args a = {};
     TRY(check_cache_i8(cache, scales, &a.r.cache, &a.scales));
+    // Keys and values are written by workgroups of their own, at their own time.
+    const Box<4> codes = cache_bytes(cache, 1), of_blocks = scale_bytes(cache, scales);
+    if (!codes.nested)
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "cache strides %lld, %lld, %lld: two slots share memory", (long long)cache->page_stride,
+                    (long long)cache->token_stride, (long long)cache->head_stride);
+    if (codes.meets_itself(bytes_apart(cache->d_v, cache->d_k)))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "the cache's d_k and d_v share memory");
+    if (of_blocks.meets_itself(bytes_apart(scales->d_v, scales->d_k)))
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "the scales' d_k and d_v share memory");
+    TRY(check_rope(rope));
     TRY(check_append(rope, cache, p));
     if (cache->head_dim > kMaxI8Dim)
         return fail(OPENMINI_QMM_ERR_UNSUPPORTED, "head_dim = %d on a cache of 8-bit integers: at most %d", cache->head_dim, kMaxI8Dim);
