@@ -70,7 +70,9 @@ int openmini_attn_decode_i8(const openmini_kv_cache_t* cache, const openmini_kv_
  * BF16), each rounded once; `k_stride` (`v_stride`) elements from a row to the next.  A token
  * past the table, before 0 or on a page outside the cache reads as zeros.  Rows of no request are
  * left as they were, and so are those from `tokens` on.  d_starts does not decrease.  Either
- * output may be NULL.  Caches of every type; `scales` is NULL but for 8-bit integers.
+ * output may be NULL; rows of both may take turns in one array (of one stride), but an output, from its
+ * first row to its last, shares no memory with what the call reads.  Caches of every type; `scales` is NULL
+ * but for 8-bit integers.
  * head_dim: a multiple of 8, at most 512; tokens: at most 2^26; requests: at most 2^20. */
 typedef struct {
     const int32_t* d_tables;

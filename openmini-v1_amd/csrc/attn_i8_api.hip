@@ -8,6 +8,7 @@ namespace {
 
 constexpr int64_t kMaxRuns = (int64_t)1 << 20;
 constexpr int64_t kMaxThreads = (int64_t)UINT32_MAX;  // of a launch
+constexpr int64_t kMaxI64 = INT64_MAX;
 
 bool prompt_sizes(int q_heads, int kv_heads, int head_dim) {
     return kv_heads >= 1 && q_heads >= kv_heads && q_heads <= 1024 && q_heads % kv_heads == 0 && decode_dim(head_dim);
@@ -15,6 +16,49 @@ bool prompt_sizes(int q_heads, int kv_heads, int head_dim) {
 
 // The workspace: the parts' maxima and sums, then their accumulators.
 size_t ml_bytes(int head_dim) { return (size_t)kPromptParts * prompt_rows(head_dim) * 8; }
+
+// Workgroups read at their own time what others may have written already: an output, from its first
+// row to its last, shares nothing with what the call reads, nor its rows with the other's.
+int check_read_memory(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales, const openmini_kv_read_args_t* p, int size,
+                      int64_t row_bytes) {
+    const Box<4> elements = cache_bytes(cache, size_of(cache->dtype));
+    struct {
+        const void* at;
+        int64_t stride;
+    } out[] = {{p->d_k_out, p->k_stride * size}, {p->d_v_out, p->v_stride * size}};
+    const struct {
+        const char* name;
+        const void* at;
+        int64_t bytes;
+    } in[] = {{"d_tables", p->d_tables, 4 * ((p->requests - 1) * p->table_stride + p->max_pages)},
+              {"d_starts", p->d_starts, 4 * (p->requests + 1)},
+              {"d_first", p->d_first, 4 * p->requests}};
+    int64_t bytes[2];
+    for (int i = 0; i < 2; ++i) {
+        // saturated: no memory is as large
+        bytes[i] = p->tokens - 1 > kMaxI64 / 4 / out[i].stride ? kMaxI64 / 4 : (p->tokens - 1) * out[i].stride + row_bytes;
+        if (!out[i].at) continue;
+        const char* with = nullptr;
+        for (const auto& x : in)
+            if (x.at && bytes_apart(out[i].at, x.at) < x.bytes && bytes_apart(x.at, out[i].at) < bytes[i]) with = x.name;
+        for (const void* at : {cache->d_k, cache->d_v}) {
+            const int64_t from = bytes_apart(out[i].at, at);
+            if (elements.meets(from, from + bytes[i])) with = "the cache";
+        }
+        if (scales)
+            for (const void* at : {scales->d_k, scales->d_v}) {
+                const int64_t from = bytes_apart(out[i].at, at);
+                if (scale_bytes(cache, scales).meets(from, from + bytes[i])) with = "the scales";
+            }
+        if (with) return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "%s and %s share memory", i ? "d_v_out" : "d_k_out", with);
+    }
+    if (!out[0].at || !out[1].at) return OPENMINI_QMM_OK;
+    const int64_t apart = bytes_apart(out[1].at, out[0].at);
+    const Axis axes[] = {{1, row_bytes}, {out[0].stride, p->tokens}};
+    if (out[0].stride == out[1].stride ? Box<2>(axes).meets_itself(apart) : apart < bytes[0] && -apart < bytes[1])
+        return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "d_k_out and d_v_out share memory");
+    return OPENMINI_QMM_OK;
+}
 
 }  // namespace
 
@@ -77,6 +121,7 @@ int openmini_kv_read(const openmini_kv_cache_t* cache, const openmini_kv_scales_
     for (const void* out : {p->d_k_out, p->d_v_out})
         if (out && (out == cache->d_k || out == cache->d_v))
             return fail(OPENMINI_QMM_ERR_INVALID_PARAM, "an output is the cache");
+    TRY(check_read_memory(cache, scales, p, size, row * size));
     TRY(qmm::current_device(nullptr));
     const int64_t held = p->max_pages * cache->page_size;
     a.tables = p->d_tables;

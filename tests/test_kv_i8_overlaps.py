@@ -63,6 +63,41 @@ def test_writes_beside_each_other(cache, scales):
     _taken(_append(_cache(**cache), _scales(**scales)))
 
 
+def _read(**kw):
+    a = dict(d_tables=5 * M, table_stride=4, max_pages=4, requests=2, d_starts=6 * M, d_first=7 * M, tokens=5, d_k_out=8 * M, d_v_out=9 * M,
+             k_stride=256, v_stride=256, out_dtype=DType.BF16)
+    a.update(kw)
+    return _native.KvReadArgs(**a)
+
+
+ROWS = 5 * 512  # bytes of an output's rows
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(d_k_out=M + 16), "the cache"), (dict(d_v_out=M + 4 * 4096 - 16), "the cache"), (dict(d_k_out=2 * M - ROWS + 16), "the cache"),
+    (dict(d_k_out=None, d_v_out=2 * M + 4096), "the cache"), (dict(d_v_out=3 * M), "the scales"), (dict(d_k_out=4 * M + 48), "the scales"),
+    (dict(d_k_out=5 * M), "d_tables"), (dict(d_k_out=5 * M - ROWS + 16), "d_tables"), (dict(d_v_out=5 * M + 16), "d_tables"), (dict(d_v_out=6 * M), "d_starts"),
+    (dict(d_k_out=7 * M), "d_first"), (dict(d_v_out=8 * M + 16), "d_k_out and d_v_out"), (dict(d_v_out=8 * M - ROWS + 16), "d_k_out and d_v_out"),
+    (dict(d_v_out=8 * M + 512 - 16, k_stride=512, v_stride=512), "d_k_out and d_v_out"),
+    (dict(d_v_out=8 * M + 512, k_stride=512, v_stride=768), "d_k_out and d_v_out"),
+    (dict(d_k_out=M - (1 << 19), k_stride=1 << 19), "share memory"), (dict(d_k_out=16, k_stride=1 << 40, tokens=1 << 26), "share memory")])
+def test_reads_over_what_they_read(kw, word):
+    _refused(_native.lib().openmini_kv_read(_cache(), _scales(), _read(**kw), None), BAD, word)
+
+
+@pytest.mark.parametrize("cache,kw", [
+    ({}, {}), ({}, dict(d_k_out=M - ROWS)), ({}, dict(d_k_out=M + 4 * 4096)), ({}, dict(d_v_out=3 * M + 64)), ({}, dict(d_v_out=5 * M + 32)),
+    ({}, dict(d_v_out=8 * M + ROWS)), ({}, dict(d_v_out=8 * M + 512, k_stride=512, v_stride=512)), ({}, dict(d_first=None, d_k_out=7 * M)),
+    # a layer's pages between those of others: an output in another layer's part
+    (dict(page_stride=1 << 17), dict(d_k_out=M + 4096)), (dict(page_stride=1 << 17), dict(d_k_out=M + (1 << 17) - ROWS))])
+def test_reads_beside_what_they_read(cache, kw):
+    """What stops the call is that this machine has no GPU."""
+    if _native.lib().openmini_qmm_is_available():
+        pytest.skip("the pointers are not memory")
+    rc = _native.lib().openmini_kv_read(_cache(**cache), _scales(), _read(**kw), None)
+    assert rc == _native.ERR_HIP, (rc, _native.last_error())
+
+
 BOXES = r"""
 #include <cstdio>
 #include <random>
