@@ -106,3 +106,50 @@ def test_prompts_over_scales_of_values_far_apart(qmm, low, high):
             p.scales[1][p.tables[r, 1:3], 0] = 2.0 ** (high if out_t != F16 else 5)
         p.upload(qmm)
         c.check(c.run(qmm, out_t), out_t)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_t", [BF16, F16])
+def test_prompts_over_two_blocks(qmm, dim, q_t):
+    """Rows that see two blocks of 16 keys, scores of 0, all keys of a block alike, value scales of 2^-8
+    to 2^-3, outputs of 32 bits: what the scales' way through the exponent costs, and next to nothing
+    else (sums of 16 equal products are exact, and three bf16 parts leave 2^-24).  In units of 2^-24: a
+    base-2 logarithm of less than 8, off by at most one unit in its last place, 8, two of them; their
+    difference, of less than 8, by half of one, 4: an exponent is off by 20, a probability by 20 log 2
+    = 14 and the exponential's 2.  A sum of probabilities by as much and the reciprocals' 2; one of each
+    for its addition, the division and the product, 3.  16 + 18 + 3 and 1 for the parts: 38 of sum p |v|.
+    lse: 18, and 3 numbers of less than 16 added, 8 each."""
+    rng, n, kv_heads = np.random.default_rng(dim + q_t), 60, 8
+    c = prompt.Case(qmm, [30] * n, [2] * n, kv_heads, kv_heads, dim, q_t, I8, lens=[32] * (2 * n), seed=dim, q_size=0.0)
+    p = c.c
+    for r in range(n):
+        for b in range(2):
+            page = p.tables[r, b]
+            p.scales[1][page, 0] = (2.0 ** rng.uniform(-8, -3, kv_heads)).astype(np.float32)
+            p.bits[1][page] = rng.integers(-127, 128, (kv_heads, dim))
+    p.upload(qmm)
+    got = c.run(qmm, F32)
+    out, lse = ref.decode(got[0], F32), got[1].astype(np.float64)
+    worst = 0.0
+    for r in range(n):
+        a, b = (p.bits[1][page, 0].astype(np.float64) * p.scales[1][page, 0].astype(np.float64)[:, None] for page in p.tables[r, :2])
+        o, tol = (a + b) / 2, 38 * 2.0 ** -24 * (np.abs(a) + np.abs(b)) / 2
+        for j in (2 * r, 2 * r + 1):
+            assert np.all(np.abs(out[j] - o) <= tol), (j, float(np.max(np.abs(out[j] - o) / np.maximum(tol, 2.0 ** -60))))
+            assert np.all(np.abs(lse[j] - np.log(32)) <= 42 * 2.0 ** -24), (j, lse[j] - np.log(32))
+            worst = max(worst, float(np.max(np.abs(out[j] - o) / np.maximum(tol, 2.0 ** -60))))
+    print(f"prompts over two blocks: at most {worst:.2f} of the bound", flush=True)
+
+
+def test_equal_prompts_give_equal_bits(qmm):
+    """A tile to a workgroup, and workgroups that share tiles: the same bits call after call, on
+    whatever the workspace holds."""
+    for held, new, heads, kv_heads, dim, q_t, c_t, out_t in (([0], [211], 64, 8, 128, BF16, I8, BF16), ([0], [1500], 16, 2, 128, BF16, I8, BF16),
+                                                             ([900, 300, 30], [300, 120, 5], 32, 8, 64, F16, F16, F32)):
+        c = prompt.Case(qmm, held, new, heads, kv_heads, dim, q_t, c_t, seed=dim)
+        attn = qmm.PromptAttention(heads, kv_heads, dim, q_t, out_t)
+        first = c.run(qmm, out_t, attn=attn)
+        for fill in (0, 0x7F, 0xFF, 0x3C):
+            attn.work.fill(fill)
+            got = c.run(qmm, out_t, attn=attn)
+            assert np.array_equal(got[0], first[0]) and np.array_equal(got[1].view(np.uint32), first[1].view(np.uint32)), fill
