@@ -119,7 +119,9 @@ int decode(const openmini_kv_cache_t* cache, const openmini_kv_scales_t* scales,
     // a window's first tile need not begin with it
     const int64_t most = (keys + tile - 1) / tile + (keys < max_len), pairs = p->rows * cache->kv_heads * head_tiles;
     a.whole = attn::decode_whole(most, pairs);
-    a.uncut = attn::decode_uncut_of(most, p->rows, (int64_t)cache->kv_heads * head_tiles, shares, sub, cache->head_dim * (f8 ? 1 : 2));
+    const int64_t units = (int64_t)cache->kv_heads * head_tiles;
+    a.uncut = i8 ? attn::decode_uncut_i8(most, p->rows, units, shares, cache->head_dim)
+                 : attn::decode_uncut(most, p->rows, units, shares, cache->head_dim, f8);
     if (a.uncut) a.launch_shares = p->rows < (int64_t)shares ? (uint32_t)p->rows : shares;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool bf16 = p->q_dtype == OPENMINI_ATTN_BF16;

@@ -31,7 +31,9 @@ constexpr int kRound = 1024;
 // 7.0 / 9.4, of 700 9.8 / 10.7, of 1000 12.5 / 10.9; 64 pairs of 1000 13.5 / 16.2, of 2000
 // 22.6 / 18.5; 256 of up to 4000, heads of 64, 46.8 / 36.4; 512 of 400 15.1 / 20.4; 1024 of
 // 200, e4m3, 16.6 / 16.3, of 60 14.3 / 9.5.  8-bit integers, heads of 128: 8 pairs of 500 keys 8.1 / 10.5, of
-// 700 9.8 / 10.5, 64 of 1000 12.1 / 14.1, of 2000 19.4 / 17.5, 512 of 1000 28.4 / 28.4.
+// 700 9.8 / 10.5, 64 of 1000 12.1 / 14.1, of 2000 19.4 / 17.5, 512 of 1000 28.4 / 28.4.  Between 16 tiles and
+// 32 the limit for few pairs is on the safe side: at 22 (700 keys) whole rows would still be .7 to .9 us
+// faster, at 32 they are 1.6 slower.
 inline bool decode_whole(int64_t most, int64_t pairs) {
     return most == 1 ? pairs <= 256 : pairs <= 512 && most <= (pairs < 64 ? 16 : 32);
 }
@@ -64,6 +66,9 @@ inline bool decode_uncut_of(int64_t most, int64_t rows, int64_t units, int64_t s
 }
 inline bool decode_uncut(int64_t most, int64_t rows, int64_t units, int64_t shares, int head_dim, bool f8) {
     return decode_uncut_of(most, rows, units, shares, decode_subtiles(head_dim, f8), head_dim * (f8 ? 1 : 2));
+}
+inline bool decode_uncut_i8(int64_t most, int64_t rows, int64_t units, int64_t shares, int head_dim) {
+    return decode_uncut_of(most, rows, units, shares, decode_subtiles_i8(head_dim), head_dim);
 }
 
 }  // namespace attn
