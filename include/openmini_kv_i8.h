@@ -44,10 +44,11 @@ typedef struct {
  * each other in the arrays, their slots one apart (as openmini_kv_plan lays them out; if they
  * do not, what the block holds afterwards is unspecified).  With `first` the place of the
  * first of them in the block, the tokens before it are held already and those behind it are
- * not.  For a block and head, a = max |x| of its new elements (k after its turn):
- *   n = max(a / 127, 2^-40)
- *   s' = n where first = 0; else the old s where s >= n; else max(n, 1.25 s)
- *   new codes: x / s' rounded to the nearest even;  held codes c: c (s / s') likewise.
+ * not.  For a block and head, a = max |x| of its new elements (k after its turn), and in fp32, each
+ * operation rounded (1/127 is one number, and so is 1 / s', which elements are multiplied by):
+ *   n = max(a * (1/127), 2^-40)
+ *   s' = n where first = 0; else the old s where s >= n; else max(n, 1.25 * s)
+ *   new codes: x * (1 / s') rounded to the nearest even;  held codes c: c * (s / s') likewise.
  * So all roundings of an element add up to at most 2.5 s', whatever the order in which a
  * block fills.  An element that is NaN or infinite makes s' NaN, until a call starts the block
  * with first = 0.  head_dim is at most 256.  One call at a time writes a block: two requests that share a block which
