@@ -23,8 +23,11 @@
 //
 // Bound by memory once the loads of the next head are on their way before a head's barrier and the
 // registers of k's and v's own instances are few enough for five workgroups a CU (both in one: three).
-// Measured (MI355X, one launch): 8191 tokens of 32 heads of 128, float in, q in fp16, 106 us (538 MB, 5.1
-// TB/s; 167 before); 200 requests' tokens of 64 and 8 heads 6.4 us; one token 4.3 us.
+// Measured (MI355X, one launch): 8191 tokens of 32 heads of 128, q in fp16, float in 104 us (538 MB, 5.1
+// TB/s), fp16 or bf16 in 119 (336 MB, 2.8); 200 requests' tokens of 64 and 8 heads 6.3 us, one token 4.5, where no block
+// grows.  Growing blocks are a thread's loop of a load, a wait and a store for each held token: one token
+// behind 8, 15 and 31 held ones 7.4, 12 and 15 us; 200 requests of which a quarter of the heads' blocks grow
+// 15 us in blocks of 16, 41 in blocks of 32 (all of them: 17, 43).  Prompts do not show it (103).
 #include "attn_rope.hpp"
 
 namespace attn {

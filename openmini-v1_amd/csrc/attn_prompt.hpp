@@ -15,20 +15,24 @@
 // transposes them by byte permutations on the way.
 //
 // 8-bit integers are exact in 16 bits; their blocks' scales act on 32-bit numbers: a key's on
-// the score, a value's as its logarithm in the exponent, so that p v_scale is what is rounded
-// to 16 bits (at most 1, whatever the scales) and l adds p v_scale / v_scale.
+// the score, a value's as its logarithm in the exponent, so that p v_scale against the row's base is what
+// is rounded to 16 bits (at most 2^15 in fp16 and 2^8 in bf16 parts, whatever the scales) and l adds p
+// v_scale / v_scale.  The logarithm and its sum are off by up to 2^-20 for scales near 2^-5 (measured: 2^-21
+// of sum p |v|), 2^-17 near 2^-60.
 //
 // The loads of a step are issued more than a step ahead of their use and its page three (heads of 192 and 256: a
 // step and two, with another workgroup on the CU); two buffers, one barrier a step.  What comes goes to LDS beside the matrix instructions of the first product.
-// Accumulators are scaled only where a maximum has grown by 2^4: with 32 rows to a wave one of them
-// grows in most steps.
+// Accumulators are scaled only where a maximum has passed its base by 2^8 (bf16 parts), 2^4 (one fp16
+// part) or at all (two fp16 parts and what they leave): with 32 rows to a wave one of them grows in most steps.
 //
 // Bound by the issue of instructions: a step of 64 keys takes a wave 2 us, alone on its SIMD or with
 // another, of which the matrix unit is busy for .4 (heads of 128); matrix and vector instructions of
-// the two waves run at the same time for two fifths of that only.  Measured (MI355X): 8191 tokens of
-// 64 / 8 heads of 128 1150 to 1215 us, 905 to 956 TFLOP/s (a large product of the library 1350); 4096
-// tokens of 32 / 8 heads of 64, 96, 128, 192, 256 150, 163, 169, 304, 357 us, on a bf16 cache of 128 172; 211 tokens of
-// 64 / 8 heads of 128 13.4; 815 tokens in six pieces behind up to 1659 keys, 32 / 8 heads of 64 in fp16, fp32 out, 38.
+// the two waves run at the same time for two fifths of that only.  Measured (MI355X, us, calls in a row once
+// clocks have settled; the first twenty on an idle card take up to a third more): 8191 tokens of 64 / 8 heads of
+// 128 1165 to 1240, 885 to 945 TFLOP/s (a large product of the library 1350); 4096 tokens of 32 / 8 heads of 64, 96,
+// 128, 192, 256 142, 159, 162, 283, 364, of 128 on a bf16, fp16, e4m3 cache 169, 176, 168 (so conversions are not what
+// binds), with fp32 out on 8-bit integers, bf16, fp16 254, 267, 248; 211 tokens of 64 / 8 heads of 128 13.6; 815 tokens
+// in six pieces behind up to 1659 keys, 32 / 8 heads of 64 in fp16, fp32 out, 38.
 // What gave nothing or less: a second product a step later, for
 // half of the waves or among the exponentials (1.24, 1.47 ms of 1.26), wave priorities, 128 keys
 // a step, three waves a SIMD of 32 keys a step (1.31 of 1.18), rows out through LDS.
@@ -95,7 +99,10 @@ __device__ __forceinline__ PromptTile prompt_tile(const int32_t* starts, uint32_
 template <int D, class T, Elem E, bool kF32, int W, int kPer>
 __global__ __launch_bounds__(64 * W, kPer) void prompt_kernel(PromptArgs a) {
     // of the second product: byte caches fit both types, fp16 has the finer step and bf16 the
-    // range that exact parts need
+    // range that exact parts need.  16-bit outputs take one part of a probability, off by as much as their
+    // own rounding: rms against 64 bits, relative, with one part and with all, fp16 on 8-bit integers 2.4e-4 /
+    // 2.1e-4, on fp16 2.5e-4 / 2.0e-4, bf16 on 8-bit integers 1.7e-3 / 1.7e-3, on bf16 2.0e-3 / 1.6e-3; 4096
+    // tokens of 32 heads 162 / 254 us
     using P = std::conditional_t<E == kHalf, T, std::conditional_t<kF32, BF16, F16>>;
     constexpr int kParts = kF32 ? P::kExactParts : 1;
     constexpr bool kLow = kF32 && P::kNarrow;  // as in decode attention: what two fp16 parts leave

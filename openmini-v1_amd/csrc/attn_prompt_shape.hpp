@@ -45,6 +45,8 @@ inline PromptShape prompt_tiles(int waves, int64_t rows, int64_t requests, int k
 // Measured (MI355X, us, four waves and eight): 200 tokens of 64 heads of 128 13.6 / 14.9, 3200 keys 97 /
 // 104; a round of pairs of 66 steps 184, of eight waves 121.  64 tokens behind 8000 keys in 1, 4, 8, 16
 // splits 251, 78, 51, 59; 512 behind 30000 in 2 and 3 530 and 690.
+// Heads of 256 on fp16 caches with fp32 outputs have a CU each however many they are; the cost of more than
+// prompt_alone counts them as the others.  The host's search takes up to 11 us (one tile over 131072 keys).
 // Of several requests a tile each is taken to be half full; a round that this estimate fills to
 // within 6 % is full or over in about half of the calls.
 inline double prompt_cost(const PromptShape& p, int head_dim, int64_t rows, int64_t requests, int64_t steps, int64_t splits) {

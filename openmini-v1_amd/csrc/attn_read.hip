@@ -5,7 +5,8 @@
 // the first is used.  A wave finds the tokens' places, a lane each, and leaves them in LDS.
 //
 // Bound by memory for long calls and by its three dependent loads (starts, page, elements) for short
-// ones.  Measured (MI355X): 64 requests of 500 to 4000 tokens, 8 heads of 128, to fp16 115 us (656 MB, 5.7 TB/s); 300
+// ones.  Measured (MI355X): 64 requests of 500 to 4000 tokens, 8 heads of 128, to fp16 113 us (656 MB, 5.8 TB/s),
+// 16-bit and e4m3 caches to 16 bits at 5.8 and 5.7 TB/s, to fp32 348 us (1005 MB, 2.9 TB/s; of 16-bit caches 3.6); 300
 // tokens to bf16 4.7 (in a trace 3.5); the last blocks of 200 requests in a trace 5.4, where a search of its own for each
 // lane's run took 6.2.  One token a thread with its place worked out by itself took 177 and 8.2.
 #include "attn_rope.hpp"
