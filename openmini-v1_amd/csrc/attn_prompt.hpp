@@ -325,7 +325,7 @@ __global__ __launch_bounds__(64 * W, kPer) void prompt_kernel(PromptArgs a) {
                 const float v = r.v_scale, k = __builtin_fmaf(a.scale, r.k_scale, r.k_scale - r.k_scale);  // of infinity NaN, as in decode attention
                 g[0] = k < 1e-37f ? 1e-37f : k;  // -inf times 0 is NaN
                 const float up = v < 8.673617379884035e-19f ? 8.673617379884035e-19f : v;  // 2^-60
-                g[1] = up <= 0x1p126f ? __builtin_amdgcn_logf(up) : __uint_as_float(0x7FC00000u);  // past it the reciprocal is 0
+                g[1] = fabsf(v) <= 0x1p126f ? __builtin_amdgcn_logf(up) : __uint_as_float(0x7FC00000u);  // past it the reciprocal is 0
                 g[2] = __builtin_amdgcn_rcpf(up);  // within 2^-23
             }
             group_lds[buf][group] = g;

@@ -72,6 +72,24 @@ def test_prompts_over_an_infinite_scale_of_keys(qmm, codes, dim, q_t, held, new,
             c.check(got, out_t, scale=scale, skip=set(seeing))
 
 
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_scales_of_values_that_are_not_finite(qmm, bad):
+    """The heads that see the block are NaN, in decode and in prompt attention alike; rows before it and
+    the other heads are as ever."""
+    for q_t, out_t in ((BF16, F32), (F16, F16)):
+        d = decode.Case(qmm, [100], 4, 2, 64, q_t, reqs=[0, 0, 0], row_lens=[100, 33, 32], seed=3)
+        c = prompt.Case(qmm, [20], [40], 4, 2, 64, q_t, I8, seed=4)
+        for case in (d, c):
+            p = case.c
+            p.scales[1][p.tables[0, 2], 0, 0] = bad  # values 32 to 47
+            p.upload(qmm)
+            seeing = [j for j, n in enumerate((d.row_lens if case is d else c.lens[:40])) if n > 32]
+            got = case.run(qmm, out_t)
+            out = ref.decode(got[0], out_t)
+            assert seeing and np.isnan(out[seeing, :2]).all() and np.isfinite(out[seeing, 2:]).all(), (case is d, np.isnan(out[seeing, :2]).sum())
+            case.check(got, out_t, skip=set(seeing))
+
+
 @pytest.mark.parametrize("q_t", [BF16, F16])
 @pytest.mark.parametrize("power", [100, 120, 124, 126, 127])
 def test_prompts_over_large_scales_of_values(qmm, q_t, power):
