@@ -33,11 +33,11 @@ int check_read_memory(const openmini_kv_cache_t* cache, const openmini_kv_scales
     } in[] = {{"d_tables", p->d_tables, 4 * ((p->requests - 1) * p->table_stride + p->max_pages)},
               {"d_starts", p->d_starts, 4 * (p->requests + 1)},
               {"d_first", p->d_first, 4 * p->requests}};
-    int64_t bytes[2];
+    int64_t bytes[2] = {0, 0};
     for (int i = 0; i < 2; ++i) {
+        if (!out[i].at) continue;  // nor is its stride looked at
         // saturated: no memory is as large
         bytes[i] = p->tokens - 1 > kMaxI64 / 4 / out[i].stride ? kMaxI64 / 4 : (p->tokens - 1) * out[i].stride + row_bytes;
-        if (!out[i].at) continue;
         const char* with = nullptr;
         for (const auto& x : in)
             if (x.at && bytes_apart(out[i].at, x.at) < x.bytes && bytes_apart(x.at, out[i].at) < bytes[i]) with = x.name;

@@ -87,7 +87,7 @@ def test_reads_over_what_they_read(kw, word):
 
 @pytest.mark.parametrize("cache,kw", [
     ({}, {}), ({}, dict(d_k_out=M - ROWS)), ({}, dict(d_k_out=M + 4 * 4096)), ({}, dict(d_v_out=3 * M + 64)), ({}, dict(d_v_out=5 * M + 32)),
-    ({}, dict(d_v_out=8 * M + ROWS)), ({}, dict(d_v_out=8 * M + 512, k_stride=512, v_stride=512)), ({}, dict(d_first=None, d_k_out=7 * M)),
+    ({}, dict(d_k_out=None, k_stride=0)), ({}, dict(d_v_out=None, v_stride=0)), ({}, dict(d_v_out=8 * M + ROWS)), ({}, dict(d_v_out=8 * M + 512, k_stride=512, v_stride=512)), ({}, dict(d_first=None, d_k_out=7 * M)),
     # a layer's pages between those of others: an output in another layer's part
     (dict(page_stride=1 << 17), dict(d_k_out=M + 4096)), (dict(page_stride=1 << 17), dict(d_k_out=M + (1 << 17) - ROWS))])
 def test_reads_beside_what_they_read(cache, kw):
